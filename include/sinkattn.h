@@ -128,6 +128,42 @@ SA_API int sa_sink_dynamic_attn_fwd(
     cudaStream_t stream);
 
 /*
+ * Backward of sa_bsattn_fwd: dq, dk, dv from dout, recomputing the
+ * probabilities from q, k and the forward pass's log-sum-exp.
+ * Replaces: the backward pass of the external block_sparse_attn_func, which
+ *   the reference imports at sinkattention/sparse_attention.py:22-28 and calls
+ *   for inference only.
+ *   P = exp(scale q k^T - lse) on kept blocks, dP = dout v^T,
+ *   delta = sum_d dout * out - dlse, dS = P * (dP - delta),
+ *   dq = scale dS k, dk = scale dS^T q, dv = P^T dout.
+ * q, dout, out, dq [B,H,Sq,128], k, v, dk, dv [B,H,Sk,128]: bf16, strides as
+ *   for sa_bsattn_fwd, each with its own. out and lse (fp32 [B,H,Sq]
+ *   contiguous) are what sa_bsattn_fwd gave for the same q, k, v, mask and
+ *   scale. dlse: nullable fp32 [B,H,Sq] contiguous, the gradient with respect
+ *   to lse. dq, dk and dv are written whole: rows whose mask row (key blocks
+ *   whose mask column) keeps nothing get 0, whatever their lse and dout hold.
+ * block_mask, m_strides, Hm, head_mask_type, softmax_scale, status: as for
+ *   sa_bsattn_fwd. Sq, Sk <= 131072. P and dS enter their products as bf16;
+ *   the sums, dP and the row statistics are fp32.
+ * Every sum is formed by one CTA in block order (no atomics on data), so equal
+ *   calls give equal bits.
+ * workspace: sa_bsattn_bwd_workspace_size(B, H, Sq, Sk) bytes, 256-byte
+ *   aligned, with any contents. Calls sharing one workspace must not overlap
+ *   on the GPU.
+ */
+SA_API size_t sa_bsattn_bwd_workspace_size(int B, int H, int Sq, int Sk);
+SA_API int sa_bsattn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                         const void* out, const int64_t do_strides[4],
+                         const int64_t q_strides[4], const int64_t k_strides[4],
+                         const int64_t v_strides[4], const int64_t o_strides[4],
+                         const float* lse, const float* dlse, int B, int H, int Sq, int Sk, int D,
+                         const uint8_t* block_mask, const int64_t m_strides[4], int Hm,
+                         const int32_t* head_mask_type, float softmax_scale, void* dq, void* dk,
+                         void* dv, const int64_t dq_strides[4], const int64_t dk_strides[4],
+                         const int64_t dv_strides[4], void* workspace, size_t ws_bytes,
+                         int32_t* status, cudaStream_t stream);
+
+/*
  * Scratch bytes sa_pool_scores needs: the work counters and flags of the
  * fused kernel (128 * (H + 5) bytes rounded up to 256, then 8 bytes per
  * group of 16 block rows of every head, rounded up to 256), then pooled Q

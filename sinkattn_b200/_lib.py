@@ -53,6 +53,12 @@ _SIGNATURES = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp,
          _i, _f, _f, _vp, _vp, _vp, _vp, _vp],
     ),
+    "sa_bsattn_bwd_workspace_size": (ctypes.c_size_t, [_i, _i, _i, _i]),
+    "sa_bsattn_bwd": (
+        _i,
+        [_vp] * 12 + [_i] * 5 + [_vp, _vp, _i, _vp, _f] + [_vp] * 7
+        + [ctypes.c_size_t, _vp, _vp],
+    ),
     "sa_pool_scores_workspace_size": (ctypes.c_size_t, [_i, _i, _i, _i, _i]),
     "sa_pool_scores": (
         _i,

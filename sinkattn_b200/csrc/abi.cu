@@ -77,6 +77,32 @@ int func_attr_once(const void* func, cudaFuncAttribute attr, int value) {
   return SA_OK;
 }
 
+int tile_map_bhsd(CUtensorMap* map, const void* base, const int64_t st[4], int B, int H, int S,
+                  int D) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return SA_ECUDA;
+  // dims innermost first: (D, S, H, B); strides in bytes for dims 1..3.
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
+  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims,
+                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return SA_ECUDA;
+  }
+  return SA_OK;
+}
+
+bool strides16_ok(const int64_t st[4]) {
+  if (st[3] != 1) return false;
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || (st[i] % 8) != 0) return false;
+  return true;
+}
+
 }  // namespace sa
 
 extern "C" const char* sa_last_error(void) { return sa::g_err; }

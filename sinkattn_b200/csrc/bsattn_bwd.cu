@@ -1,0 +1,758 @@
+// bsattn_bwd.cu — block-sparse attention backward for sm_100a.
+//
+// With P = exp(scale * Q K^T - lse) over the kept 128x128 blocks (0 elsewhere),
+// delta_i = sum_d dO_id O_id - dlse_i and dP = dO V^T, the gradients are
+//   dV = P^T dO,   dS = P o (dP - delta),   dQ = scale dS K,   dK = scale dS^T Q.
+// The probabilities are recomputed from Q, K and the row statistics of the
+// forward pass; nothing of size Sq x Sk is stored.
+//
+// Two kinds of tiles run through one persistent kernel:
+//   kind 0  one key block, over the query blocks that keep it (a mask column):
+//           dK and dV stay in TMEM.   X = K Q^T (= S^T),  Y = V dO^T (= dP^T),
+//           dV += P^T dO,  dK += dS^T Q          (4 products per kept block)
+//   kind 1  one query block, over its kept key blocks (a mask row): dQ stays in
+//           TMEM.   X = Q K^T,  Y = dO V^T,  dQ += dS K            (3 products)
+// Both have the same shape: two resident 128x128 tiles A1, A2, two streamed
+// tiles B1, B2 per block, X = A1 B1^T, Y = A2 B2^T, acc1 += P B2 (kind 0),
+// acc2 += dS B1. The transposed S of kind 0 makes P^T and dS^T the TMEM A
+// operands of their products, so neither ever passes through shared memory.
+// Recomputing S and dP for dQ costs 7 products per kept block where 5 would
+// do, and buys gradients that are each summed by one CTA in list order: no
+// atomics, the same bits on every run, and no fp32 dQ buffer in HBM (64 KB of
+// reductions per kept block).
+
+#include <math.h>
+
+#include "sa_common.cuh"
+
+namespace sa {
+namespace attn_bwd {
+
+constexpr int kT = 128;            // rows of every tile; head dim
+// Ring slots. B1 of a block is held from X to the block's last product, B2 not
+// as long; 64 KB of resident tiles leave room for five.
+constexpr int kB1 = 3, kB2 = 2;
+constexpr int kThreads = 384;      // 4 role warps + 2 warpgroups of arithmetic
+constexpr int kTileBytes = kT * kT * 2;
+constexpr int kBoxBytes = kTileBytes / 2;      // one 64-column box
+constexpr int kStatBytes = 2 * kT * 4;         // -lse (log2 units) and -delta of 128 rows
+constexpr int kMaxBlocks = 1024;               // per mask row or column (S <= 131072)
+constexpr int kListReaders = 2 + 256;
+constexpr uint32_t kColX = 0, kColY = 128, kColAcc1 = 256, kColAcc2 = 384;
+
+struct Params {
+  int B, H, Sq, Sk, nq, nk;
+  const uint8_t* mask;
+  int64_t ms0, ms1, ms2, ms3;
+  const int32_t* head_mask_type;
+  float scale, scale_log2;
+  const float* nstat;   // [B*H][nq*128][.]: first all -lse*log2(e), then all -delta
+  int64_t stat_plane;   // elements of one plane
+  __nv_bfloat16 *dq, *dk, *dv;
+  int64_t dqs0, dqs1, dqs2, dks0, dks1, dks2, dvs0, dvs1, dvs2;
+  int* next_tile;
+  int32_t* status;
+  int tiles0, tiles;    // kind-0 tiles come first
+};
+
+struct __align__(16) SmemCtl {
+  float stats[2][2 * kT];          // [block parity] -lse and -delta of a query block (kind 0)
+  uint64_t b1_full[kB1], b1_empty[kB1];
+  uint64_t b2_full[kB2], b2_empty[kB2];
+  uint64_t st_full[2];             // [block parity] statistics loaded (kind 1: a bare arrival)
+  uint64_t a_full[2], a_empty[2];  // [0] A1, [1] A2
+  uint64_t list_full[2], list_empty[2];
+  uint64_t x_full;       // X of a block computed (commit)
+  uint64_t x_done;       // kind 0: P written over X; kind 1: X copied out. 256 arrivals
+  uint64_t y_full[2];    // [block parity] Y computed (commit)
+  uint64_t ds_full[2];   // [block parity] dS written over Y, 256 arrivals
+  uint64_t acc_full;     // a tile's sums are complete (commit)
+  uint64_t acc_free;     // a tile's sums have been read, 256 arrivals
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int n_blocks[2];
+  int tile_id[2];
+  uint32_t kept[2][kMaxBlocks / 32];  // [slot] bit c of word i: block 32 i + c is kept
+};
+
+// The tiles need 1024-byte alignment (128-byte swizzle); dynamic shared memory
+// starts on it (checked by the kernel), so no slack is reserved.
+constexpr size_t kSmemBytes = (2 + kB1 + kB2) * kTileBytes + sizeof(SmemCtl);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+
+struct Tile {
+  int kind, blk, h, b;
+};
+
+__device__ __forceinline__ Tile tile_of(const Params& p, int t) {
+  Tile r;
+  r.kind = t >= p.tiles0 ? 1 : 0;
+  const int u = r.kind ? t - p.tiles0 : t;
+  const int n = r.kind ? p.nq : p.nk;
+  r.blk = u % n;
+  const int bh = u / n;
+  r.h = bh % p.H;
+  r.b = bh / p.H;
+  return r;
+}
+
+// Row statistics: one 16-lane group per query row sums dO . O in fp32. Rows
+// past Sq and rows without a finite log-sum-exp (no kept key) get -inf, which
+// makes every P of theirs 0. Bound by reading dO and O once.
+constexpr int kPrepRows = 4;  // rows of a 16-lane group, loaded together
+__global__ void __launch_bounds__(256)
+    row_stats_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ out,
+                     int64_t ds0, int64_t ds1, int64_t ds2, int64_t os0, int64_t os1, int64_t os2,
+                     const float* __restrict__ lse, const float* __restrict__ dlse, int H, int Sq,
+                     int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_tile) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next_tile = 0;
+  const int bh = blockIdx.y;
+  const int h = bh % H, b = bh / H;
+  const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int r0 = blockIdx.x * (16 * kPrepRows) + g;
+  uint4 x[kPrepRows], y[kPrepRows];
+#pragma unroll
+  for (int i = 0; i < kPrepRows; ++i) {
+    const int r = r0 + 16 * i;
+    x[i] = y[i] = make_uint4(0, 0, 0, 0);
+    if (r < Sq) {
+      x[i] = __ldg(reinterpret_cast<const uint4*>(dout + b * ds0 + h * ds1 + (int64_t)r * ds2) + l);
+      y[i] = __ldg(reinterpret_cast<const uint4*>(out + b * os0 + h * os1 + (int64_t)r * os2) + l);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPrepRows; ++i) {
+    const int r = r0 + 16 * i;
+    const uint32_t* a = reinterpret_cast<const uint32_t*>(&x[i]);
+    const uint32_t* c = reinterpret_cast<const uint32_t*>(&y[i]);
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = fmaf(__uint_as_float(a[e] << 16), __uint_as_float(c[e] << 16), s);
+      s = fmaf(__uint_as_float(a[e] & 0xffff0000u), __uint_as_float(c[e] & 0xffff0000u), s);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (l == 0 && r < rows_pad) {
+      float nl = -INFINITY, nd = 0.f;
+      if (r < Sq) {
+        const int64_t i0 = (int64_t)bh * Sq + r;
+        const float v = lse[i0];
+        if (v != -INFINITY) {
+          nl = -v * 1.4426950408889634f;
+          nd = (dlse != nullptr ? dlse[i0] : 0.f) - s;
+        }
+      }
+      const int64_t o0 = (int64_t)bh * rows_pad + r;
+      nstat[o0] = nl;
+      nstat[plane + o0] = nd;
+    }
+  }
+}
+
+// Writes one 128x128 fp32 accumulator (times mul) as bf16 rows; this thread's
+// half: 64 columns of its row.
+__device__ __forceinline__ void store_acc(uint32_t taddr, float mul, __nv_bfloat16* dst,
+                                          bool write) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t o[32];
+    tmem_ld32(taddr + c * 32, o);
+    tmem_wait_ld();
+    reg_fence32(o);
+    if (write) {
+      uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          w[u] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * u]) * mul,
+                             __uint_as_float(o[8 * v + 2 * u + 1]) * mul);
+        d4[v] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void store_zero(__nv_bfloat16* dst) {
+  uint4* d4 = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+  for (int v = 0; v < 8; ++v) d4[v] = make_uint4(0, 0, 0, 0);
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    bsattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q,
+                      const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v,
+                      const __grid_constant__ CUtensorMap tm_do, const Params p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* a_tile = smem;                       // A1, A2
+  uint8_t* b1_ring = smem + 2 * kTileBytes;
+  uint8_t* b2_ring = b1_ring + kB1 * kTileBytes;
+  SmemCtl* ctl = reinterpret_cast<SmemCtl*>(b2_ring + kB2 * kTileBytes);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if ((smem_u32(smem) & 1023u) != 0u) {
+    if (threadIdx.x == 0) report_timeout(p.status);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kB1; ++i) {
+      mbar_init(&ctl->b1_full[i], 1);
+      mbar_init(&ctl->b1_empty[i], 1);
+    }
+    for (int i = 0; i < kB2; ++i) {
+      mbar_init(&ctl->b2_full[i], 1);
+      mbar_init(&ctl->b2_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->st_full[i], 1);
+      mbar_init(&ctl->a_full[i], 1);
+      mbar_init(&ctl->a_empty[i], 1);
+      mbar_init(&ctl->list_full[i], 1);
+      mbar_init(&ctl->list_empty[i], kListReaders);
+      mbar_init(&ctl->y_full[i], 1);
+      mbar_init(&ctl->ds_full[i], 256);
+    }
+    mbar_init(&ctl->x_full, 1);
+    mbar_init(&ctl->x_done, 256);
+    mbar_init(&ctl->acc_full, 1);
+    mbar_init(&ctl->acc_free, 256);
+    mbar_init(&ctl->drain, 1);
+    ctl->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tm_q);
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+    prefetch_tensormap(&tm_do);
+  }
+  if (warp == 2) {
+    tmem_alloc(&ctl->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  const uint32_t tmem = ctl->tmem_base;
+  volatile int* abort_flag = &ctl->abort_flag;
+
+  if (warp == 2) {
+    // ---------------- tiles and their kept-block lists, two ahead ----------------
+    for (int k = 0;; ++k) {
+      const int slot = k & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&ctl->list_empty[slot], ((uint32_t)(k >> 1) & 1u) ^ 1u,
+                                             p.status, abort_flag)))
+        break;
+      int t = 0;
+      if (lane == 0) t = atomicAdd(p.next_tile, 1);
+      t = __shfl_sync(0xffffffffu, t, 0);
+      if (t >= p.tiles) {
+        if (lane == 0) {
+          ctl->tile_id[slot] = -1;
+          ctl->n_blocks[slot] = 0;
+          mbar_arrive(&ctl->list_full[slot]);
+        }
+        break;
+      }
+      const Tile tl = tile_of(p, t);
+      int mh = tl.h;
+      bool dense = false;
+      if (p.head_mask_type != nullptr) {
+        const int ty = p.head_mask_type[tl.h];
+        if (ty > 0) mh = ty - 1; else dense = true;
+      }
+      const uint8_t* m = p.mask + (int64_t)tl.b * p.ms0 + (int64_t)mh * p.ms1 +
+                         (int64_t)tl.blk * (tl.kind ? p.ms2 : p.ms3);
+      const int64_t step = tl.kind ? p.ms3 : p.ms2;
+      const int n = tl.kind ? p.nk : p.nq;
+      // all mask bytes are loaded before any is used; bit i of `bits` is block
+      // 32 i + lane
+      const int nw = (n + 31) >> 5;
+      uint32_t bits = 0;
+#pragma unroll 8
+      for (int i = 0; i < nw; ++i) {
+        const int c = i * 32 + lane;
+        const bool keep = c < n && (dense || m[(int64_t)c * step] != 0);
+        bits |= (uint32_t)keep << i;
+      }
+      int count = 0;
+      for (int i = 0; i < nw; ++i) {
+        const uint32_t bal = __ballot_sync(0xffffffffu, (bits >> i) & 1u);
+        if (lane == 0) ctl->kept[slot][i] = bal;
+        count += __popc(bal);
+      }
+      if (lane == 0) {
+        ctl->n_blocks[slot] = count;
+        ctl->tile_id[slot] = t;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->list_full[slot]);
+    }
+  } else if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      int J = 0, e = 0;        // blocks and tiles loaded
+      int sent[4] = {0, 0, 0, 0};  // loads issued: A1, A2, B1, B2
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = mbar_wait(bar, parity, p.status, abort_flag);
+        return ok;
+      };
+      auto load = [&](const CUtensorMap* map, uint64_t* bar, uint8_t* dst, int blk,
+                      const Tile& tl) {
+        mbar_arrive_expect_tx(bar, kTileBytes);
+        tma_load_4d(map, bar, dst, 0, blk * kT, tl.h, tl.b);
+        tma_load_4d(map, bar, dst + kBoxBytes, 64, blk * kT, tl.h, tl.b);
+      };
+      for (int k = 0; ok; ++k) {
+        const int slot = k & 1;
+        if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
+        const int t = ctl->tile_id[slot];
+        if (t < 0) break;
+        const Tile tl = tile_of(p, t);
+        const int n = ctl->n_blocks[slot];
+        const CUtensorMap* ma[2] = {tl.kind ? &tm_q : &tm_k, tl.kind ? &tm_do : &tm_v};
+        const CUtensorMap* mb[2] = {tl.kind ? &tm_k : &tm_q, tl.kind ? &tm_v : &tm_do};
+        const float* stat = p.nstat + (int64_t)(tl.b * p.H + tl.h) * p.nq * kT;
+        int word = 0;
+        uint32_t bits = ctl->kept[slot][0];
+        for (int j = 0; j < n; ++j, ++J) {
+          while (bits == 0u) bits = ctl->kept[slot][++word];  // n bits are set in all
+          const int blk = word * 32 + __ffs(bits) - 1;
+          bits &= bits - 1u;
+          // the resident tiles are free once the previous tile's last X / Y is complete
+          if (j == 0) {
+            if (!wait(&ctl->a_empty[0], ((uint32_t)e & 1u) ^ 1u)) break;
+            load(ma[0], &ctl->a_full[0], a_tile, tl.blk, tl);
+            ++sent[0];
+          }
+          const int s1 = J % kB1, s2 = J % kB2;
+          if (!wait(&ctl->b1_empty[s1], ((uint32_t)(J / kB1) & 1u) ^ 1u)) break;
+          load(mb[0], &ctl->b1_full[s1], b1_ring + s1 * kTileBytes, blk, tl);
+          ++sent[2];
+          if (j == 0) {
+            if (!wait(&ctl->a_empty[1], ((uint32_t)e & 1u) ^ 1u)) break;
+            load(ma[1], &ctl->a_full[1], a_tile + kTileBytes, tl.blk, tl);
+            ++sent[1];
+          }
+          if (!wait(&ctl->b2_empty[s2], ((uint32_t)(J / kB2) & 1u) ^ 1u)) break;
+          load(mb[1], &ctl->b2_full[s2], b2_ring + s2 * kTileBytes, blk, tl);
+          ++sent[3];
+          // the statistics of two blocks ago have been read once their dS is written
+          if (J >= 2 && !wait(&ctl->ds_full[J & 1], (uint32_t)((J - 2) >> 1) & 1u)) break;
+          if (tl.kind == 0) {
+            mbar_arrive_expect_tx(&ctl->st_full[J & 1], kStatBytes);
+            bulk_load(ctl->stats[J & 1], stat + (int64_t)blk * kT, kT * 4, &ctl->st_full[J & 1]);
+            bulk_load(ctl->stats[J & 1] + kT, stat + p.stat_plane + (int64_t)blk * kT, kT * 4,
+                      &ctl->st_full[J & 1]);
+          } else {
+            mbar_arrive(&ctl->st_full[J & 1]);
+          }
+        }
+        if (!ok) break;
+        if (n > 0) ++e;
+        mbar_arrive(&ctl->list_empty[slot]);
+      }
+      // no copy of this CTA may be in flight when it exits
+      for (int w = 0; w < 2; ++w)
+        if (sent[w] > 0) mbar_wait_drain(&ctl->a_full[w], (uint32_t)(sent[w] - 1) & 1u);
+      for (int i = max(0, sent[2] - kB1); i < sent[2]; ++i)
+        mbar_wait_drain(&ctl->b1_full[i % kB1], (uint32_t)(i / kB1) & 1u);
+      for (int i = max(0, sent[3] - kB2); i < sent[3]; ++i)
+        mbar_wait_drain(&ctl->b2_full[i % kB2], (uint32_t)(i / kB2) & 1u);
+      for (int i = max(0, J - 2); i < J; ++i)
+        mbar_wait_drain(&ctl->st_full[i & 1], (uint32_t)(i >> 1) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_kk = make_idesc_bf16(kT, kT, 0, 0);  // B rows are N, K-major
+      constexpr uint32_t idesc_mn = make_idesc_bf16(kT, kT, 0, 1);  // B rows are K, N-major
+      const uint32_t a_base = smem_u32(a_tile);
+      const uint32_t b1_base = smem_u32(b1_ring), b2_base = smem_u32(b2_ring);
+      int J = 0;   // blocks of earlier tiles
+      int e = 0;   // earlier tiles with blocks
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = mbar_wait(bar, parity, p.status, abort_flag);
+        return ok;
+      };
+      auto b1_tile = [&](int i) { return b1_base + (uint32_t)(i % kB1) * kTileBytes; };
+      auto b2_tile = [&](int i) { return b2_base + (uint32_t)(i % kB2) * kTileBytes; };
+      // D = A B^T with both tiles K-major in shared memory
+      auto mma_x = [&](uint32_t a, uint32_t b, uint32_t d_col) {
+#pragma unroll
+        for (int kk = 0; kk < kT / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kBoxBytes + (kk & 3) * 32;
+          mma_ss(tmem + d_col, make_sdesc_sw128(a + off, 16, 1024),
+                 make_sdesc_sw128(b + off, 16, 1024), idesc_kk, kk > 0 ? 1u : 0u);
+        }
+      };
+      // acc (+)= A . B, A = bf16 pairs in TMEM: each warpgroup's 64 columns of
+      // K lie in the first 32 of the 64 columns it read
+      auto mma_acc = [&](uint32_t a_col, uint32_t b, uint32_t d_col, bool first) {
+#pragma unroll
+        for (int kk = 0; kk < kT / 16; ++kk)
+          mma_ts(tmem + d_col, tmem + a_col + (kk >> 2) * 64 + (kk & 3) * 8,
+                 make_sdesc_sw128(b + kk * 2048, kBoxBytes, 1024), idesc_mn,
+                 (!first || kk > 0) ? 1u : 0u);
+      };
+      for (int k = 0; ok; ++k) {
+        const int slot = k & 1;
+        if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
+        const int t = ctl->tile_id[slot];
+        if (t < 0) break;
+        const int kind = t >= p.tiles0 ? 1 : 0;
+        const int n = ctl->n_blocks[slot];
+        if (n > 0) {
+          // kind 1 has no acc1: its columns are the second Y buffer
+          auto y_col = [&](int j) { return (kind && (j & 1)) ? kColAcc1 : kColY; };
+          bool acc_ready = e == 0;
+          auto wait_acc = [&]() {
+            if (!acc_ready) acc_ready = wait(&ctl->acc_free, (uint32_t)(e - 1) & 1u);
+            return ok;
+          };
+          auto issue_x = [&](int j) {
+            const int i = J + j;
+            if (j == 0 && !wait(&ctl->a_full[0], (uint32_t)e & 1u)) return;
+            if (!wait(&ctl->b1_full[i % kB1], (uint32_t)(i / kB1) & 1u)) return;
+            tc_fence_after();
+            mma_x(a_base, b1_tile(i), kColX);
+            mma_commit(&ctl->x_full);
+            if (j == n - 1) mma_commit(&ctl->a_empty[0]);
+          };
+          auto issue_y = [&](int j) {
+            const int i = J + j;
+            if (j == 0 && !wait(&ctl->a_full[1], (uint32_t)e & 1u)) return;
+            if (kind && j == 1 && !wait_acc()) return;
+            if (!wait(&ctl->b2_full[i % kB2], (uint32_t)(i / kB2) & 1u)) return;
+            tc_fence_after();
+            mma_x(a_base + kTileBytes, b2_tile(i), y_col(j));
+            mma_commit(&ctl->y_full[i & 1]);
+            if (kind) mma_commit(&ctl->b2_empty[i % kB2]);
+            if (j == n - 1) mma_commit(&ctl->a_empty[1]);
+          };
+          issue_x(0);
+          issue_y(0);
+          for (int j = 0; j < n && ok; ++j) {
+            const int i = J + j;
+            if (!wait(&ctl->x_done, (uint32_t)i & 1u)) break;
+            tc_fence_after();
+            if (!kind) {
+              if (!wait_acc()) break;
+              tc_fence_after();
+              mma_acc(kColX, b2_tile(i), kColAcc1, j == 0);
+              mma_commit(&ctl->b2_empty[i % kB2]);
+            }
+            if (j + 1 < n) {
+              issue_x(j + 1);
+              if (kind) issue_y(j + 1);
+            }
+            if (!wait(&ctl->ds_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
+            if (!wait_acc()) break;
+            tc_fence_after();
+            mma_acc(y_col(j), b1_tile(i), kColAcc2, j == 0);
+            mma_commit(&ctl->b1_empty[i % kB1]);
+            if (j + 1 < n && !kind) issue_y(j + 1);
+          }
+          if (!ok) break;
+          mma_commit(&ctl->acc_full);
+          J += n;
+          ++e;
+        }
+        mbar_arrive(&ctl->list_empty[slot]);
+      }
+      mma_commit(&ctl->drain);
+      mbar_wait_drain(&ctl->drain, 0);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------- probabilities, dS and the outputs ----------------
+    // Warpgroup g owns columns 64g..64g+63 of X and Y; a thread one row (TMEM
+    // lane) of them. P is kept in fp32 registers from X to dS.
+    const int g = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_self = tmem + lane_off + g * 64;
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+    bool ok = true;
+    int J = 0, e = 0;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      // warp-uniform: the TMEM accesses that follow are warp-collective
+      ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, abort_flag));
+      return ok;
+    };
+    for (int k = 0; ok; ++k) {
+      const int slot = k & 1;
+      if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
+      const int t = ctl->tile_id[slot];
+      if (t < 0) break;
+      const Tile tl = tile_of(p, t);
+      const int n = ctl->n_blocks[slot];
+      const int grow = tl.blk * kT + row;
+      const bool write = grow < (tl.kind ? p.Sq : p.Sk);
+      __nv_bfloat16 *o1 = nullptr, *o2;
+      if (tl.kind) {
+        o2 = p.dq + tl.b * p.dqs0 + tl.h * p.dqs1 + (int64_t)grow * p.dqs2 + g * 64;
+      } else {
+        o1 = p.dv + tl.b * p.dvs0 + tl.h * p.dvs1 + (int64_t)grow * p.dvs2 + g * 64;
+        o2 = p.dk + tl.b * p.dks0 + tl.h * p.dks1 + (int64_t)grow * p.dks2 + g * 64;
+      }
+      if (n == 0) {
+        if (write) {
+          if (!tl.kind) store_zero(o1);
+          store_zero(o2);
+        }
+        mbar_arrive(&ctl->list_empty[slot]);
+        continue;
+      }
+      float row_nl = 0.f, row_nd = 0.f;
+      if (tl.kind) {
+        const float* src = p.nstat + (int64_t)(tl.b * p.H + tl.h) * p.nq * kT + grow;
+        row_nl = src[0];
+        row_nd = src[p.stat_plane];
+      }
+      // the last key block of a ragged length, if it is kept
+      const bool ragged = tl.kind && (p.Sk % kT) != 0 &&
+                          ((ctl->kept[slot][(p.nk - 1) >> 5] >> ((p.nk - 1) & 31)) & 1u);
+      const uint64_t row_nl2 = f2_pack(row_nl, row_nl), row_nd2 = f2_pack(row_nd, row_nd);
+      for (int j = 0; j < n; ++j) {
+        const uint32_t jp = (uint32_t)(J + j);
+        uint64_t pr[32];  // 64 probabilities, in pairs
+        if (!wait(&ctl->st_full[jp & 1u], (jp >> 1) & 1u)) break;
+        if (tl.kind == 0) {
+          const float* st = ctl->stats[jp & 1u];
+          if (!wait(&ctl->x_full, jp & 1u)) break;
+          tc_fence_after();
+          const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(st + g * 64);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32], pk[16];
+            tmem_ld32(t_self + kColX + c * 32, r);
+            tmem_wait_ld();
+            reg_fence32(r);
+#pragma unroll
+            for (int u = 0; u < 16; u += 2) {
+              const ulonglong2 s2 = nl[c * 8 + (u >> 1)];
+#pragma unroll
+              for (int v = 0; v < 2; ++v) {
+                const uint64_t x2 =
+                    f2_fma(f2_pack(__uint_as_float(r[2 * (u + v)]),
+                                   __uint_as_float(r[2 * (u + v) + 1])),
+                           scale2, v ? s2.y : s2.x);
+                float x0, x1;
+                f2_unpack(x2, x0, x1);
+                x0 = ex2_approx(x0);
+                x1 = ex2_approx(x1);
+                pr[c * 16 + u + v] = f2_pack(x0, x1);
+                pk[u + v] = pack_bf16x2(x0, x1);
+              }
+            }
+            tmem_st16(t_self + kColX + c * 16, pk);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&ctl->x_done);
+          if (!wait(&ctl->y_full[jp & 1u], (jp >> 1) & 1u)) break;
+          tc_fence_after();
+          const ulonglong2* nd = reinterpret_cast<const ulonglong2*>(st + kT + g * 64);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32], pk[16];
+            tmem_ld32(t_self + kColY + c * 32, r);
+            tmem_wait_ld();
+            reg_fence32(r);
+#pragma unroll
+            for (int u = 0; u < 16; u += 2) {
+              const ulonglong2 s2 = nd[c * 8 + (u >> 1)];
+#pragma unroll
+              for (int v = 0; v < 2; ++v) {
+                const uint64_t d2 = f2_mul(pr[c * 16 + u + v],
+                                           f2_add(f2_pack(__uint_as_float(r[2 * (u + v)]),
+                                                          __uint_as_float(r[2 * (u + v) + 1])),
+                                                  v ? s2.y : s2.x));
+                float d0, d1;
+                f2_unpack(d2, d0, d1);
+                pk[u + v] = pack_bf16x2(d0, d1);
+              }
+            }
+            tmem_st16(t_self + kColY + c * 16, pk);
+          }
+        } else {
+          if (!wait(&ctl->x_full, jp & 1u)) break;
+          tc_fence_after();
+          uint32_t r[2][32];
+          tmem_ld32(t_self + kColX, r[0]);
+          tmem_ld32(t_self + kColX + 32, r[1]);
+          tmem_wait_ld();
+          reg_fence32(r[0]);
+          reg_fence32(r[1]);
+          tc_fence_before();
+          mbar_arrive(&ctl->x_done);
+#pragma unroll
+          for (int u = 0; u < 32; ++u) {
+            const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(r[u >> 4][2 * (u & 15)]),
+                                               __uint_as_float(r[u >> 4][2 * (u & 15) + 1])),
+                                       scale2, row_nl2);
+            float x0, x1;
+            f2_unpack(x2, x0, x1);
+            pr[u] = f2_pack(ex2_approx(x0), ex2_approx(x1));
+          }
+          // keys past Sk: their K rows are 0, but exp(-lse) may overflow
+          if (ragged && j == n - 1) {
+            const int valid = p.Sk - (p.nk - 1) * kT - g * 64;
+#pragma unroll
+            for (int u = 0; u < 32; ++u) {
+              float x0, x1;
+              f2_unpack(pr[u], x0, x1);
+              pr[u] = f2_pack(2 * u < valid ? x0 : 0.f, 2 * u + 1 < valid ? x1 : 0.f);
+            }
+          }
+          if (!wait(&ctl->y_full[jp & 1u], (jp >> 1) & 1u)) break;
+          tc_fence_after();
+          const uint32_t y = t_self + ((j & 1) ? kColAcc1 : kColY);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t q[32], pk[16];
+            tmem_ld32(y + c * 32, q);
+            tmem_wait_ld();
+            reg_fence32(q);
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+              const uint64_t d2 =
+                  f2_mul(pr[c * 16 + u], f2_add(f2_pack(__uint_as_float(q[2 * u]),
+                                                        __uint_as_float(q[2 * u + 1])),
+                                                row_nd2));
+              float d0, d1;
+              f2_unpack(d2, d0, d1);
+              pk[u] = pack_bf16x2(d0, d1);
+            }
+            tmem_st16(y + c * 16, pk);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ctl->ds_full[jp & 1u]);
+      }
+      if (!ok) break;
+      if (!wait(&ctl->acc_full, (uint32_t)e & 1u)) break;
+      tc_fence_after();
+      if (!tl.kind) store_acc(t_self + kColAcc1, 1.0f, o1, write);
+      store_acc(t_self + kColAcc2, p.scale, o2, write);
+      tc_fence_before();
+      mbar_arrive(&ctl->acc_free);
+      J += n;
+      ++e;
+      mbar_arrive(&ctl->list_empty[slot]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace attn_bwd
+}  // namespace sa
+
+extern "C" size_t sa_bsattn_bwd_workspace_size(int B, int H, int Sq, int Sk) {
+  using namespace sa::attn_bwd;
+  if (B < 1 || H < 1 || Sq < 1 || Sk < 1) return 0;
+  const size_t rows = (size_t)((Sq + kT - 1) / kT) * kT;
+  return 256 + 2 * sizeof(float) * (size_t)B * H * rows;
+}
+
+extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                             const void* out, const int64_t do_strides[4],
+                             const int64_t q_strides[4], const int64_t k_strides[4],
+                             const int64_t v_strides[4], const int64_t o_strides[4],
+                             const float* lse, const float* dlse, int B, int H, int Sq, int Sk,
+                             int D, const uint8_t* block_mask, const int64_t m_strides[4], int Hm,
+                             const int32_t* head_mask_type, float softmax_scale, void* dq,
+                             void* dk, void* dv, const int64_t dq_strides[4],
+                             const int64_t dk_strides[4], const int64_t dv_strides[4],
+                             void* workspace, size_t ws_bytes, int32_t* status,
+                             cudaStream_t stream) {
+  using namespace sa::attn_bwd;
+  const char* fn = "sa_bsattn_bwd";
+  SA_CHECK_ARG(dout && q && k && v && out && lse && block_mask && dq && dk && dv,
+               "%s: null tensor pointer", fn);
+  SA_CHECK_ARG(do_strides && q_strides && k_strides && v_strides && o_strides && m_strides &&
+                   dq_strides && dk_strides && dv_strides,
+               "%s: null stride array", fn);
+  SA_CHECK_ARG(D == kT, "%s: head dim must be 128, got %d", fn, D);
+  SA_CHECK_ARG(B >= 1 && H >= 1 && Sq >= 1 && Sk >= 1,
+               "%s: B, H, Sq, Sk must be >= 1 (got %d, %d, %d, %d)", fn, B, H, Sq, Sk);
+  SA_CHECK_ARG(Sq <= kMaxBlocks * kT && Sk <= kMaxBlocks * kT,
+               "%s: Sq, Sk must be at most %d (got %d, %d)", fn, kMaxBlocks * kT, Sq, Sk);
+  const int nq = (Sq + kT - 1) / kT, nk = (Sk + kT - 1) / kT;
+  SA_CHECK_ARG((int64_t)B * H <= 65535 && (int64_t)(nq + nk) * H * B <= 0x40000000,
+               "%s: too many heads or tiles (B %d, H %d)", fn, B, H);
+  const int64_t* all[] = {do_strides, q_strides,  k_strides,  v_strides,
+                          o_strides,  dq_strides, dk_strides, dv_strides};
+  for (const int64_t* st : all)
+    SA_CHECK_ARG(sa::strides16_ok(st),
+                 "%s: tensors need stride(dim)=1 and other strides multiple of 8 elements "
+                 "(16 bytes)", fn);
+  SA_CHECK_ARG(((uintptr_t)dout | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out |
+                (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0,
+               "%s: tensor base pointers must be 16-byte aligned", fn);
+  SA_CHECK_ARG(Hm >= 1 && (head_mask_type != nullptr || Hm == H),
+               "%s: mask has %d heads but H=%d and no head_mask_type", fn, Hm, H);
+  const size_t need = sa_bsattn_bwd_workspace_size(B, H, Sq, Sk);
+  SA_CHECK_ARG(workspace != nullptr && ws_bytes >= need && (uintptr_t)workspace % 256 == 0,
+               "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", fn, need, ws_bytes);
+
+  CUtensorMap tq, tk, tv, td;
+  int rc;
+  if ((rc = sa::tile_map_bhsd(&tq, q, q_strides, B, H, Sq, D)) != SA_OK) return rc;
+  if ((rc = sa::tile_map_bhsd(&tk, k, k_strides, B, H, Sk, D)) != SA_OK) return rc;
+  if ((rc = sa::tile_map_bhsd(&tv, v, v_strides, B, H, Sk, D)) != SA_OK) return rc;
+  if ((rc = sa::tile_map_bhsd(&td, dout, do_strides, B, H, Sq, D)) != SA_OK) return rc;
+
+  Params p;
+  p.B = B; p.H = H; p.Sq = Sq; p.Sk = Sk; p.nq = nq; p.nk = nk;
+  p.mask = block_mask;
+  p.ms0 = m_strides[0]; p.ms1 = m_strides[1]; p.ms2 = m_strides[2]; p.ms3 = m_strides[3];
+  p.head_mask_type = head_mask_type;
+  p.scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf((float)D);
+  p.scale_log2 = p.scale * 1.4426950408889634f;
+  float* nstat = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  p.nstat = nstat;
+  p.stat_plane = (int64_t)B * H * nq * kT;
+  p.dq = static_cast<__nv_bfloat16*>(dq);
+  p.dk = static_cast<__nv_bfloat16*>(dk);
+  p.dv = static_cast<__nv_bfloat16*>(dv);
+  p.dqs0 = dq_strides[0]; p.dqs1 = dq_strides[1]; p.dqs2 = dq_strides[2];
+  p.dks0 = dk_strides[0]; p.dks1 = dk_strides[1]; p.dks2 = dk_strides[2];
+  p.dvs0 = dv_strides[0]; p.dvs1 = dv_strides[1]; p.dvs2 = dv_strides[2];
+  p.next_tile = static_cast<int*>(workspace);
+  p.status = status;
+  p.tiles0 = nk * H * B;
+  p.tiles = p.tiles0 + nq * H * B;
+
+  if ((rc = sa::func_attr_once((const void*)bsattn_bwd_kernel,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes)) !=
+      SA_OK)
+    return rc;
+  const dim3 pg((unsigned)((nq * kT + 16 * kPrepRows - 1) / (16 * kPrepRows)), (unsigned)(B * H));
+  row_stats_kernel<<<pg, 256, 0, stream>>>(
+      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
+      do_strides[0], do_strides[1], do_strides[2], o_strides[0], o_strides[1], o_strides[2], lse,
+      dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_tile);
+  SA_CUDA_TRY(cudaGetLastError());
+  const int sms = sa::sm_count_current_device();
+  bsattn_bwd_kernel<<<p.tiles < sms ? p.tiles : sms, kThreads, kSmemBytes, stream>>>(tq, tk, tv,
+                                                                                  td, p);
+  SA_CUDA_TRY(cudaGetLastError());
+  return SA_OK;
+}

@@ -706,36 +706,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 namespace {
 
-int make_map_bshd(CUtensorMap* map, const void* base, const int64_t st[4], int B, int H, int S,
-                  int D) {
-  sa::EncodeTiledFn enc = sa::encode_tiled_fn();
-  if (enc == nullptr) return SA_ECUDA;
-  // dims innermost first: (D, S, H, B); strides in bytes for dims 1..3.
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
-  cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
-  cuuint32_t box[4] = {64, 128, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims,
-                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    sa::set_error("cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
-    return SA_ECUDA;
-  }
-  return SA_OK;
-}
-
-bool strides_ok(const int64_t st[4]) {
-  if (st[3] != 1) return false;
-  for (int i = 0; i < 3; ++i)
-    if (st[i] < 0 || (st[i] % 8) != 0) return false;
-  return true;
-}
-
-}  // namespace
-
-namespace {
-
 // Shared by sa_bsattn_fwd (k2 == nullptr) and sa_sink_dynamic_attn_fwd.
 int launch_attention(const char* fn, const void* q, const void* k, const void* v,
                      const int64_t q_strides[4], const int64_t k_strides[4],
@@ -761,8 +731,8 @@ int launch_attention(const char* fn, const void* q, const void* k, const void* v
   SA_CHECK_ARG(nk + nk2 <= kMaxBlocks && nk2 < 0x8000,
                "%s: %d + %d key blocks exceed %d", fn, nk, nk2, kMaxBlocks);
   SA_CHECK_ARG((int64_t)nq * H * B <= 0x7fffffff, "%s: too many query tiles", fn);
-  SA_CHECK_ARG(strides_ok(q_strides) && strides_ok(k_strides) && strides_ok(v_strides) &&
-                   strides_ok(o_strides) && (!dual || (strides_ok(k2_strides) && strides_ok(v2_strides))),
+  SA_CHECK_ARG(sa::strides16_ok(q_strides) && sa::strides16_ok(k_strides) && sa::strides16_ok(v_strides) &&
+                   sa::strides16_ok(o_strides) && (!dual || (sa::strides16_ok(k2_strides) && sa::strides16_ok(v2_strides))),
                "%s: q/k/v/out need stride(dim)=1 and other strides multiple of 8 "
                "elements (16 bytes)", fn);
   SA_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out |
@@ -774,11 +744,11 @@ int launch_attention(const char* fn, const void* q, const void* k, const void* v
 
   CUtensorMap tk, tv, tk2, tv2;
   int rc;
-  if ((rc = make_map_bshd(&tk, k, k_strides, B, H, Sk, D)) != SA_OK) return rc;
-  if ((rc = make_map_bshd(&tv, v, v_strides, B, H, Sk, D)) != SA_OK) return rc;
+  if ((rc = sa::tile_map_bhsd(&tk, k, k_strides, B, H, Sk, D)) != SA_OK) return rc;
+  if ((rc = sa::tile_map_bhsd(&tv, v, v_strides, B, H, Sk, D)) != SA_OK) return rc;
   if (dual) {
-    if ((rc = make_map_bshd(&tk2, k2, k2_strides, B, H, Sk2, D)) != SA_OK) return rc;
-    if ((rc = make_map_bshd(&tv2, v2, v2_strides, B, H, Sk2, D)) != SA_OK) return rc;
+    if ((rc = sa::tile_map_bhsd(&tk2, k2, k2_strides, B, H, Sk2, D)) != SA_OK) return rc;
+    if ((rc = sa::tile_map_bhsd(&tv2, v2, v2_strides, B, H, Sk2, D)) != SA_OK) return rc;
   } else {
     tk2 = tk;  // unused
     tv2 = tv;

@@ -39,6 +39,14 @@ int sm_count_current_device();
 // size they can need, so that no call lowers it under another's launch.
 int func_attr_once(const void* func, cudaFuncAttribute attr, int value);
 
+// Tensor map of a strided bf16 [B,H,S,D] tensor (element strides st, st[3] = 1)
+// for 64-channel x 128-row boxes in the 128-byte swizzle; rows past S read 0.
+int tile_map_bhsd(CUtensorMap* map, const void* base, const int64_t st[4], int B, int H, int S,
+                  int D);
+
+// stride(dim) = 1 and the other strides non-negative multiples of 8 elements.
+bool strides16_ok(const int64_t st[4]);
+
 }  // namespace sa
 
 #define SA_CHECK_ARG(cond, ...)      \
@@ -309,6 +317,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
         "=r"(r[31])
       : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {

@@ -188,6 +188,100 @@ def bsattn_fwd(
     return out, (lse if return_lse else None)
 
 
+def bsattn_bwd(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    block_mask: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    head_mask_type: Optional[torch.Tensor] = None,
+    dlse: Optional[torch.Tensor] = None,
+    dq: Optional[torch.Tensor] = None,
+    dk: Optional[torch.Tensor] = None,
+    dv: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+):
+    """Gradients of bsattn_fwd with respect to q, k and v.
+
+    dout [B,H,Sq,D] bf16; q, k, v, block_mask, softmax_scale, head_mask_type
+    as given to bsattn_fwd, out and lse as it returned them; dlse: optional
+    fp32 [B,H,Sq] gradient with respect to lse. Returns (dq, dk, dv) bf16;
+    each defaults to a [B,S,H,D]-contiguous buffer viewed as [B,H,S,D]. Equal
+    calls give equal bits. A given `workspace` (uint8,
+    sa_bsattn_bwd_workspace_size bytes) may hold anything; calls sharing one
+    must not overlap on the GPU.
+    """
+    dev = _require_cuda(dout, q, k, v, out, lse, block_mask, head_mask_type, dlse, dq, dk, dv,
+                        workspace)
+    if q.dim() != 4 or k.dim() != 4:
+        raise RuntimeError("bsattn_bwd expects 4-D [B,H,S,D] tensors")
+    B, H, Sq, D = q.shape
+    Sk = k.shape[2]
+    for name, t, S in (("dout", dout, Sq), ("q", q, Sq), ("k", k, Sk), ("v", v, Sk),
+                       ("out", out, Sq), ("dq", dq, Sq), ("dk", dk, Sk), ("dv", dv, Sk)):
+        if t is None:
+            continue
+        if t.dtype != torch.bfloat16 or t.shape != (B, H, S, D):
+            raise RuntimeError(f"bsattn_bwd: {name} must be bf16 {(B, H, S, D)}, got {t.dtype} "
+                               f"{tuple(t.shape)}")
+        if name in ("dq", "dk", "dv") and not _bf16_view_ok(t):
+            raise RuntimeError(f"bsattn_bwd: {name} must have stride(-1)=1, 16-byte strides and "
+                               "alignment")
+    for name, t in (("lse", lse), ("dlse", dlse)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (B, H, Sq)):
+            raise RuntimeError(f"bsattn_bwd: {name} must be fp32 {(B, H, Sq)}, got {t.dtype} "
+                               f"{tuple(t.shape)}")
+    head_mask_type = _check_block_mask("bsattn_bwd", block_mask, head_mask_type, B, H, Sq, Sk)
+    dout, q, k, v, out = (_as_kernel_layout(t) for t in (dout, q, k, v, out))
+    lse = lse.contiguous()
+    dlse = None if dlse is None else dlse.contiguous()
+
+    def grad(S):
+        return torch.empty((B, S, H, D), dtype=torch.bfloat16, device=dev).permute(0, 2, 1, 3)
+
+    dq = grad(Sq) if dq is None else dq
+    dk = grad(Sk) if dk is None else dk
+    dv = grad(Sk) if dv is None else dv
+    lib = _lib.load()
+    need = int(lib.sa_bsattn_bwd_workspace_size(B, H, Sq, Sk))
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    ms = list(block_mask.stride())
+    if block_mask.shape[0] == 1:
+        ms[0] = 0
+    st = _lib.strides4
+    with torch.cuda.device(dev):
+        rc = lib.sa_bsattn_bwd(
+            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st(dout),
+            st(q), st(k), st(v), st(out), lse.data_ptr(), _ptr(dlse), B, H, Sq, Sk, D,
+            block_mask.data_ptr(), (_lib.ctypes.c_int64 * 4)(*ms), block_mask.shape[1],
+            _ptr(head_mask_type), -1.0 if softmax_scale is None else float(softmax_scale),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), st(dq), st(dk), st(dv),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            DeviceStatus.pointer(dev), _stream(dev))
+    _lib.check(rc, "sa_bsattn_bwd")
+    return dq, dk, dv
+
+
+def _check_block_mask(fn: str, block_mask: torch.Tensor, head_mask_type: Optional[torch.Tensor],
+                      B: int, H: int, Sq: int, Sk: int) -> Optional[torch.Tensor]:
+    nq, nk = math.ceil(Sq / BLOCK), math.ceil(Sk / BLOCK)
+    if block_mask.dim() != 4 or block_mask.shape[-2:] != (nq, nk) \
+            or block_mask.shape[0] not in (1, B):
+        raise RuntimeError(f"{fn}: block_mask must be [{B}|1, Hm, {nq}, {nk}], got "
+                           f"{tuple(block_mask.shape)}")
+    if block_mask.dtype not in (torch.bool, torch.uint8):
+        raise RuntimeError(f"{fn}: block_mask must be bool/uint8, got {block_mask.dtype}")
+    if head_mask_type is None:
+        return None
+    if head_mask_type.dtype != torch.int32 or head_mask_type.numel() != H:
+        raise RuntimeError(f"{fn}: head_mask_type must be int32 [{H}]")
+    return head_mask_type.contiguous()
+
+
 def sink_dynamic_attn(
     q: torch.Tensor,
     k: torch.Tensor,

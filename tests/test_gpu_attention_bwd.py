@@ -1,0 +1,284 @@
+"""Gradients of the block-sparse attention against the formulas in 64 bits.
+
+Tolerances, element by element, from the kernel's roundings (u = 2^-8, half a
+bf16 step relative to the value; every sum is fp32):
+  * out as the forward kernel stores it is off by u (P|V|) (its bf16 P) plus
+    u |out|, so delta = sum dout * out is off by e_d = sum_d |dout| (u P|V| + u |out|);
+  * P carries e_p = 2^-13: the exponent is a fp32 difference of terms below 2^9
+    (three roundings of 2^-24 * 2^9 * log2 units, 0.7 of it in the result) and
+    the fp32 log-sum-exp of the same size;
+  * dv = P^T dout rounds P to bf16: (u + e_p) P^T|dout|, then u |dv|;
+  * dS = P (dP - delta) rounds to bf16: (u + e_p) |dS| + P (e_d + 2^-15 |dout||v|^T)
+    (fp32 dP, 128 terms), and dq, dk sum it against |k|, |q|, then u |dq|, u |dk|.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -8
+E_P = 2.0 ** -13
+
+
+def token_mask(mask, B, H, Sq, Sk, hmt=None):
+    m = mask.expand(B, -1, -1, -1)
+    if hmt is not None:
+        m = torch.stack([torch.ones_like(m[:, 0]) if t == 0 else m[:, t - 1]
+                         for t in hmt.tolist()], dim=1)
+    m = m.bool().repeat_interleave(128, dim=2)[:, :, :Sq]
+    return m.repeat_interleave(128, dim=3)[..., :Sk]
+
+
+def reference(q, k, v, dout, keep, scale, dlse=None):
+    """(dq, dk, dv), and the bounds above, in 64 bits."""
+    q, k, v, g = (t.double() for t in (q, k, v, dout))
+    kt, vt = k.transpose(-1, -2), v.transpose(-1, -2)
+    s = (q @ kt) * scale
+    s = torch.where(keep, s, torch.full_like(s, -math.inf))
+    p = torch.nan_to_num(torch.softmax(s, dim=-1), nan=0.0)
+    out = p @ v
+    dp = g @ vt
+    delta = (g * out).sum(-1, keepdim=True)
+    if dlse is not None:
+        delta = delta - dlse.double()[..., None]
+    ds = p * (dp - delta)
+    dq, dk, dv = scale * ds @ k, scale * ds.transpose(-1, -2) @ q, p.transpose(-1, -2) @ g
+    e_d = (g.abs() * (U * (p @ v.abs()) + U * out.abs())).sum(-1, keepdim=True)
+    e_ds = (U + E_P) * ds.abs() + p * (e_d + 2.0 ** -15 * (g.abs() @ vt.abs()))
+    bq = scale * e_ds @ k.abs() + U * dq.abs()
+    bk = scale * e_ds.transpose(-1, -2) @ q.abs() + U * dk.abs()
+    bv = (U + E_P) * p.transpose(-1, -2) @ g.abs() + U * dv.abs()
+    return (dq, dk, dv), (bq, bk, bv)
+
+
+def check(got, ref, bound):
+    for name, a, r, b in zip(("dq", "dk", "dv"), got, ref, bound):
+        assert a.shape == r.shape and a.dtype == torch.bfloat16
+        err = (a.double() - r).abs()
+        assert torch.isfinite(a).all(), f"{name} not finite"
+        # 2^-100: nothing smaller is told apart (fp32 sums flush no larger terms)
+        over = err - (b * 1.001 + 2.0 ** -100)
+        worst = int(over.argmax())
+        assert float(over.max()) <= 0, (f"{name} off by {float(err.view(-1)[worst]):.3e} where "
+                                        f"{float(b.view(-1)[worst]):.3e} is allowed")
+
+
+def make(B, H, Sq, Sk, p, seed, scale=1.0, empty=0.0, layout="bshd", Bm=None):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def t(S):
+        if layout == "bshd":
+            x = torch.randn(B, S, H, 128, generator=g, device="cuda").permute(0, 2, 1, 3)
+        else:
+            x = torch.randn(B, H, S, 128, generator=g, device="cuda")
+        return (x * scale).bfloat16()
+
+    q, k, v, dout = t(Sq), t(Sk), t(Sk), t(Sq)
+    nq, nk = math.ceil(Sq / 128), math.ceil(Sk / 128)
+    mask = torch.rand(Bm or B, H, nq, nk, generator=g, device="cuda") < p
+    if empty == 0.0:
+        mask[..., 0] = True
+    else:
+        mask &= torch.rand(Bm or B, H, nq, 1, generator=g, device="cuda") >= empty
+    return q, k, v, dout, mask
+
+
+def run(q, k, v, dout, mask, scale=None, hmt=None, dlse=None, **kw):
+    from sinkattn_b200 import ops
+
+    out, lse = ops.bsattn_fwd(q, k, v, mask, softmax_scale=scale, head_mask_type=hmt)
+    got = ops.bsattn_bwd(dout, q, k, v, out, lse, mask, softmax_scale=scale, head_mask_type=hmt,
+                         dlse=dlse, **kw)
+    torch.cuda.synchronize()
+    ops.DeviceStatus.check()
+    return got
+
+
+def both(q, k, v, dout, mask, scale=None, hmt=None, dlse=None, **kw):
+    B, H, Sq, D = q.shape
+    got = run(q, k, v, dout, mask, scale, hmt, dlse, **kw)
+    keep = token_mask(mask, B, H, Sq, k.shape[2], hmt)
+    ref, bound = reference(q, k, v, dout, keep, scale or 1 / math.sqrt(D), dlse)
+    check(got, ref, bound)
+    return got
+
+
+def test_one_block():
+    both(*make(1, 1, 128, 128, 1.0, 0))
+
+
+@pytest.mark.parametrize("B,H,Sq,Sk,p", [
+    (1, 1, 1, 1, 1.0), (2, 2, 1, 300, 1.0), (1, 2, 128, 1, 1.0), (2, 3, 257, 129, 0.5),
+    (1, 2, 640, 33, 1.0), (2, 2, 1000, 1092, 0.4), (1, 2, 129, 4000, 0.3), (1, 1, 4000, 70, 1.0),
+    (1, 3, 2048, 2048, 0.2), (3, 5, 384, 640, 1.0),
+])
+def test_shapes(B, H, Sq, Sk, p):
+    both(*make(B, H, Sq, Sk, p, Sq * 7 + Sk))
+
+
+@pytest.mark.parametrize("layout", ["bshd", "bhsd"])
+@pytest.mark.parametrize("empty", [0.3, 1.0])
+def test_rows_and_columns_that_keep_nothing(layout, empty):
+    both(*make(2, 3, 900, 700, 0.25, 5, empty=empty, layout=layout))
+
+
+def test_mask_shared_by_the_batch_and_strided():
+    q, k, v, dout, mask = make(3, 2, 500, 600, 0.5, 6, Bm=1)
+    both(q, k, v, dout, mask)
+    wide = torch.zeros(1, 2, mask.shape[2], 2 * mask.shape[3], dtype=torch.bool, device="cuda")
+    wide[..., ::2] = mask
+    a = run(q, k, v, dout, mask)
+    b = run(q, k, v, dout, wide[..., ::2])
+    c = run(q, k, v, dout, mask.transpose(2, 3).contiguous().transpose(2, 3))
+    for x, y, z in zip(a, b, c):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_head_mask_type():
+    q, k, v, dout, mask = make(2, 4, 400, 500, 0.4, 7)
+    hmt = torch.tensor([2, 0, 1, 1], dtype=torch.int32, device="cuda")
+    both(q, k, v, dout, mask[:, :2], hmt=hmt)
+
+
+@pytest.mark.parametrize("scale", [0.02, 0.3])
+def test_scale(scale):
+    both(*make(1, 2, 300, 300, 0.7, 8), scale=scale)
+
+
+def test_gradient_of_the_log_sum_exp():
+    q, k, v, dout, mask = make(2, 2, 500, 400, 0.5, 9)
+    dlse = torch.randn(2, 2, 500, device="cuda")
+    both(q, k, v, dout, mask, dlse=dlse)
+
+
+def test_statistics_that_overflow_outside_the_lengths():
+    """All logits near -280: exp(-lse) overflows for the zero rows behind the
+    last key, which must not reach dq."""
+    q, k, v, dout, mask = make(1, 2, 200, 150, 1.0, 10)
+    q = (q * 0.01 + 5).bfloat16()
+    k = (k * 0.01 - 5).bfloat16()
+    keep = token_mask(mask, 1, 2, 200, 150)
+    got = run(q, k, v, dout, mask)
+    ref, bound = reference(q, k, v, dout, keep, 1 / math.sqrt(128))
+    check(got, ref, bound)
+
+
+def test_nan_and_inf_where_nothing_is_kept():
+    q, k, v, dout, mask = make(1, 2, 512, 640, 0.5, 11)
+    mask[..., 3] = False      # a key block nobody keeps
+    mask[:, :, 2] = False     # a query block that keeps nothing
+    keep = token_mask(mask, 1, 2, 512, 640)
+    ref, bound = reference(q, k, v, dout, keep, 1 / math.sqrt(128))
+    k[:, :, 384:512] = float("nan")
+    v[:, :, 384:512] = float("inf")
+    q[:, :, 256:384] = float("inf")
+    dout[:, :, 256:384] = float("nan")
+    check(run(q, k, v, dout, mask), ref, bound)
+
+
+def test_outputs_given_by_the_caller_and_what_lies_behind_them():
+    q, k, v, dout, mask = make(2, 2, 300, 200, 0.6, 12)
+    plain = run(q, k, v, dout, mask)
+
+    def window(S):  # a strided window of a larger buffer, the rest a marker
+        buf = torch.full((2, S + 7, 2, 3, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+        return buf, buf[:, :S, :, 1].permute(0, 2, 1, 3)
+
+    bufs = [window(S) for S in (300, 200, 200)]
+    got = run(q, k, v, dout, mask, dq=bufs[0][1], dk=bufs[1][1], dv=bufs[2][1])
+    for (buf, view), a, b, S in zip(bufs, got, plain, (300, 200, 200)):
+        assert a.data_ptr() == view.data_ptr() and torch.equal(a, b)
+        rest = buf.clone()
+        rest[:, :S, :, 1] = 7.0
+        assert (rest == 7.0).all()
+
+
+def test_layouts_and_misaligned_inputs_agree():
+    q, k, v, dout, mask = make(2, 3, 450, 330, 0.5, 13)
+    a = run(q, k, v, dout, mask)
+    b = run(*(t.contiguous() for t in (q, k, v, dout)), mask)
+
+    def odd(t):  # a view whose base and rows are not 16-byte aligned
+        buf = torch.zeros(*t.shape[:-1], 133, dtype=t.dtype, device="cuda")
+        buf[..., 3:131] = t
+        return buf[..., 3:131]
+
+    c = run(*(odd(t) for t in (q, k, v, dout)), mask)
+    for x, y, z in zip(a, b, c):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_keys_shared_by_heads():
+    """Keys and values broadcast over the heads by a stride of 0."""
+    q, k, v, dout, mask = make(1, 4, 300, 300, 0.6, 14, layout="bhsd")
+    ks, vs = k[:, :1].expand(-1, 4, -1, -1), v[:, :1].expand(-1, 4, -1, -1)
+    a = run(q, ks, vs, dout, mask)
+    b = run(q, ks.contiguous(), vs.contiguous(), dout, mask)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_equal_calls_give_equal_bits():
+    args = make(1, 4, 3000, 3000, 0.3, 15)
+    first = run(*args)
+    for _ in range(5):
+        for a, b in zip(first, run(*args)):
+            assert torch.equal(a, b)
+
+
+def test_captured_and_on_two_streams():
+    from sinkattn_b200 import ops
+
+    q, k, v, dout, mask = make(1, 3, 700, 700, 0.5, 16)
+    q2, k2, v2, dout2, mask2 = make(1, 3, 700, 700, 0.5, 17)
+    want = [x.clone() for x in run(q, k, v, dout, mask)]
+    want2 = [x.clone() for x in run(q2, k2, v2, dout2, mask2)]
+    out, lse = ops.bsattn_fwd(q, k, v, mask)
+    out2, lse2 = ops.bsattn_fwd(q2, k2, v2, mask2)
+    static = [t.clone() for t in (dout, q, k, v, out, lse, mask)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.bsattn_bwd(*static)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        graph.replay()  # and, beside it, an eager call on another stream
+        with torch.cuda.stream(side):
+            beside = ops.bsattn_bwd(dout2, q2, k2, v2, out2, lse2, mask2)
+        torch.cuda.synchronize()
+        for a, b, c, d in zip(got, want, beside, want2):
+            assert torch.equal(a, b) and torch.equal(c, d)
+    for s, t in zip(static, (dout2, q2, k2, v2, out2, lse2, mask2)):
+        s.copy_(t)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want2):
+        assert torch.equal(a, b)
+    del graph
+
+
+def test_gradient_against_differences():
+    """The scalar sum(dout * out) along a random direction, by differences of
+    the formulas in 64 bits."""
+    q, k, v, dout, mask = make(1, 1, 200, 260, 0.7, 18)
+    keep = token_mask(mask, 1, 1, 200, 260)
+    dirs = [torch.randn(t.shape, dtype=torch.float64, device="cuda") for t in (q, k, v)]
+
+    def value(h):
+        a, b, c = (t.double() + h * d for t, d in zip((q, k, v), dirs))
+        s = (a @ b.transpose(-1, -2)) / math.sqrt(128)
+        p = torch.softmax(torch.where(keep, s, torch.full_like(s, -math.inf)), dim=-1)
+        return float((dout.double() * (p @ c)).sum())
+
+    h = 1e-4
+    want = (value(h) - value(-h)) / (2 * h)
+    got = run(q, k, v, dout, mask)
+    slope = sum(float((a.double() * d).sum()) for a, d in zip(got, dirs))
+    # the sum of n independent roundings of at most `bound` each: 6 standard deviations
+    _, bound = reference(q, k, v, dout, keep, 1 / math.sqrt(128))
+    tol = 6 * math.sqrt(sum(float((b * d).square().sum()) for b, d in zip(bound, dirs)))
+    assert abs(slope - want) <= tol, (slope, want, tol)
