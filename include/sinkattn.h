@@ -51,6 +51,12 @@ extern "C" {
 /* Device status codes written into `status` by kernels. */
 #define SA_DEV_OK 0
 #define SA_DEV_WAIT_TIMEOUT 1 /* an mbarrier wait exceeded its iteration limit */
+#define SA_DEV_BAD_INDEX 2    /* a position outside the rotary tables */
+
+/* Element types of the entry points that take one. */
+#define SA_DTYPE_BF16 0
+#define SA_DTYPE_FP16 1
+#define SA_DTYPE_FP32 2
 
 /* Mask-builder modes (offline_text_video_coverage_mode). */
 #define SA_COVERAGE_JOINT 0
@@ -396,6 +402,82 @@ SA_API int sa_qk_norm_rope(const void* q_in, const void* k_in, int64_t q_in_row_
                            cudaStream_t stream);
 
 /*
+ * Gradient of sa_qk_norm_rope with respect to its inputs and weights, from
+ * the gradients dq, dk of its outputs (the rounding between the norm and the
+ * rotation counts as the identity).
+ * Replaces: the backward pass of apply_fast_qk_norm + apply_fast_rotary_qk
+ *   (wanx/runtime/fast_misc.py:834-864, 216-234), which the reference's Wan
+ *   processor runs for inference only.
+ *   g = the rotation transposed applied to dq, u = g w, r = rstd:
+ *   dq_in = r (u - q r^2 mean(u q)), dw_q = sum over rows of g q r; k alike.
+ * Arguments as for sa_qk_norm_rope (q, k its inputs; dq, dk, dq_in, dk_in
+ * bf16 rows with strides of their own; dq_in may be dq, dk_in may be dk).
+ * dw_q, dw_k: fp32 [hidden], both or neither, only with weights. fp32 sums in a
+ * fixed order: equal calls give equal bits. rows may be 0 (dw = 0).
+ * workspace (only for dw): sa_qk_norm_rope_bwd_workspace_size(hidden) bytes,
+ *   16-byte aligned, any contents, not shared by calls that overlap.
+ */
+SA_API size_t sa_qk_norm_rope_bwd_workspace_size(int hidden);
+SA_API int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_row_stride,
+                               int64_t dk_row_stride, const void* q, const void* k,
+                               int64_t q_row_stride, int64_t k_row_stride, int rows, int S,
+                               int hidden, int D, const void* w_q, const void* w_k, int w_is_bf16,
+                               float eps, const float* cos_table, const float* sin_table,
+                               int64_t freq_row_stride, void* dq_in, void* dk_in,
+                               int64_t dqi_row_stride, int64_t dki_row_stride, float* dw_q,
+                               float* dw_k, void* workspace, size_t ws_bytes,
+                               cudaStream_t stream);
+
+/*
+ * Q/K producer of models that norm every head by itself (Z-Image's norm_q and
+ * norm_k, applied per head before the rotary embedding): RMSNorm over the D
+ * channels of each head, then the rotation, for Q and K in one pass.
+ *   r = 1 / sqrt(mean(x^2) + eps), y = x r w,
+ *   (o_a, o_b) = (y_a cos - y_b sin, y_a sin + y_b cos) for the pairs
+ *   (a, b) = (2i, 2i+1) (interleaved != 0) or (i, i + rot_dim/2), i < rot_dim/2;
+ *   channels from rot_dim on are y. fp32 throughout, rounded once.
+ * q, q_out [B,S,Hq,D], k, k_out [B,S,Hk,D] of `dtype` (SA_DTYPE_*), strides in
+ *   the order (batch, seq, head, dim) with stride(dim) = 1, 16-byte aligned
+ *   bases and strides; an output may be its input. Hk may be 0 (no k). D a
+ *   multiple of 8 up to 256.
+ * w_q, w_k: [D] of w_dtype, both NULL for none. cos/sin: fp32 [table_rows,
+ *   >= rot_dim/2] with the given row stride, both NULL for no rotation; rot_dim
+ *   a multiple of 8 (16 without interleaving) up to D.
+ * positions: NULL (token s of a sequence uses table row s, table_rows >= S) or
+ *   int32 / int64 (positions_i64) [B,S] with pos_strides: the token's table
+ *   row, e.g. of single tokens late in a sequence. For a position outside the
+ *   tables nothing is read there: the token's rows (and the gradients of the
+ *   weights) become NaN and *status (nullable) SA_DEV_BAD_INDEX.
+ */
+SA_API int sa_qk_head_norm_rope(
+    const void* q, const void* k, const int64_t q_strides[4], const int64_t k_strides[4], int B,
+    int S, int Hq, int Hk, int D, int dtype, const void* w_q, const void* w_k, int w_dtype,
+    float eps, const float* cos_table, const float* sin_table, int64_t freq_row_stride,
+    int table_rows, int rot_dim, int interleaved, const void* positions, int positions_i64,
+    const int64_t pos_strides[2], void* q_out, void* k_out, const int64_t qo_strides[4],
+    const int64_t ko_strides[4], int32_t* status, cudaStream_t stream);
+
+/*
+ * Gradient of sa_qk_head_norm_rope from the gradients dq, dk of its outputs
+ * (formulas as for sa_qk_norm_rope_bwd, the mean over D): dq_in, dk_in of
+ * `dtype` (an output may be its dq or dk) and dw_q, dw_k fp32 [D] summed over
+ * tokens and heads (nullable together; only with weights). Other arguments as
+ * above. Equal calls give equal bits. B or S may be 0 (dw = 0).
+ * workspace (only for dw): sa_qk_head_norm_rope_bwd_workspace_size(D) bytes,
+ *   16-byte aligned, any contents, not shared by calls that overlap.
+ */
+SA_API size_t sa_qk_head_norm_rope_bwd_workspace_size(int D);
+SA_API int sa_qk_head_norm_rope_bwd(
+    const void* dq, const void* dk, const int64_t dq_strides[4], const int64_t dk_strides[4],
+    const void* q, const void* k, const int64_t q_strides[4], const int64_t k_strides[4], int B,
+    int S, int Hq, int Hk, int D, int dtype, const void* w_q, const void* w_k, int w_dtype,
+    float eps, const float* cos_table, const float* sin_table, int64_t freq_row_stride,
+    int table_rows, int rot_dim, int interleaved, const void* positions, int positions_i64,
+    const int64_t pos_strides[2], void* dq_in, void* dk_in, const int64_t dqi_strides[4],
+    const int64_t dki_strides[4], float* dw_q, float* dw_k, void* workspace, size_t ws_bytes,
+    int32_t* status, cudaStream_t stream);
+
+/*
  * Per-row minimal coverage block mask.
  * Replaces: _build_direct_mean_coverage_mask (sinkattention/sparse_attention.py:268-376)
  *   including _build_offline_required_mask (sparse_attention.py:241-265).
@@ -510,8 +592,8 @@ SA_API int sa_ulysses_combine_units(const void* out_units, const float* lse_unit
  *   (the same address where the device uses unified addressing);
  *   sa_status_destroy frees it.
  * sa_check_status: reads a host-readable status word without synchronising:
- *   SA_OK if no kernel reported a failure, else SA_ETIMEOUT (with a message)
- *   and the word is reset to SA_DEV_OK. A launch's report becomes visible once
+ *   SA_OK if no kernel reported a failure, else SA_ETIMEOUT (SA_EINVAL for
+ *   SA_DEV_BAD_INDEX) with a message, and the word is reset to SA_DEV_OK. A launch's report becomes visible once
  *   the launch has run, so a caller that needs a verdict on a given launch
  *   synchronises its stream first.
  */

@@ -21,6 +21,11 @@ SA_ECUDA = -4
 
 SA_DEV_OK = 0
 SA_DEV_WAIT_TIMEOUT = 1
+SA_DEV_BAD_INDEX = 2
+
+SA_DTYPE_BF16 = 0
+SA_DTYPE_FP16 = 1
+SA_DTYPE_FP32 = 2
 
 SA_COVERAGE_JOINT = 0
 SA_COVERAGE_VIDEO_RESIDUAL = 1
@@ -37,6 +42,7 @@ _c_i64_3 = ctypes.c_int64 * 3
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_l = ctypes.c_int64
 
 # name -> (restype, argtypes); mirrors include/sinkattn.h
 _SIGNATURES = {
@@ -90,6 +96,23 @@ _SIGNATURES = {
         _i,
         [_vp, _vp, ctypes.c_int64, ctypes.c_int64, _i, _i, _i, _i, _vp, _vp, _i, _f, _vp, _vp,
          ctypes.c_int64, _vp, _vp, ctypes.c_int64, ctypes.c_int64, _vp],
+    ),
+    "sa_qk_norm_rope_bwd_workspace_size": (ctypes.c_size_t, [_i]),
+    "sa_qk_norm_rope_bwd": (
+        _i,
+        [_vp, _vp, _l, _l, _vp, _vp, _l, _l, _i, _i, _i, _i, _vp, _vp, _i, _f, _vp, _vp, _l, _vp,
+         _vp, _l, _l, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+    ),
+    "sa_qk_head_norm_rope": (
+        _i,
+        [_vp] * 4 + [_i] * 6 + [_vp, _vp, _i, _f, _vp, _vp, _l, _i, _i, _i, _vp, _i, _vp]
+        + [_vp] * 6,
+    ),
+    "sa_qk_head_norm_rope_bwd_workspace_size": (ctypes.c_size_t, [_i]),
+    "sa_qk_head_norm_rope_bwd": (
+        _i,
+        [_vp] * 8 + [_i] * 6 + [_vp, _vp, _i, _f, _vp, _vp, _l, _i, _i, _i, _vp, _i, _vp]
+        + [_vp] * 7 + [ctypes.c_size_t, _vp, _vp],
     ),
     "sa_coverage_mask": (
         _i,
@@ -161,6 +184,10 @@ def check(rc: int, what: str) -> None:
 def strides4(t) -> "ctypes.Array":
     st = t.stride()
     return _c_i64_4(*[int(x) for x in st])
+
+
+def strides4_opt(t) -> "ctypes.Array | None":
+    return None if t is None else _c_i64_4(*t.stride())
 
 
 def strides3(t) -> "ctypes.Array":

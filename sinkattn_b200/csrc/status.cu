@@ -57,6 +57,11 @@ extern "C" int sa_check_status(int32_t* status) {
   const int32_t v = *reinterpret_cast<volatile int32_t*>(status);
   if (v == SA_DEV_OK) return SA_OK;
   *reinterpret_cast<volatile int32_t*>(status) = SA_DEV_OK;
+  if (v == SA_DEV_BAD_INDEX) {
+    sa::set_error(
+        "a kernel met a position outside the rotary tables: the rows of those tokens are NaN");
+    return SA_EINVAL;
+  }
   sa::set_error(
       "a bounded wait in a kernel gave up (device status %d): the outputs of the launches "
       "that shared this status word since the last check are not valid",

@@ -914,6 +914,245 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, head_dim: int, eps: float,
     return out_q, out_k
 
 
+def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                     head_dim: int, eps: float, w_q: Optional[torch.Tensor] = None,
+                     w_k: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+                     sin: Optional[torch.Tensor] = None, dq: Optional[torch.Tensor] = None,
+                     dk: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None):
+    """Gradient of qk_norm_rope from the gradients of its two outputs.
+
+    q, k, head_dim, eps, w_q, w_k, cos, sin as given to qk_norm_rope; dq_out,
+    dk_out bf16 [B, S, hidden]. Returns (dq, dk, dw_q, dw_k): bf16 [B, S,
+    hidden] (dq may be dq_out, dk may be dk_out) and fp32 [hidden] (None
+    without weights). Equal calls give equal bits. Calls sharing a `workspace`
+    (uint8, sa_qk_norm_rope_bwd_workspace_size bytes) must not overlap.
+    """
+    dev = _require_cuda(dq_out, dk_out, q, k, w_q, w_k, cos, sin, dq, dk, workspace)
+    if q.dim() != 3:
+        raise RuntimeError("qk_norm_rope_bwd expects [B, S, hidden] tensors")
+    B, S, hidden = q.shape
+    for name, t in (("dq_out", dq_out), ("dk_out", dk_out), ("q", q), ("k", k), ("dq", dq),
+                    ("dk", dk)):
+        if t is not None and (t.dtype != torch.bfloat16 or t.shape != (B, S, hidden)):
+            raise RuntimeError(f"qk_norm_rope_bwd: {name} must be bf16 {(B, S, hidden)}, got "
+                               f"{t.dtype} {tuple(t.shape)}")
+
+    def rows(t):  # uniform 16-byte rows, as the kernel walks them
+        return t.numel() == 0 or (
+            t.stride(-1) == 1 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
+            and (B == 1 or t.stride(0) == S * t.stride(1)))
+
+    dq_out, dk_out, q, k = (t if rows(t) else _aligned(t) for t in (dq_out, dk_out, q, k))
+    dq = torch.empty((B, S, hidden), dtype=torch.bfloat16, device=dev) if dq is None else dq
+    dk = torch.empty((B, S, hidden), dtype=torch.bfloat16, device=dev) if dk is None else dk
+    if not (rows(dq) and rows(dk)):
+        raise RuntimeError("qk_norm_rope_bwd outputs need uniform rows, 16-byte aligned")
+    if (w_q is None) != (w_k is None) or (cos is None) != (sin is None):
+        raise RuntimeError("qk_norm_rope_bwd: w_q and w_k, cos and sin go together")
+    dw_q = dw_k = None
+    w_bf16 = 1
+    if w_q is not None:
+        if w_q.shape != (hidden,) or w_k.shape != (hidden,):
+            raise RuntimeError(f"norm weights must have {hidden} elements")
+        if w_q.dtype == torch.bfloat16 and w_k.dtype == torch.bfloat16:
+            w_q, w_k = _aligned(w_q), _aligned(w_k)
+        else:
+            w_q, w_k, w_bf16 = _aligned(w_q.float()), _aligned(w_k.float()), 0
+        dw_q = torch.empty(hidden, dtype=torch.float32, device=dev)
+        dw_k = torch.empty(hidden, dtype=torch.float32, device=dev)
+    fs = 0
+    if cos is not None:
+        if cos.shape != (S, head_dim // 2) or sin.shape != (S, head_dim // 2):
+            raise ValueError(f"Rotary frequency shape mismatch: expected {(S, head_dim // 2)}, "
+                             f"got {tuple(cos.shape)} and {tuple(sin.shape)}")
+        cos, sin = _aligned(cos.float()), _aligned(sin.float())
+        fs = cos.stride(0)
+    lib = _lib.load()
+    ws_bytes = 0
+    with torch.cuda.device(dev):
+        if dw_q is not None:
+            if workspace is None:
+                workspace = torch.empty(int(lib.sa_qk_norm_rope_bwd_workspace_size(hidden)),
+                                        dtype=torch.uint8, device=dev)
+            ws_bytes = workspace.numel() * workspace.element_size()
+        rc = lib.sa_qk_norm_rope_bwd(
+            dq_out.data_ptr(), dk_out.data_ptr(), dq_out.stride(1), dk_out.stride(1),
+            q.data_ptr(), k.data_ptr(), q.stride(1), k.stride(1), B * S, max(S, 1), hidden,
+            int(head_dim), _ptr(w_q), _ptr(w_k), w_bf16, float(eps), _ptr(cos), _ptr(sin), fs,
+            dq.data_ptr(), dk.data_ptr(), dq.stride(1), dk.stride(1), _ptr(dw_q), _ptr(dw_k),
+            _ptr(workspace) if ws_bytes else None, ws_bytes, _stream(dev))
+    _lib.check(rc, "sa_qk_norm_rope_bwd")
+    return dq, dk, dw_q, dw_k
+
+
+_DTYPES = {torch.bfloat16: _lib.SA_DTYPE_BF16, torch.float16: _lib.SA_DTYPE_FP16,
+           torch.float32: _lib.SA_DTYPE_FP32}
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t itself when contiguous on a 16-byte boundary, else a copy that is."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _view16_ok(t: torch.Tensor) -> bool:
+    n = 16 // t.element_size()
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and not any(s % n for s in t.stride()[:-1]))
+
+
+def _head_norm_args(fn: str, q, k, w_q, w_k, cos, sin, positions, interleaved):
+    """Checks and lays out what qk_head_norm_rope and its gradient share; the
+    order of the returned arguments is the C entry points'."""
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise RuntimeError(f"{fn} expects q, k of [B, S, heads, D]")
+    B, S, Hq, D = q.shape
+    Hk = 0 if k is None else k.shape[2]
+    if q.dtype not in _DTYPES:
+        raise RuntimeError(f"{fn} expects bf16, fp16 or fp32, got {q.dtype}")
+    if k is not None and (k.dtype != q.dtype or k.shape != (B, S, Hk, D)):
+        raise RuntimeError(f"{fn}: k must be {q.dtype} {(B, S, Hk, D)}, got {k.dtype} "
+                           f"{tuple(k.shape)}")
+    if (w_q is None) != (w_k is None) and k is not None or (w_q is None and w_k is not None):
+        raise RuntimeError(f"{fn}: w_q and w_k go together")
+    w_dtype = _lib.SA_DTYPE_FP32
+    if w_q is not None:
+        same = w_q.dtype in _DTYPES and (w_k is None or w_k.dtype == w_q.dtype)
+        for w in (w_q, w_k):
+            if w is not None and w.shape != (D,):
+                raise RuntimeError(f"{fn}: norm weights must have {D} elements, got "
+                                   f"{tuple(w.shape)}")
+        w_q, w_k = (None if w is None else _aligned(w if same else w.float()) for w in (w_q, w_k))
+        w_dtype = _DTYPES[w_q.dtype]
+    if (cos is None) != (sin is None):
+        raise RuntimeError(f"{fn}: cos and sin go together")
+    fs = rot = rows = 0
+    if cos is not None:
+        if cos.dim() != 2 or sin.shape != cos.shape or cos.dtype != torch.float32 \
+                or sin.dtype != torch.float32:
+            raise RuntimeError(f"{fn}: cos and sin must be fp32 [table rows, rotated channels / 2]"
+                               f", got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} "
+                               f"{tuple(sin.shape)}")
+        rows, rot = cos.shape[0], 2 * cos.shape[1]
+        if not (_view16_ok(cos) and _view16_ok(sin)) or cos.stride(0) != sin.stride(0) \
+                or cos.stride(0) < rot // 2:
+            cos, sin = _aligned(cos), _aligned(sin)
+        fs = cos.stride(0)
+    pst = None
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
+                or positions.shape[-1] != S or positions.dim() == 2 and positions.shape[0] != B:
+            raise RuntimeError(f"{fn}: positions must be int32 or int64 [{B}, {S}] or [{S}], got "
+                               f"{positions.dtype} {tuple(positions.shape)}")
+        if cos is None:
+            raise RuntimeError(f"{fn}: positions need cos and sin")
+        sb = positions.stride(0) if positions.dim() == 2 else 0
+        pst = (_lib.ctypes.c_int64 * 2)(sb, positions.stride(-1))
+    tail = (B, S, Hq, Hk, D, _DTYPES[q.dtype], _ptr(w_q), _ptr(w_k), w_dtype)
+    tab = (_ptr(cos), _ptr(sin), fs, rows, rot, int(bool(interleaved)), _ptr(positions),
+           int(positions is not None and positions.dtype == torch.int64), pst)
+    # the tensors stay referenced until the launch
+    return tail, tab, (w_q, w_k, cos, sin, positions)
+
+
+def _head_tensor(fn: str, name: str, t: Optional[torch.Tensor], like: Optional[torch.Tensor],
+                 out: bool):
+    if like is None:
+        if t is not None:
+            raise RuntimeError(f"{fn}: {name} without k")
+        return None
+    if t is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if t.dtype != like.dtype or t.shape != like.shape:
+        raise RuntimeError(f"{fn}: {name} must be {like.dtype} {tuple(like.shape)}, got {t.dtype} "
+                           f"{tuple(t.shape)}")
+    if _view16_ok(t):
+        return t
+    if out:
+        raise RuntimeError(f"{fn}: {name} must have stride(-1)=1, 16-byte strides and alignment")
+    return _aligned(t)
+
+
+def qk_head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], eps: float,
+                      w_q: Optional[torch.Tensor] = None, w_k: Optional[torch.Tensor] = None,
+                      cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None, interleaved: bool = True,
+                      out_q: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None):
+    """RMSNorm of every head over its own channels + rotary embedding for Q and K.
+
+    q [B,S,Hq,D], k [B,S,Hk,D] (or None): bf16, fp16 or fp32; D a multiple of 8
+    up to 256. w_q, w_k: [D] or None. cos, sin: fp32 [T, R/2] or None (no
+    rotation): the first R channels are rotated in pairs (2i, 2i+1)
+    (interleaved) or (i, i + R/2); R a multiple of 8 (16). Token s of a sequence
+    uses table row s, or row positions[b, s] (int32 / int64 [B,S] or [S]) where
+    given; a position outside the table makes the token's rows NaN and is
+    reported by DeviceStatus. fp32 throughout, rounded once. Returns (q, k) of
+    the input type; out_q/out_k may alias q/k or be views of a larger buffer.
+    """
+    dev = _require_cuda(q, k, w_q, w_k, cos, sin, positions, out_q, out_k)
+    fn = "qk_head_norm_rope"
+    sizes, tab, keep = _head_norm_args(fn, q, k, w_q, w_k, cos, sin, positions, interleaved)
+    q = _head_tensor(fn, "q", q, q, False)
+    k = _head_tensor(fn, "k", k, k, False)
+    out_q = _head_tensor(fn, "out_q", out_q, q, True)
+    out_k = _head_tensor(fn, "out_k", out_k, k, True)
+    st = _lib.strides4_opt
+    with torch.cuda.device(dev):
+        rc = _lib.load().sa_qk_head_norm_rope(
+            q.data_ptr(), _ptr(k), st(q), st(k), *sizes, float(eps), *tab, out_q.data_ptr(),
+            _ptr(out_k), st(out_q), st(out_k), DeviceStatus.pointer(dev), _stream(dev))
+    _lib.check(rc, "sa_qk_head_norm_rope")
+    return out_q, out_k
+
+
+def qk_head_norm_rope_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor,
+                          k: Optional[torch.Tensor], eps: float,
+                          w_q: Optional[torch.Tensor] = None, w_k: Optional[torch.Tensor] = None,
+                          cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                          positions: Optional[torch.Tensor] = None, interleaved: bool = True,
+                          dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None,
+                          workspace: Optional[torch.Tensor] = None):
+    """Gradient of qk_head_norm_rope from the gradients of its outputs.
+
+    dq_out, dk_out: like q, k; the other arguments as given to
+    qk_head_norm_rope. Returns (dq, dk, dw_q, dw_k): like q and k (dq may be
+    dq_out, dk may be dk_out), and fp32 [D] sums over tokens and heads (None
+    without weights). Equal calls give equal bits. Calls sharing a `workspace`
+    (uint8, sa_qk_head_norm_rope_bwd_workspace_size bytes) must not overlap.
+    """
+    dev = _require_cuda(dq_out, dk_out, q, k, w_q, w_k, cos, sin, positions, dq, dk, workspace)
+    fn = "qk_head_norm_rope_bwd"
+    sizes, tab, keep = _head_norm_args(fn, q, k, w_q, w_k, cos, sin, positions, interleaved)
+    if k is not None and dk_out is None:
+        raise RuntimeError(f"{fn}: dk_out is missing")
+    dw_q = dw_k = None
+    D = q.shape[-1]
+    if w_q is not None:
+        dw_q = torch.empty(D, dtype=torch.float32, device=dev)
+        dw_k = None if k is None else torch.empty(D, dtype=torch.float32, device=dev)
+    dq_out = _head_tensor(fn, "dq_out", dq_out, q, False)
+    dk_out = _head_tensor(fn, "dk_out", dk_out, k, False)
+    q, k = _head_tensor(fn, "q", q, q, False), _head_tensor(fn, "k", k, k, False)
+    dq, dk = _head_tensor(fn, "dq", dq, q, True), _head_tensor(fn, "dk", dk, k, True)
+    lib = _lib.load()
+    st = _lib.strides4_opt
+    ws_bytes = 0
+    with torch.cuda.device(dev):
+        if dw_q is not None:
+            if workspace is None:
+                workspace = torch.empty(int(lib.sa_qk_head_norm_rope_bwd_workspace_size(D)),
+                                        dtype=torch.uint8, device=dev)
+            ws_bytes = workspace.numel() * workspace.element_size()
+        rc = lib.sa_qk_head_norm_rope_bwd(
+            dq_out.data_ptr(), _ptr(dk_out), st(dq_out), st(dk_out), q.data_ptr(), _ptr(k), st(q),
+            st(k), *sizes, float(eps), *tab, dq.data_ptr(), _ptr(dk), st(dq), st(dk), _ptr(dw_q),
+            _ptr(dw_k), _ptr(workspace) if ws_bytes else None, ws_bytes,
+            DeviceStatus.pointer(dev), _stream(dev))
+    _lib.check(rc, "sa_qk_head_norm_rope_bwd")
+    return dq, dk, dw_q, dw_k
+
+
 def mean_pool_seq(x: torch.Tensor, pool: int, prefix: int = 0) -> torch.Tensor:
     """_mean_pool_sequence_preserve_prefix on a bf16 [B,H,S,D] view."""
     dev = _require_cuda(x)
