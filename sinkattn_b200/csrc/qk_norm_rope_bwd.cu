@@ -5,10 +5,11 @@
 // and r = 1 / sqrt(mean x^2 + eps) over the hidden channels of a row:
 //   dx = r (u - x r^2 mean(u x)),   dw = sum over rows of g x r.
 // Memory-bound: x and the upstream gradient are read and dx written once
-// (6 bf16 values per hidden channel of Q and K together). A team of 1, 2 or 4
-// warps takes a row of Q or of K, at most 48 channels a lane, so that the row,
-// its gradient and the lane's part of dw stay in registers and both sums of
-// the row are reduced together.
+// (6 bf16 values per hidden channel of Q and K together). A block takes whole
+// rows, one 8-channel vector of Q and one of K per thread, so that the angles
+// are read once for both, dw needs 16 registers and the next row's vectors are
+// loaded before the current row's sums are reduced. (A warp per row, 48
+// channels a lane, needed 158 registers and reached 28% of the copy rate.)
 
 #include <math.h>
 
@@ -17,28 +18,35 @@
 namespace sa {
 namespace nr {
 
-__global__ void __launch_bounds__(256)
+// 32 columns per block, 32 interleaved chains of rows: short enough that the
+// loads of a chain are all in flight (8 chains took 10 us for 600 rows).
+constexpr int kChains = 32;
+__global__ void __launch_bounds__(32 * kChains)
     partial_rows_kernel(const float* __restrict__ part, int rows, int cols, int pitch,
                         float* __restrict__ out0, float* __restrict__ out1, int cols0) {
-  __shared__ float red[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), chain = threadIdx.x >> 5;
+  __shared__ float red[kChains][33];
+  const int l = threadIdx.x & 31, chain = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + l;
   float s = 0.f;
   if (c < cols) {
 #pragma unroll 8
-    for (int r = chain; r < rows; r += 8) s += part[(int64_t)r * pitch + c];
+    for (int r = chain; r < rows; r += kChains) s += part[(int64_t)r * pitch + c];
   }
-  red[chain][threadIdx.x & 31] = s;
+  red[chain][l] = s;
   __syncthreads();
-  if (chain == 0 && c < cols) {
+  // warp w sums column w of the block over the chains
+  s = red[l][chain];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x & 31];
-    if (c < cols0) out0[c] = s; else out1[c - cols0] = s;
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int cw = blockIdx.x * 32 + chain;
+  if (l == 0 && cw < cols) {
+    if (cw < cols0) out0[cw] = s; else out1[cw - cols0] = s;
   }
 }
 
 int sum_partial_rows(const float* part, int rows, int cols, int pitch, float* out0, float* out1,
                      int cols0, cudaStream_t stream) {
-  partial_rows_kernel<<<(cols + 31) / 32, 256, 0, stream>>>(part, rows, cols, pitch, out0, out1,
+  partial_rows_kernel<<<(cols + 31) / 32, 32 * kChains, 0, stream>>>(part, rows, cols, pitch, out0, out1,
                                                             cols0);
   SA_CUDA_TRY(cudaGetLastError());
   return SA_OK;
@@ -50,8 +58,8 @@ namespace qkrope_bwd {
 
 using namespace sa::nr;
 
-constexpr int kWarps = 4;
 constexpr int kMaxHidden = 4096;
+constexpr int kMaxThreads = kMaxHidden / 8;
 
 struct Params {
   const __nv_bfloat16* d[2];  // upstream gradients of q, k
@@ -67,145 +75,135 @@ struct Params {
   float* part;  // [partial rows][2][hidden], NULL without dw
 };
 
-// 8 channels of the upstream gradient, rotated back.
-__device__ __forceinline__ void rotated(const Raw8<__nv_bfloat16>& raw, const float* cos_row,
-                                        const float* sin_row, int c0, int D, float (&g)[8]) {
-  unpack8(raw, g);
-  if (cos_row == nullptr) return;
-  const int p0 = (c0 % D) >> 1;
-  const float4 c4 = __ldg(reinterpret_cast<const float4*>(cos_row + p0));
-  const float4 s4 = __ldg(reinterpret_cast<const float4*>(sin_row + p0));
-  const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+// Four sums over a warp at once: after two exchange steps a lane carries one
+// of the four (by its lowest two bits), then they are reduced over the rest.
+// Lane l < 4 ends with value l. 6 shuffles where 20 would do one by one.
+__device__ __forceinline__ float warp_sum4(float a, float b, float c, float d, int lane) {
+  const bool hi = lane & 1, hi2 = lane & 2;
+  float x = hi ? b : a, y = hi ? d : c;  // kept: values 0/1 and 2/3 by the lowest bit
+  x += __shfl_xor_sync(0xffffffffu, hi ? a : b, 1);
+  y += __shfl_xor_sync(0xffffffffu, hi ? c : d, 1);
+  float z = hi2 ? y : x;
+  z += __shfl_xor_sync(0xffffffffu, hi2 ? x : y, 2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float e = g[2 * i], o = g[2 * i + 1];
-    g[2 * i] = e * c[i] + o * s[i];
-    g[2 * i + 1] = o * c[i] - e * s[i];
-  }
+  for (int o = 4; o < 32; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  return z;
 }
 
-// W warps form a team that takes rows of one tensor: the block's teams are q,
-// k, q, k (W = 1), q, k (W = 2) or one of them by the block's parity (W = 4).
-template <int VPL, int W>
-__global__ void __launch_bounds__(32 * kWarps) kernel(const Params p) {
-  constexpr int kTeams = kWarps / W;
-  __shared__ float2 sums[2][kWarps];
-  extern __shared__ float stage[];  // W = 1: dw of the second q and k team
-  const int team = (threadIdx.x >> 5) / W;
-  const int64_t gteam = (int64_t)blockIdx.x * kTeams + team;
-  const int which = (int)(gteam & 1);
-  const int tl = threadIdx.x - team * 32 * W;  // thread of the team
-  const int nvec = p.hidden >> 3;
+struct Row {
+  Raw8<__nv_bfloat16> x[2], d[2];
+};
+
+__device__ __forceinline__ Row load_row(const Params& p, int64_t row, int c0, bool on) {
+  Row r;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    r.x[w] = r.d[w] = Raw8<__nv_bfloat16>{};
+    if (on) {
+      r.x[w] = load8(p.x[w] + row * p.xs[w] + c0);
+      r.d[w] = load8(p.d[w] + row * p.ds[w] + c0);
+    }
+  }
+  return r;
+}
+
+// One thread per 8 channels; rows blockIdx.x, + gridDim.x, ... Registers are
+// capped so that 768 threads fit an SM.
+template <int MAXT>
+__global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
+  __shared__ __align__(16) float sums[2][MAXT / 32][4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int c0 = threadIdx.x * 8;
+  const bool on = c0 < p.hidden;
+  const int p0 = (c0 % p.D) >> 1;
   const float inv_n = 1.f / (float)p.hidden;
-  float acc[VPL][8];
+  V8 acc[2] = {fill8(0.f), fill8(0.f)};
+  V8 w[2];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-  const int64_t step = (int64_t)gridDim.x * kTeams / 2;
+  for (int i = 0; i < 2; ++i) w[i] = load_weight8(p.w[i], p.w_dtype, on ? c0 : 0);
+  Row next = load_row(p, blockIdx.x, c0, on);
   int turn = 0;
-  for (int64_t row = gteam >> 1; row < p.rows; row += step, turn ^= 1) {
-    const __nv_bfloat16* xr = p.x[which] + row * p.xs[which];
-    const __nv_bfloat16* dr = p.d[which] + row * p.ds[which];
-    __nv_bfloat16* orow = p.o[which] + row * p.os[which];
-    Raw8<__nv_bfloat16> rx[VPL], rd[VPL];
+  for (int row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const Row cur = next;
+    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.cos_t != nullptr && on) {
+      const int64_t s = (unsigned)row % (unsigned)p.S;
+      c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t + s * p.fs + p0));
+      s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t + s * p.fs + p0));
+    }
+    if (p.rows - row > (int)gridDim.x) next = load_row(p, (int64_t)row + gridDim.x, c0, on);
+    const uint64_t c2[2] = {f2_pack(c4.x, c4.y), f2_pack(c4.z, c4.w)};
+    const uint64_t s2[2] = {f2_pack(s4.x, s4.y), f2_pack(s4.z, s4.w)};
+    const uint64_t n2[2] = {f2_pack(-s4.x, -s4.y), f2_pack(-s4.z, -s4.w)};
+    V8 x[2], g[2];
+    float ss[2], dot[2];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int v = tl + i * 32 * W;
-      rx[i] = rd[i] = Raw8<__nv_bfloat16>{};
-      if (v < nvec) {
-        rx[i] = load8(xr + v * 8);
-        rd[i] = load8(dr + v * 8);
+    for (int i = 0; i < 2; ++i) {
+      x[i] = unpack8(cur.x[i]);
+      const V8 d = unpack8(cur.d[i]);
+      uint64_t a2 = 0ull, b2 = 0ull;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        g[i].v[2 * j] = f2_fma(d.v[2 * j], c2[j], f2_mul(d.v[2 * j + 1], s2[j]));
+        g[i].v[2 * j + 1] = f2_fma(d.v[2 * j + 1], c2[j], f2_mul(d.v[2 * j], n2[j]));
       }
-    }
-    const int s = (int)(row % p.S);
-    const float* crow = p.cos_t != nullptr ? p.cos_t + (int64_t)s * p.fs : nullptr;
-    const float* srow = p.sin_t != nullptr ? p.sin_t + (int64_t)s * p.fs : nullptr;
-    float ss = 0.f, dot = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int v = tl + i * 32 * W;
-      if (v >= nvec) continue;
-      float x[8], g[8], w[8];
-      unpack8(rx[i], x);
-      rotated(rd[i], crow, srow, v * 8, p.D, g);
-      load_weight8(p.w[which], p.w_dtype, v * 8, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ss = fmaf(x[j], x[j], ss);
-        dot = fmaf(g[j] * w[j], x[j], dot);
+      for (int j = 0; j < 4; ++j) {
+        a2 = f2_fma(x[i].v[j], x[i].v[j], a2);
+        b2 = f2_fma(f2_mul(g[i].v[j], w[i].v[j]), x[i].v[j], b2);
       }
+      ss[i] = sum2(a2);
+      dot[i] = sum2(b2);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    }
-    if (W > 1) {
-      // two buffers in turn: a warp writes the next row's sums only after the
-      // whole team has passed this row's barrier
-      if ((threadIdx.x & 31) == 0) sums[turn][threadIdx.x >> 5] = make_float2(ss, dot);
-      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(32 * W) : "memory");
-      ss = dot = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        ss += sums[turn][team * W + w].x;
-        dot += sums[turn][team * W + w].y;
-      }
-    }
-    const float r = __fdiv_rn(1.f, __fsqrt_rn(ss * inv_n + p.eps));
-    const float m = r * r * dot * inv_n;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int v = tl + i * 32 * W;
-      if (v >= nvec) continue;
-      float x[8], g[8], w[8];
-      unpack8(rx[i], x);
-      rotated(rd[i], crow, srow, v * 8, p.D, g);
-      load_weight8(p.w[which], p.w_dtype, v * 8, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        acc[i][j] = fmaf(g[j] * r, x[j], acc[i][j]);
-        x[j] = r * (g[j] * w[j] - x[j] * m);
-      }
-      store8(orow + v * 8, x);
-    }
-  }
-  if (p.part == nullptr) return;
-  if (W == 1) {
-    if (team >= 2) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int v = tl + i * 32;
-        if (v < nvec) store8(stage + which * p.hidden + v * 8, acc[i]);
-      }
-    }
+    const float z = warp_sum4(ss[0], dot[0], ss[1], dot[1], lane);
+    // two buffers in turn: a warp writes a row's sums only after the block has
+    // passed the barrier of the row before, so the row before that has been read
+    if (lane < 4) sums[turn][warp][lane] = z;
     __syncthreads();
-    if (team >= 2) return;
-  }
-  const int64_t prow = W == 4 ? blockIdx.x >> 1 : blockIdx.x;
-  float* dst = p.part + (prow * 2 + which) * p.hidden;
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const int v = tl + i * 32 * W;
-    if (v >= nvec) continue;
-    if (W == 1) {
-      const float* other = stage + which * p.hidden + v * 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i][j] += other[j];
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int v = 0; v < warps; ++v) {
+      const float4 q = *reinterpret_cast<const float4*>(sums[turn][v]);
+      t.x += q.x; t.y += q.y; t.z += q.z; t.w += q.w;
     }
-    store8(dst + v * 8, acc[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float r = inv_sqrt(fmaf(i ? t.z : t.x, inv_n, p.eps));
+      const float m = -r * r * r * (i ? t.w : t.y) * inv_n;
+      const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
+      V8 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t gr = f2_mul(g[i].v[j], r2);
+        acc[i].v[j] = f2_fma(gr, x[i].v[j], acc[i].v[j]);
+        o.v[j] = f2_fma(x[i].v[j], m2, f2_mul(gr, w[i].v[j]));
+      }
+      if (on) store8(p.o[i] + (int64_t)row * p.os[i] + c0, o);
+    }
   }
+  if (p.part == nullptr || !on) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    store8(p.part + ((int64_t)blockIdx.x * 2 + i) * p.hidden + c0, acc[i]);
 }
 
-int max_blocks() { return sa::sm_count_current_device() * 4; }
+// Blocks: 768 threads per SM, and at least two rows each where there
+// are that few, as every block leaves a partial row of dw to be read again.
+int blocks_of(int rows, int threads) {
+  const int per_sm = 768 / threads > 1 ? 768 / threads : 1;
+  const int64_t most = (int64_t)sa::sm_count_current_device() * (per_sm < 16 ? per_sm : 16);
+  const int64_t want = ((int64_t)rows + 1) / 2;
+  return (int)(want < most ? want : most);
+}
+
+int threads_of(int hidden) { return (hidden / 8 + 31) / 32 * 32; }
 
 }  // namespace qkrope_bwd
 }  // namespace sa
 
 extern "C" size_t sa_qk_norm_rope_bwd_workspace_size(int hidden) {
-  if (hidden < 8) return 0;
-  return (size_t)sa::qkrope_bwd::max_blocks() * 2 * hidden * sizeof(float);
+  if (hidden < 8 || hidden > sa::qkrope_bwd::kMaxHidden) return 0;
+  using namespace sa::qkrope_bwd;
+  return (size_t)blocks_of(0x7ffffffe, threads_of(hidden)) * 2 * hidden * sizeof(float);
 }
 
 extern "C" int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_row_stride,
@@ -260,26 +258,10 @@ extern "C" int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_ro
     p.eps = eps;
     p.cos_t = cos_table; p.sin_t = sin_table; p.fs = freq_row_stride;
     p.part = dw_q != nullptr ? part : nullptr;
-    // the narrowest team whose lanes hold at most 48 channels each
-    const int W = hidden <= 1536 ? 1 : hidden <= 2 * 1536 ? 2 : 4;
-    const int64_t rows_of_block = W == 1 ? 2 : 1;  // per tensor
-    int64_t blocks = W == 4 ? 2 * (int64_t)rows : (rows + rows_of_block - 1) / rows_of_block;
-    if (blocks > max_blocks()) blocks = max_blocks();  // even, as 4 blocks per SM
-    part_rows = (int)(W == 4 ? blocks / 2 : blocks);
-    const int vpl = (hidden / 8 + 32 * W - 1) / (32 * W);
-    const size_t smem = W == 1 ? (size_t)2 * hidden * sizeof(float) : 0;
-#define SA_LAUNCH(V, WW) kernel<V, WW><<<(int)blocks, 32 * kWarps, smem, stream>>>(p)
-    if (W == 1) {
-      if (vpl <= 2) SA_LAUNCH(2, 1);
-      else if (vpl <= 4) SA_LAUNCH(4, 1);
-      else SA_LAUNCH(6, 1);
-    } else if (W == 2) {
-      if (vpl <= 4) SA_LAUNCH(4, 2);
-      else SA_LAUNCH(6, 2);
-    } else {
-      SA_LAUNCH(4, 4);
-    }
-#undef SA_LAUNCH
+    const int threads = threads_of(hidden);
+    part_rows = blocks_of(rows, threads);
+    if (threads <= 256) kernel<256><<<part_rows, threads, 0, stream>>>(p);
+    else kernel<kMaxThreads><<<part_rows, threads, 0, stream>>>(p);
     SA_CUDA_TRY(cudaGetLastError());
   }
   if (dw_q == nullptr) return SA_OK;
