@@ -186,9 +186,6 @@ def strides4(t) -> "ctypes.Array":
     return _c_i64_4(*[int(x) for x in st])
 
 
-def strides4_opt(t) -> "ctypes.Array | None":
-    return None if t is None else _c_i64_4(*t.stride())
-
 
 def strides3(t) -> "ctypes.Array":
     st = t.stride()

@@ -56,6 +56,38 @@ def _as_kernel_layout(t: torch.Tensor) -> torch.Tensor:
     return t if _bf16_view_ok(t) else t.contiguous()
 
 
+# Checks and ctypes arguments that follow from the tensors' metadata alone
+# (shapes, strides, types, devices) are worked out once per combination and
+# kept: what a call still does is pointers, alignment, buffers and the launch.
+_PLANS: dict = {}
+
+
+def _remember(key, plan):
+    if len(_PLANS) >= 4096:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
+
+
+def _meta(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+
+
+def _launch(idx: int, name: str, fn, *args) -> None:
+    """Calls an entry point whose last argument is the stream, on device idx."""
+    if torch.cuda.current_device() == idx:
+        rc = fn(*args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, _raw_stream(idx))
+    if rc != _lib.SA_OK:
+        _lib.check(rc, name)
+
+
 class DeviceStatus:
     """The status word kernels write when a bounded wait gives up, one per
     device, in mapped page-locked host memory (sa_status_create): kernels
@@ -214,8 +246,36 @@ def bsattn_bwd(
     sa_bsattn_bwd_workspace_size bytes) may hold anything; calls sharing one
     must not overlap on the GPU.
     """
-    dev = _require_cuda(dout, q, k, v, out, lse, block_mask, head_mask_type, dlse, dq, dk, dv,
-                        workspace)
+    key = ("bsattn_bwd", _meta(dout), _meta(q), _meta(k), _meta(v), _meta(out), _meta(lse),
+           _meta(block_mask), softmax_scale, _meta(head_mask_type), _meta(dlse), _meta(dq),
+           _meta(dk), _meta(dv))
+    plan = _PLANS.get(key) or _remember(key, _bsattn_bwd_plan(
+        dout, q, k, v, out, lse, block_mask, softmax_scale, head_mask_type, dlse, dq, dk, dv))
+    idx, dev, fits, in_strides, middle, grads, out_strides, need, status = plan
+    ins = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
+    if not fits or (ins[0] | ins[1] | ins[2] | ins[3] | ins[4]) & 15:
+        dout, q, k, v, out = (_aligned(t) if not _view16_ok(t) else t
+                              for t in (dout, q, k, v, out))
+        return bsattn_bwd(dout, q, k, v, out, lse.contiguous(), block_mask, softmax_scale,
+                          None if head_mask_type is None else head_mask_type.contiguous(),
+                          None if dlse is None else dlse.contiguous(), dq, dk, dv, workspace)
+    # each gradient by default [B,S,H,D]-contiguous, viewed [B,H,S,D]
+    dq, dk, dv = (torch.empty_strided(*g, dtype=torch.bfloat16, device=dev) if t is None else t
+                  for t, g in zip((dq, dk, dv), grads))
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.get_device() != idx:
+        raise RuntimeError(f"bsattn_bwd: workspace must be on {dev}")
+    _launch(idx, "sa_bsattn_bwd", _lib.load().sa_bsattn_bwd, *ins, *in_strides, lse.data_ptr(),
+            _ptr(dlse), *middle[0], block_mask.data_ptr(), *middle[1], _ptr(head_mask_type),
+            middle[2], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *out_strides,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), status)
+    return dq, dk, dv
+
+
+def _bsattn_bwd_plan(dout, q, k, v, out, lse, block_mask, softmax_scale, head_mask_type, dlse, dq,
+                     dk, dv):
+    dev = _require_cuda(dout, q, k, v, out, lse, block_mask, head_mask_type, dlse, dq, dk, dv)
     if q.dim() != 4 or k.dim() != 4:
         raise RuntimeError("bsattn_bwd expects 4-D [B,H,S,D] tensors")
     B, H, Sq, D = q.shape
@@ -234,36 +294,22 @@ def bsattn_bwd(
         if t is not None and (t.dtype != torch.float32 or t.shape != (B, H, Sq)):
             raise RuntimeError(f"bsattn_bwd: {name} must be fp32 {(B, H, Sq)}, got {t.dtype} "
                                f"{tuple(t.shape)}")
-    head_mask_type = _check_block_mask("bsattn_bwd", block_mask, head_mask_type, B, H, Sq, Sk)
-    dout, q, k, v, out = (_as_kernel_layout(t) for t in (dout, q, k, v, out))
-    lse = lse.contiguous()
-    dlse = None if dlse is None else dlse.contiguous()
-
-    def grad(S):
-        return torch.empty((B, S, H, D), dtype=torch.bfloat16, device=dev).permute(0, 2, 1, 3)
-
-    dq = grad(Sq) if dq is None else dq
-    dk = grad(Sk) if dk is None else dk
-    dv = grad(Sk) if dv is None else dv
-    lib = _lib.load()
-    need = int(lib.sa_bsattn_bwd_workspace_size(B, H, Sq, Sk))
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _check_block_mask("bsattn_bwd", block_mask, head_mask_type, B, H, Sq, Sk)
+    fits = (all(t.stride(-1) == 1 and not any(x % 8 for x in t.stride()[:-1])
+                for t in (dout, q, k, v, out))
+            and all(t is None or t.is_contiguous() for t in (lse, dlse, head_mask_type)))
+    need = int(_lib.load().sa_bsattn_bwd_workspace_size(B, H, Sq, Sk))
     ms = list(block_mask.stride())
     if block_mask.shape[0] == 1:
         ms[0] = 0
-    st = _lib.strides4
-    with torch.cuda.device(dev):
-        rc = lib.sa_bsattn_bwd(
-            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), st(dout),
-            st(q), st(k), st(v), st(out), lse.data_ptr(), _ptr(dlse), B, H, Sq, Sk, D,
-            block_mask.data_ptr(), (_lib.ctypes.c_int64 * 4)(*ms), block_mask.shape[1],
-            _ptr(head_mask_type), -1.0 if softmax_scale is None else float(softmax_scale),
-            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), st(dq), st(dk), st(dv),
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-            DeviceStatus.pointer(dev), _stream(dev))
-    _lib.check(rc, "sa_bsattn_bwd")
-    return dq, dk, dv
+    i64x4 = _lib.ctypes.c_int64 * 4
+    grads = [((B, H, S, D), (S * H * D, D, H * D, 1)) for S in (Sq, Sk, Sk)]
+    out_strides = [i64x4(*(g[1] if t is None else t.stride()))
+                   for t, g in zip((dq, dk, dv), grads)]
+    return (dev.index, dev, fits, [_lib.strides4(t) for t in (dout, q, k, v, out)],
+            ((B, H, Sq, Sk, D), (i64x4(*ms), block_mask.shape[1]),
+             -1.0 if softmax_scale is None else float(softmax_scale)),
+            grads, out_strides, need, DeviceStatus.pointer(dev))
 
 
 def _check_block_mask(fn: str, block_mask: torch.Tensor, head_mask_type: Optional[torch.Tensor],
@@ -928,7 +974,52 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
     without weights). Equal calls give equal bits. Calls sharing a `workspace`
     (uint8, sa_qk_norm_rope_bwd_workspace_size bytes) must not overlap.
     """
-    dev = _require_cuda(dq_out, dk_out, q, k, w_q, w_k, cos, sin, dq, dk, workspace)
+    key = ("qk_norm_rope_bwd", _meta(dq_out), _meta(dk_out), _meta(q), _meta(k), head_dim, eps,
+           _meta(w_q), _meta(w_k), _meta(cos), _meta(sin), _meta(dq), _meta(dk))
+    plan = _PLANS.get(key) or _remember(key, _qk_norm_rope_bwd_plan(
+        dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, sin, dq, dk))
+    idx, dev, fits, in_rows, sizes, w_bf16, fs, out_rows, need = plan
+    ptrs = [_ptr(t) for t in (dq_out, dk_out, q, k, w_q, w_k, cos, sin)]
+    if not fits or any(x is not None and x & 15 for x in ptrs):
+        def rows(t):
+            return t if _uniform_rows(t) and t.data_ptr() % 16 == 0 else _aligned(t)
+
+        def weight(w):
+            return w if w is None else _aligned(w if w_bf16 else w.float())
+
+        def table(t):
+            return t if t is None else _aligned(t.float())
+
+        return qk_norm_rope_bwd(rows(dq_out), rows(dk_out), rows(q), rows(k), head_dim, eps,
+                                weight(w_q), weight(w_k), table(cos), table(sin), dq, dk,
+                                workspace)
+    dq = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if dq is None else dq
+    dk = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if dk is None else dk
+    dw_q = dw_k = None
+    if need:
+        dw_q = torch.empty(sizes[2], dtype=torch.float32, device=dev)
+        dw_k = torch.empty(sizes[2], dtype=torch.float32, device=dev)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.get_device() != idx:
+            raise RuntimeError(f"qk_norm_rope_bwd: workspace must be on {dev}")
+    ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if need \
+        else (None, 0)
+    _launch(idx, "sa_qk_norm_rope_bwd", _lib.load().sa_qk_norm_rope_bwd, ptrs[0], ptrs[1],
+            in_rows[0], in_rows[1], ptrs[2], ptrs[3], in_rows[2], in_rows[3], *sizes, ptrs[4],
+            ptrs[5], w_bf16, eps, ptrs[6], ptrs[7], fs, dq.data_ptr(), dk.data_ptr(), *out_rows,
+            _ptr(dw_q), _ptr(dw_k), *ws)
+    return dq, dk, dw_q, dw_k
+
+
+def _uniform_rows(t: torch.Tensor) -> bool:
+    """[B, S, hidden] whose B * S rows lie at one stride of whole 16-byte vectors."""
+    return t.numel() == 0 or (t.stride(-1) == 1 and t.stride(1) % 8 == 0
+                              and (t.shape[0] == 1 or t.stride(0) == t.shape[1] * t.stride(1)))
+
+
+def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, sin, dq, dk):
+    dev = _require_cuda(dq_out, dk_out, q, k, w_q, w_k, cos, sin, dq, dk)
     if q.dim() != 3:
         raise RuntimeError("qk_norm_rope_bwd expects [B, S, hidden] tensors")
     B, S, hidden = q.shape
@@ -937,53 +1028,31 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
         if t is not None and (t.dtype != torch.bfloat16 or t.shape != (B, S, hidden)):
             raise RuntimeError(f"qk_norm_rope_bwd: {name} must be bf16 {(B, S, hidden)}, got "
                                f"{t.dtype} {tuple(t.shape)}")
-
-    def rows(t):  # uniform 16-byte rows, as the kernel walks them
-        return t.numel() == 0 or (
-            t.stride(-1) == 1 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
-            and (B == 1 or t.stride(0) == S * t.stride(1)))
-
-    dq_out, dk_out, q, k = (t if rows(t) else _aligned(t) for t in (dq_out, dk_out, q, k))
-    dq = torch.empty((B, S, hidden), dtype=torch.bfloat16, device=dev) if dq is None else dq
-    dk = torch.empty((B, S, hidden), dtype=torch.bfloat16, device=dev) if dk is None else dk
-    if not (rows(dq) and rows(dk)):
-        raise RuntimeError("qk_norm_rope_bwd outputs need uniform rows, 16-byte aligned")
+        if t is not None and name in ("dq", "dk") and not _uniform_rows(t):
+            raise RuntimeError("qk_norm_rope_bwd outputs need uniform rows, 16-byte aligned")
     if (w_q is None) != (w_k is None) or (cos is None) != (sin is None):
         raise RuntimeError("qk_norm_rope_bwd: w_q and w_k, cos and sin go together")
-    dw_q = dw_k = None
+    fits = all(_uniform_rows(t) for t in (dq_out, dk_out, q, k))
     w_bf16 = 1
     if w_q is not None:
         if w_q.shape != (hidden,) or w_k.shape != (hidden,):
             raise RuntimeError(f"norm weights must have {hidden} elements")
-        if w_q.dtype == torch.bfloat16 and w_k.dtype == torch.bfloat16:
-            w_q, w_k = _aligned(w_q), _aligned(w_k)
-        else:
-            w_q, w_k, w_bf16 = _aligned(w_q.float()), _aligned(w_k.float()), 0
-        dw_q = torch.empty(hidden, dtype=torch.float32, device=dev)
-        dw_k = torch.empty(hidden, dtype=torch.float32, device=dev)
-    fs = 0
+        w_bf16 = int(w_q.dtype == torch.bfloat16 and w_k.dtype == torch.bfloat16)
+        fits = fits and w_q.is_contiguous() and w_k.is_contiguous() and (
+            w_bf16 or w_q.dtype == w_k.dtype == torch.float32)
     if cos is not None:
         if cos.shape != (S, head_dim // 2) or sin.shape != (S, head_dim // 2):
             raise ValueError(f"Rotary frequency shape mismatch: expected {(S, head_dim // 2)}, "
                              f"got {tuple(cos.shape)} and {tuple(sin.shape)}")
-        cos, sin = _aligned(cos.float()), _aligned(sin.float())
-        fs = cos.stride(0)
-    lib = _lib.load()
-    ws_bytes = 0
-    with torch.cuda.device(dev):
-        if dw_q is not None:
-            if workspace is None:
-                workspace = torch.empty(int(lib.sa_qk_norm_rope_bwd_workspace_size(hidden)),
-                                        dtype=torch.uint8, device=dev)
-            ws_bytes = workspace.numel() * workspace.element_size()
-        rc = lib.sa_qk_norm_rope_bwd(
-            dq_out.data_ptr(), dk_out.data_ptr(), dq_out.stride(1), dk_out.stride(1),
-            q.data_ptr(), k.data_ptr(), q.stride(1), k.stride(1), B * S, max(S, 1), hidden,
-            int(head_dim), _ptr(w_q), _ptr(w_k), w_bf16, float(eps), _ptr(cos), _ptr(sin), fs,
-            dq.data_ptr(), dk.data_ptr(), dq.stride(1), dk.stride(1), _ptr(dw_q), _ptr(dw_k),
-            _ptr(workspace) if ws_bytes else None, ws_bytes, _stream(dev))
-    _lib.check(rc, "sa_qk_norm_rope_bwd")
-    return dq, dk, dw_q, dw_k
+        fits = fits and all(t.dtype == torch.float32 and t.is_contiguous() for t in (cos, sin))
+    need = 0
+    if w_q is not None:
+        with torch.cuda.device(dev):
+            need = int(_lib.load().sa_qk_norm_rope_bwd_workspace_size(hidden))
+    return (dev.index, dev, fits, [t.stride(1) for t in (dq_out, dk_out, q, k)],
+            (B * S, max(S, 1), hidden, int(head_dim)), w_bf16,
+            0 if cos is None else head_dim // 2,
+            [hidden if t is None else t.stride(1) for t in (dq, dk)], need)
 
 
 _DTYPES = {torch.bfloat16: _lib.SA_DTYPE_BF16, torch.float16: _lib.SA_DTYPE_FP16,
@@ -1002,29 +1071,45 @@ def _view16_ok(t: torch.Tensor) -> bool:
             and not any(s % n for s in t.stride()[:-1]))
 
 
-def _head_norm_args(fn: str, q, k, w_q, w_k, cos, sin, positions, interleaved):
-    """Checks and lays out what qk_head_norm_rope and its gradient share; the
-    order of the returned arguments is the C entry points'."""
+def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, outs):
+    """What qk_head_norm_rope and its gradient derive from their tensors'
+    metadata. more: further (name, tensor, like) inputs; outs: the same of
+    outputs, None for one to be allocated."""
+    dev = _require_cuda(q, k, w_q, w_k, cos, sin, positions, *(t for _, t, _ in more + outs))
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise RuntimeError(f"{fn} expects q, k of [B, S, heads, D]")
     B, S, Hq, D = q.shape
     Hk = 0 if k is None else k.shape[2]
     if q.dtype not in _DTYPES:
         raise RuntimeError(f"{fn} expects bf16, fp16 or fp32, got {q.dtype}")
-    if k is not None and (k.dtype != q.dtype or k.shape != (B, S, Hk, D)):
-        raise RuntimeError(f"{fn}: k must be {q.dtype} {(B, S, Hk, D)}, got {k.dtype} "
+    if k is not None and (k.dtype != q.dtype or k.shape != (B, S, Hk, D) or Hk == 0):
+        raise RuntimeError(f"{fn}: k must be {q.dtype} [{B}, {S}, heads, {D}], got {k.dtype} "
                            f"{tuple(k.shape)}")
-    if (w_q is None) != (w_k is None) and k is not None or (w_q is None and w_k is not None):
-        raise RuntimeError(f"{fn}: w_q and w_k go together")
+    for name, t, like in more + outs:
+        if like is None and t is not None:
+            raise RuntimeError(f"{fn}: {name} without k")
+        if t is not None and (t.dtype != like.dtype or t.shape != like.shape):
+            raise RuntimeError(f"{fn}: {name} must be {like.dtype} {tuple(like.shape)}, got "
+                               f"{t.dtype} {tuple(t.shape)}")
+    for name, t, like in more:
+        if like is not None and t is None:
+            raise RuntimeError(f"{fn}: {name} is missing")
+    for name, t, _ in outs:
+        if t is not None and not _strides16_ok(t):
+            raise RuntimeError(f"{fn}: {name} must have stride(-1)=1, 16-byte strides and "
+                               "alignment")
+    fits = all(t is None or _strides16_ok(t) for t in (q, k, *(t for _, t, _ in more)))
     w_dtype = _lib.SA_DTYPE_FP32
+    if w_q is None and w_k is not None or k is not None and (w_q is None) != (w_k is None):
+        raise RuntimeError(f"{fn}: w_q and w_k go together")
     if w_q is not None:
-        same = w_q.dtype in _DTYPES and (w_k is None or w_k.dtype == w_q.dtype)
         for w in (w_q, w_k):
             if w is not None and w.shape != (D,):
                 raise RuntimeError(f"{fn}: norm weights must have {D} elements, got "
                                    f"{tuple(w.shape)}")
-        w_q, w_k = (None if w is None else _aligned(w if same else w.float()) for w in (w_q, w_k))
-        w_dtype = _DTYPES[w_q.dtype]
+        same = w_q.dtype in _DTYPES and (w_k is None or w_k.dtype == w_q.dtype)
+        fits = fits and same and w_q.is_contiguous() and (w_k is None or w_k.is_contiguous())
+        w_dtype = _DTYPES[w_q.dtype] if same else w_dtype
     if (cos is None) != (sin is None):
         raise RuntimeError(f"{fn}: cos and sin go together")
     fs = rot = rows = 0
@@ -1035,10 +1120,9 @@ def _head_norm_args(fn: str, q, k, w_q, w_k, cos, sin, positions, interleaved):
                                f", got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} "
                                f"{tuple(sin.shape)}")
         rows, rot = cos.shape[0], 2 * cos.shape[1]
-        if not (_view16_ok(cos) and _view16_ok(sin)) or cos.stride(0) != sin.stride(0) \
-                or cos.stride(0) < rot // 2:
-            cos, sin = _aligned(cos), _aligned(sin)
         fs = cos.stride(0)
+        fits = fits and _strides16_ok(cos) and _strides16_ok(sin) and fs == sin.stride(0) \
+            and fs >= rot // 2
     pst = None
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
@@ -1049,29 +1133,44 @@ def _head_norm_args(fn: str, q, k, w_q, w_k, cos, sin, positions, interleaved):
             raise RuntimeError(f"{fn}: positions need cos and sin")
         sb = positions.stride(0) if positions.dim() == 2 else 0
         pst = (_lib.ctypes.c_int64 * 2)(sb, positions.stride(-1))
-    tail = (B, S, Hq, Hk, D, _DTYPES[q.dtype], _ptr(w_q), _ptr(w_k), w_dtype)
-    tab = (_ptr(cos), _ptr(sin), fs, rows, rot, int(bool(interleaved)), _ptr(positions),
-           int(positions is not None and positions.dtype == torch.int64), pst)
-    # the tensors stay referenced until the launch
-    return tail, tab, (w_q, w_k, cos, sin, positions)
+    need = 0
+    if w_q is not None and more:
+        with torch.cuda.device(dev):
+            need = int(_lib.load().sa_qk_head_norm_rope_bwd_workspace_size(D))
+    i64x4 = _lib.ctypes.c_int64 * 4
+
+    def st(t, like):
+        if like is None:
+            return None
+        if t is None:
+            b, s, h, d = like.shape
+            return i64x4(s * h * d, h * d, d, 1)
+        return _lib.strides4(t)
+
+    return (dev.index, dev, fits, (st(q, q), st(k, k)), [st(t, like) for _, t, like in more],
+            [st(t, like) for _, t, like in outs], (B, S, Hq, Hk, D, _DTYPES[q.dtype]), w_dtype,
+            (fs, rows, rot, int(bool(interleaved))),
+            int(positions is not None and positions.dtype == torch.int64), pst, need,
+            DeviceStatus.pointer(dev))
 
 
-def _head_tensor(fn: str, name: str, t: Optional[torch.Tensor], like: Optional[torch.Tensor],
-                 out: bool):
-    if like is None:
-        if t is not None:
-            raise RuntimeError(f"{fn}: {name} without k")
-        return None
-    if t is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if t.dtype != like.dtype or t.shape != like.shape:
-        raise RuntimeError(f"{fn}: {name} must be {like.dtype} {tuple(like.shape)}, got {t.dtype} "
-                           f"{tuple(t.shape)}")
-    if _view16_ok(t):
-        return t
-    if out:
-        raise RuntimeError(f"{fn}: {name} must have stride(-1)=1, 16-byte strides and alignment")
-    return _aligned(t)
+def _strides16_ok(t: torch.Tensor) -> bool:
+    n = 16 // t.element_size()
+    return t.stride(-1) == 1 and not any(s % n for s in t.stride()[:-1])
+
+
+def _head_norm_copies(w_q, w_k, cos, sin, tensors):
+    """The arguments laid out as the kernels read them, copied where they are not."""
+    def fit(t):
+        return t if t is None or _view16_ok(t) else _aligned(t)
+
+    if w_q is not None:
+        same = w_q.dtype in _DTYPES and (w_k is None or w_k.dtype == w_q.dtype)
+        w_q, w_k = (None if w is None else _aligned(w if same else w.float()) for w in (w_q, w_k))
+    if cos is not None and not (_view16_ok(cos) and _view16_ok(sin)
+                                and cos.stride(0) == sin.stride(0) >= cos.shape[1]):
+        cos, sin = _aligned(cos), _aligned(sin)
+    return [fit(t) for t in tensors], w_q, w_k, cos, sin
 
 
 def qk_head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], eps: float,
@@ -1090,19 +1189,25 @@ def qk_head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], eps: float,
     reported by DeviceStatus. fp32 throughout, rounded once. Returns (q, k) of
     the input type; out_q/out_k may alias q/k or be views of a larger buffer.
     """
-    dev = _require_cuda(q, k, w_q, w_k, cos, sin, positions, out_q, out_k)
     fn = "qk_head_norm_rope"
-    sizes, tab, keep = _head_norm_args(fn, q, k, w_q, w_k, cos, sin, positions, interleaved)
-    q = _head_tensor(fn, "q", q, q, False)
-    k = _head_tensor(fn, "k", k, k, False)
-    out_q = _head_tensor(fn, "out_q", out_q, q, True)
-    out_k = _head_tensor(fn, "out_k", out_k, k, True)
-    st = _lib.strides4_opt
-    with torch.cuda.device(dev):
-        rc = _lib.load().sa_qk_head_norm_rope(
-            q.data_ptr(), _ptr(k), st(q), st(k), *sizes, float(eps), *tab, out_q.data_ptr(),
-            _ptr(out_k), st(out_q), st(out_k), DeviceStatus.pointer(dev), _stream(dev))
-    _lib.check(rc, "sa_qk_head_norm_rope")
+    key = (fn, _meta(q), _meta(k), _meta(w_q), _meta(w_k), _meta(cos), _meta(sin),
+           _meta(positions), interleaved, _meta(out_q), _meta(out_k))
+    plan = _PLANS.get(key) or _remember(key, _head_norm_plan(
+        fn, q, k, w_q, w_k, cos, sin, positions, interleaved, [],
+        [("out_q", out_q, q), ("out_k", out_k, k)]))
+    idx, dev, fits, st, _, ost, sizes, w_dtype, tab, pos64, pst, _, status = plan
+    pq, pk, pwq, pwk, pc, ps = (_ptr(t) for t in (q, k, w_q, w_k, cos, sin))
+    if not fits or (pq | (pk or 0) | (pwq or 0) | (pwk or 0) | (pc or 0) | (ps or 0)) & 15:
+        (q, k), w_q, w_k, cos, sin = _head_norm_copies(w_q, w_k, cos, sin, (q, k))
+        return qk_head_norm_rope(q, k, eps, w_q, w_k, cos, sin, positions, interleaved, out_q,
+                                 out_k)
+    if out_q is None:
+        out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if out_k is None and k is not None:
+        out_k = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    _launch(idx, "sa_qk_head_norm_rope", _lib.load().sa_qk_head_norm_rope, pq, pk, *st, *sizes,
+            pwq, pwk, w_dtype, eps, pc, ps, *tab, _ptr(positions), pos64, pst, out_q.data_ptr(),
+            _ptr(out_k), *ost, status)
     return out_q, out_k
 
 
@@ -1121,35 +1226,37 @@ def qk_head_norm_rope_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], 
     without weights). Equal calls give equal bits. Calls sharing a `workspace`
     (uint8, sa_qk_head_norm_rope_bwd_workspace_size bytes) must not overlap.
     """
-    dev = _require_cuda(dq_out, dk_out, q, k, w_q, w_k, cos, sin, positions, dq, dk, workspace)
     fn = "qk_head_norm_rope_bwd"
-    sizes, tab, keep = _head_norm_args(fn, q, k, w_q, w_k, cos, sin, positions, interleaved)
-    if k is not None and dk_out is None:
-        raise RuntimeError(f"{fn}: dk_out is missing")
+    key = (fn, _meta(dq_out), _meta(dk_out), _meta(q), _meta(k), _meta(w_q), _meta(w_k),
+           _meta(cos), _meta(sin), _meta(positions), interleaved, _meta(dq), _meta(dk))
+    plan = _PLANS.get(key) or _remember(key, _head_norm_plan(
+        fn, q, k, w_q, w_k, cos, sin, positions, interleaved,
+        [("dq_out", dq_out, q), ("dk_out", dk_out, k)], [("dq", dq, q), ("dk", dk, k)]))
+    idx, dev, fits, st, dst, ost, sizes, w_dtype, tab, pos64, pst, need, status = plan
+    ptrs = [_ptr(t) for t in (dq_out, dk_out, q, k, w_q, w_k, cos, sin)]
+    if not fits or any(x is not None and x & 15 for x in ptrs):
+        (dq_out, dk_out, q, k), w_q, w_k, cos, sin = _head_norm_copies(
+            w_q, w_k, cos, sin, (dq_out, dk_out, q, k))
+        return qk_head_norm_rope_bwd(dq_out, dk_out, q, k, eps, w_q, w_k, cos, sin, positions,
+                                     interleaved, dq, dk, workspace)
+    if dq is None:
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if dk is None and k is not None:
+        dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
     dw_q = dw_k = None
-    D = q.shape[-1]
-    if w_q is not None:
-        dw_q = torch.empty(D, dtype=torch.float32, device=dev)
-        dw_k = None if k is None else torch.empty(D, dtype=torch.float32, device=dev)
-    dq_out = _head_tensor(fn, "dq_out", dq_out, q, False)
-    dk_out = _head_tensor(fn, "dk_out", dk_out, k, False)
-    q, k = _head_tensor(fn, "q", q, q, False), _head_tensor(fn, "k", k, k, False)
-    dq, dk = _head_tensor(fn, "dq", dq, q, True), _head_tensor(fn, "dk", dk, k, True)
-    lib = _lib.load()
-    st = _lib.strides4_opt
-    ws_bytes = 0
-    with torch.cuda.device(dev):
-        if dw_q is not None:
-            if workspace is None:
-                workspace = torch.empty(int(lib.sa_qk_head_norm_rope_bwd_workspace_size(D)),
-                                        dtype=torch.uint8, device=dev)
-            ws_bytes = workspace.numel() * workspace.element_size()
-        rc = lib.sa_qk_head_norm_rope_bwd(
-            dq_out.data_ptr(), _ptr(dk_out), st(dq_out), st(dk_out), q.data_ptr(), _ptr(k), st(q),
-            st(k), *sizes, float(eps), *tab, dq.data_ptr(), _ptr(dk), st(dq), st(dk), _ptr(dw_q),
-            _ptr(dw_k), _ptr(workspace) if ws_bytes else None, ws_bytes,
-            DeviceStatus.pointer(dev), _stream(dev))
-    _lib.check(rc, "sa_qk_head_norm_rope_bwd")
+    if need:
+        dw_q = torch.empty(sizes[4], dtype=torch.float32, device=dev)
+        dw_k = None if k is None else torch.empty(sizes[4], dtype=torch.float32, device=dev)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.get_device() != idx:
+            raise RuntimeError(f"{fn}: workspace must be on {dev}")
+    ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if need \
+        else (None, 0)
+    _launch(idx, "sa_qk_head_norm_rope_bwd", _lib.load().sa_qk_head_norm_rope_bwd, ptrs[0],
+            ptrs[1], *dst, ptrs[2], ptrs[3], *st, *sizes, ptrs[4], ptrs[5], w_dtype, eps, ptrs[6],
+            ptrs[7], *tab, _ptr(positions), pos64, pst, dq.data_ptr(), _ptr(dk), *ost,
+            _ptr(dw_q), _ptr(dw_k), *ws, status)
     return dq, dk, dw_q, dw_k
 
 
