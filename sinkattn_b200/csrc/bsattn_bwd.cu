@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* b2_ring = b1_ring + kB1 * kTileBytes;
   SmemCtl* ctl = reinterpret_cast<SmemCtl*>(b2_ring + kB2 * kTileBytes);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);  // warp-uniform
   const int lane = threadIdx.x & 31;
   if ((smem_u32(smem) & 1023u) != 0u) {
     if (threadIdx.x == 0) report_timeout(p.status);
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
 
-  const uint32_t tmem = ctl->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   volatile int* abort_flag = &ctl->abort_flag;
 
   if (warp == 2) {
@@ -373,11 +373,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    // The elected-thread region in warp-uniform control flow and descriptors
+    // that are built once and moved by constants keep the issue short. Beside
+    // two arithmetic warps that fill the scheduler, 8 MMAs of 128x128x16 (512
+    // clocks of tensor core) took 791 clocks to issue this way and 1715 from a
+    // `lane == 0` branch (519 and 513 alone; in isolation, all SMs).
+    if (elect_one_sync()) {
       constexpr uint32_t idesc_kk = make_idesc_bf16(kT, kT, 0, 0);  // B rows are N, K-major
       constexpr uint32_t idesc_mn = make_idesc_bf16(kT, kT, 0, 1);  // B rows are K, N-major
-      const uint32_t a_base = smem_u32(a_tile);
-      const uint32_t b1_base = smem_u32(b1_ring), b2_base = smem_u32(b2_ring);
+      const uint64_t a_desc = make_sdesc_sw128(smem_u32(a_tile), 16, 1024);
+      const uint64_t b1_kk = make_sdesc_sw128(smem_u32(b1_ring), 16, 1024);
+      const uint64_t b2_kk = make_sdesc_sw128(smem_u32(b2_ring), 16, 1024);
+      const uint64_t b1_mn = make_sdesc_sw128(smem_u32(b1_ring), kBoxBytes, 1024);
+      const uint64_t b2_mn = make_sdesc_sw128(smem_u32(b2_ring), kBoxBytes, 1024);
+      constexpr uint64_t kTileDesc = kTileBytes >> 4;
       int J = 0;   // blocks of earlier tiles
       int e = 0;   // earlier tiles with blocks
       bool ok = true;
@@ -385,25 +394,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) ok = mbar_wait(bar, parity, p.status, abort_flag);
         return ok;
       };
-      auto b1_tile = [&](int i) { return b1_base + (uint32_t)(i % kB1) * kTileBytes; };
-      auto b2_tile = [&](int i) { return b2_base + (uint32_t)(i % kB2) * kTileBytes; };
       // D = A B^T with both tiles K-major in shared memory
-      auto mma_x = [&](uint32_t a, uint32_t b, uint32_t d_col) {
+      auto mma_x = [&](uint64_t a, uint64_t b, uint32_t d_col) {
+        const uint32_t d = tmem + d_col;
 #pragma unroll
         for (int kk = 0; kk < kT / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kBoxBytes + (kk & 3) * 32;
-          mma_ss(tmem + d_col, make_sdesc_sw128(a + off, 16, 1024),
-                 make_sdesc_sw128(b + off, 16, 1024), idesc_kk, kk > 0 ? 1u : 0u);
+          const uint64_t off = ((kk >> 2) * kBoxBytes + (kk & 3) * 32) >> 4;
+          mma_ss(d, a + off, b + off, idesc_kk, kk > 0 ? 1u : 0u);
         }
       };
       // acc (+)= A . B, A = bf16 pairs in TMEM: each warpgroup's 64 columns of
       // K lie in the first 32 of the 64 columns it read
-      auto mma_acc = [&](uint32_t a_col, uint32_t b, uint32_t d_col, bool first) {
+      auto mma_acc = [&](uint32_t a_col, uint64_t b, uint32_t d_col, bool first) {
+        const uint32_t d = tmem + d_col, a = tmem + a_col;
+        mma_ts(d, a, b, idesc_mn, first ? 0u : 1u);
 #pragma unroll
-        for (int kk = 0; kk < kT / 16; ++kk)
-          mma_ts(tmem + d_col, tmem + a_col + (kk >> 2) * 64 + (kk & 3) * 8,
-                 make_sdesc_sw128(b + kk * 2048, kBoxBytes, 1024), idesc_mn,
-                 (!first || kk > 0) ? 1u : 0u);
+        for (int kk = 1; kk < kT / 16; ++kk)
+          mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + ((kk * 2048) >> 4), idesc_mn, 1u);
       };
       for (int k = 0; ok; ++k) {
         const int slot = k & 1;
@@ -425,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j == 0 && !wait(&ctl->a_full[0], (uint32_t)e & 1u)) return;
             if (!wait(&ctl->b1_full[i % kB1], (uint32_t)(i / kB1) & 1u)) return;
             tc_fence_after();
-            mma_x(a_base, b1_tile(i), kColX);
+            mma_x(a_desc, b1_kk + (uint64_t)(i % kB1) * kTileDesc, kColX);
             mma_commit(&ctl->x_full);
             if (j == n - 1) mma_commit(&ctl->a_empty[0]);
           };
@@ -435,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (kind && j == 1 && !wait_acc()) return;
             if (!wait(&ctl->b2_full[i % kB2], (uint32_t)(i / kB2) & 1u)) return;
             tc_fence_after();
-            mma_x(a_base + kTileBytes, b2_tile(i), y_col(j));
+            mma_x(a_desc + kTileDesc, b2_kk + (uint64_t)(i % kB2) * kTileDesc, y_col(j));
             mma_commit(&ctl->y_full[i & 1]);
             if (kind) mma_commit(&ctl->b2_empty[i % kB2]);
             if (j == n - 1) mma_commit(&ctl->a_empty[1]);
@@ -449,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!kind) {
               if (!wait_acc()) break;
               tc_fence_after();
-              mma_acc(kColX, b2_tile(i), kColAcc1, j == 0);
+              mma_acc(kColX, b2_mn + (uint64_t)(i % kB2) * kTileDesc, kColAcc1, j == 0);
               mma_commit(&ctl->b2_empty[i % kB2]);
             }
             if (j + 1 < n) {
@@ -459,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait(&ctl->ds_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
             if (!wait_acc()) break;
             tc_fence_after();
-            mma_acc(y_col(j), b1_tile(i), kColAcc2, j == 0);
+            mma_acc(y_col(j), b1_mn + (uint64_t)(i % kB1) * kTileDesc, kColAcc2, j == 0);
             mma_commit(&ctl->b1_empty[i % kB1]);
             if (j + 1 < n && !kind) issue_y(j + 1);
           }
