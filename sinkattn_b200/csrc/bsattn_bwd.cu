@@ -63,7 +63,9 @@ struct __align__(16) SmemCtl {
   uint64_t a_full[2], a_empty[2];  // [0] A1, [1] A2
   uint64_t list_full[2], list_empty[2];
   uint64_t x_full;       // X of a block computed (commit)
-  uint64_t x_done;       // kind 0: P written over X; kind 1: X copied out. 256 arrivals
+  // kind 0: [c] columns 32c..32c+31 of each warpgroup's P written over X; kind
+  // 1: X copied out, [1] only. 256 arrivals
+  uint64_t x_done[2];
   uint64_t y_full[2];    // [block parity] Y computed (commit)
   uint64_t ds_full[2];   // [block parity] dS written over Y, 256 arrivals
   uint64_t acc_full;     // a tile's sums are complete (commit)
@@ -219,7 +221,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl->ds_full[i], 256);
     }
     mbar_init(&ctl->x_full, 1);
-    mbar_init(&ctl->x_done, 256);
+    mbar_init(&ctl->x_done[0], 256);
+    mbar_init(&ctl->x_done[1], 256);
     mbar_init(&ctl->acc_full, 1);
     mbar_init(&ctl->acc_free, 256);
     mbar_init(&ctl->drain, 1);
@@ -404,13 +407,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       // acc (+)= A . B, A = bf16 pairs in TMEM: each warpgroup's 64 columns of
-      // K lie in the first 32 of the 64 columns it read
-      auto mma_acc = [&](uint32_t a_col, uint64_t b, uint32_t d_col, bool first) {
+      // K lie in the first 32 of the 64 columns it read. Half c: the columns
+      // 32c..32c+31 of both warpgroups.
+      auto mma_acc_half = [&](int c, uint32_t a_col, uint64_t b, uint32_t d_col, bool first) {
         const uint32_t d = tmem + d_col, a = tmem + a_col;
-        mma_ts(d, a, b, idesc_mn, first ? 0u : 1u);
 #pragma unroll
-        for (int kk = 1; kk < kT / 16; ++kk)
-          mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + ((kk * 2048) >> 4), idesc_mn, 1u);
+        for (int u = 0; u < 4; ++u) {
+          const int kk = (u >> 1) * 4 + c * 2 + (u & 1);
+          mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + ((kk * 2048) >> 4), idesc_mn,
+                 u > 0 || !first ? 1u : 0u);
+        }
       };
       for (int k = 0; ok; ++k) {
         const int slot = k & 1;
@@ -451,13 +457,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           issue_y(0);
           for (int j = 0; j < n && ok; ++j) {
             const int i = J + j;
-            if (!wait(&ctl->x_done, (uint32_t)i & 1u)) break;
-            tc_fence_after();
             if (!kind) {
-              if (!wait_acc()) break;
+              // each half of P is used as soon as it is there
+              const uint64_t b = b2_mn + (uint64_t)(i % kB2) * kTileDesc;
+              if (!wait_acc() || !wait(&ctl->x_done[0], (uint32_t)i & 1u)) break;
               tc_fence_after();
-              mma_acc(kColX, b2_mn + (uint64_t)(i % kB2) * kTileDesc, kColAcc1, j == 0);
+              mma_acc_half(0, kColX, b, kColAcc1, j == 0);
+              if (!wait(&ctl->x_done[1], (uint32_t)i & 1u)) break;
+              tc_fence_after();
+              mma_acc_half(1, kColX, b, kColAcc1, false);
               mma_commit(&ctl->b2_empty[i % kB2]);
+            } else {
+              if (!wait(&ctl->x_done[1], (uint32_t)i & 1u)) break;
+              tc_fence_after();
             }
             if (j + 1 < n) {
               issue_x(j + 1);
@@ -466,7 +478,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait(&ctl->ds_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
             if (!wait_acc()) break;
             tc_fence_after();
-            mma_acc(y_col(j), b1_mn + (uint64_t)(i % kB1) * kTileDesc, kColAcc2, j == 0);
+            const uint64_t b = b1_mn + (uint64_t)(i % kB1) * kTileDesc;
+            mma_acc_half(0, y_col(j), b, kColAcc2, j == 0);
+            mma_acc_half(1, y_col(j), b, kColAcc2, false);
             mma_commit(&ctl->b1_empty[i % kB1]);
             if (j + 1 < n && !kind) issue_y(j + 1);
           }
@@ -564,10 +578,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             tmem_st16(t_self + kColX + c * 16, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ctl->x_done[c]);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(&ctl->x_done);
           if (!wait(&ctl->y_full[jp & 1u], (jp >> 1) & 1u)) break;
           tc_fence_after();
           const ulonglong2* nd = reinterpret_cast<const ulonglong2*>(st + kT + g * 64);
@@ -603,7 +617,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           reg_fence32(r[0]);
           reg_fence32(r[1]);
           tc_fence_before();
-          mbar_arrive(&ctl->x_done);
+          mbar_arrive(&ctl->x_done[0]);  // unused here, kept in step with kind 0
+          mbar_arrive(&ctl->x_done[1]);
 #pragma unroll
           for (int u = 0; u < 32; ++u) {
             const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(r[u >> 4][2 * (u & 15)]),
