@@ -32,12 +32,15 @@ constexpr int kT = 128;            // rows of every tile; head dim
 // Ring slots. B1 of a block is held from X to the block's last product, B2 not
 // as long; 64 KB of resident tiles leave room for five.
 constexpr int kB1 = 3, kB2 = 2;
-constexpr int kThreads = 384;      // 4 role warps + 2 warpgroups of arithmetic
+constexpr int kGroups = 4;         // warpgroups of arithmetic
+constexpr int kCols = kT / kGroups;  // columns of X and Y each of them owns
+constexpr int kWorkers = kGroups * 128;
+constexpr int kThreads = 128 + kWorkers;  // 4 role warps, then the workers
 constexpr int kTileBytes = kT * kT * 2;
 constexpr int kBoxBytes = kTileBytes / 2;      // one 64-column box
 constexpr int kStatBytes = 2 * kT * 4;         // -lse (log2 units) and -delta of 128 rows
 constexpr int kMaxBlocks = 1024;               // per mask row or column (S <= 131072)
-constexpr int kListReaders = 2 + 256;
+constexpr int kListReaders = 2 + kWorkers;
 constexpr uint32_t kColX = 0, kColY = 128, kColAcc1 = 256, kColAcc2 = 384;
 
 struct Params {
@@ -63,13 +66,13 @@ struct __align__(16) SmemCtl {
   uint64_t a_full[2], a_empty[2];  // [0] A1, [1] A2
   uint64_t list_full[2], list_empty[2];
   uint64_t x_full;       // X of a block computed (commit)
-  // kind 0: [c] columns 32c..32c+31 of each warpgroup's P written over X; kind
-  // 1: X copied out, [1] only. 256 arrivals
+  // kind 0: [c] half c of each warpgroup's P columns written over X; kind 1: X
+  // copied out. kWorkers arrivals
   uint64_t x_done[2];
   uint64_t y_full[2];    // [block parity] Y computed (commit)
-  uint64_t ds_full[2];   // [block parity] dS written over Y, 256 arrivals
+  uint64_t ds_full[2];   // [block parity] dS written over Y, kWorkers arrivals
   uint64_t acc_full;     // a tile's sums are complete (commit)
-  uint64_t acc_free;     // a tile's sums have been read, 256 arrivals
+  uint64_t acc_free;     // a tile's sums have been read, kWorkers arrivals
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
@@ -154,34 +157,30 @@ __global__ void __launch_bounds__(256)
 }
 
 // Writes one 128x128 fp32 accumulator (times mul) as bf16 rows; this thread's
-// half: 64 columns of its row.
+// part: kCols columns of its row.
 __device__ __forceinline__ void store_acc(uint32_t taddr, float mul, __nv_bfloat16* dst,
                                           bool write) {
+  uint32_t o[kCols];
+  tmem_ld32(taddr, o);
+  tmem_wait_ld();
+  reg_fence32(o);
+  if (!write) return;
+  uint4* d4 = reinterpret_cast<uint4*>(dst);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t o[32];
-    tmem_ld32(taddr + c * 32, o);
-    tmem_wait_ld();
-    reg_fence32(o);
-    if (write) {
-      uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+  for (int v = 0; v < kCols / 8; ++v) {
+    uint32_t w[4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        uint32_t w[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          w[u] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * u]) * mul,
-                             __uint_as_float(o[8 * v + 2 * u + 1]) * mul);
-        d4[v] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
+    for (int u = 0; u < 4; ++u)
+      w[u] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * u]) * mul,
+                         __uint_as_float(o[8 * v + 2 * u + 1]) * mul);
+    d4[v] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
 __device__ __forceinline__ void store_zero(__nv_bfloat16* dst) {
   uint4* d4 = reinterpret_cast<uint4*>(dst);
 #pragma unroll
-  for (int v = 0; v < 8; ++v) d4[v] = make_uint4(0, 0, 0, 0);
+  for (int v = 0; v < kCols / 8; ++v) d4[v] = make_uint4(0, 0, 0, 0);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -218,13 +217,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl->list_full[i], 1);
       mbar_init(&ctl->list_empty[i], kListReaders);
       mbar_init(&ctl->y_full[i], 1);
-      mbar_init(&ctl->ds_full[i], 256);
+      mbar_init(&ctl->ds_full[i], kWorkers);
     }
     mbar_init(&ctl->x_full, 1);
-    mbar_init(&ctl->x_done[0], 256);
-    mbar_init(&ctl->x_done[1], 256);
+    mbar_init(&ctl->x_done[0], kWorkers);
+    mbar_init(&ctl->x_done[1], kWorkers);
     mbar_init(&ctl->acc_full, 1);
-    mbar_init(&ctl->acc_free, 256);
+    mbar_init(&ctl->acc_free, kWorkers);
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     fence_barrier_init();
@@ -406,15 +405,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_ss(d, a + off, b + off, idesc_kk, kk > 0 ? 1u : 0u);
         }
       };
-      // acc (+)= A . B, A = bf16 pairs in TMEM: each warpgroup's 64 columns of
-      // K lie in the first 32 of the 64 columns it read. Half c: the columns
-      // 32c..32c+31 of both warpgroups.
+      // acc (+)= A . B, A = bf16 pairs in TMEM: the kCols columns of each
+      // warpgroup lie packed in the first half of the columns it read. Half c:
+      // the c-th half of every warpgroup's columns.
       auto mma_acc_half = [&](int c, uint32_t a_col, uint64_t b, uint32_t d_col, bool first) {
+        constexpr int per = kCols / 16;  // 16-column steps of a warpgroup
         const uint32_t d = tmem + d_col, a = tmem + a_col;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int kk = (u >> 1) * 4 + c * 2 + (u & 1);
-          mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + ((kk * 2048) >> 4), idesc_mn,
+          const int kk = (u / (per / 2)) * per + c * (per / 2) + u % (per / 2);
+          mma_ts(d, a + (kk / per) * kCols + (kk % per) * 8, b + ((kk * 2048) >> 4), idesc_mn,
                  u > 0 || !first ? 1u : 0u);
         }
       };
@@ -497,12 +497,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= 4) {
     // ---------------- probabilities, dS and the outputs ----------------
-    // Warpgroup g owns columns 64g..64g+63 of X and Y; a thread one row (TMEM
-    // lane) of them. P is kept in fp32 registers from X to dS.
+    // Warpgroup g owns columns kCols g, ... of X and Y; a thread one row (TMEM
+    // lane) of them. P is kept in fp32 registers from X to dS. Four warps per
+    // scheduler hide each other's TMEM and barrier latencies.
     const int g = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_self = tmem + lane_off + g * 64;
+    const uint32_t t_self = tmem + lane_off + g * kCols;
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     bool ok = true;
     int J = 0, e = 0;
@@ -522,10 +523,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool write = grow < (tl.kind ? p.Sq : p.Sk);
       __nv_bfloat16 *o1 = nullptr, *o2;
       if (tl.kind) {
-        o2 = p.dq + tl.b * p.dqs0 + tl.h * p.dqs1 + (int64_t)grow * p.dqs2 + g * 64;
+        o2 = p.dq + tl.b * p.dqs0 + tl.h * p.dqs1 + (int64_t)grow * p.dqs2 + g * kCols;
       } else {
-        o1 = p.dv + tl.b * p.dvs0 + tl.h * p.dvs1 + (int64_t)grow * p.dvs2 + g * 64;
-        o2 = p.dk + tl.b * p.dks0 + tl.h * p.dks1 + (int64_t)grow * p.dks2 + g * 64;
+        o1 = p.dv + tl.b * p.dvs0 + tl.h * p.dvs1 + (int64_t)grow * p.dvs2 + g * kCols;
+        o2 = p.dk + tl.b * p.dks0 + tl.h * p.dks1 + (int64_t)grow * p.dks2 + g * kCols;
       }
       if (n == 0) {
         if (write) {
@@ -547,92 +548,79 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t row_nl2 = f2_pack(row_nl, row_nl), row_nd2 = f2_pack(row_nd, row_nd);
       for (int j = 0; j < n; ++j) {
         const uint32_t jp = (uint32_t)(J + j);
-        uint64_t pr[32];  // 64 probabilities, in pairs
+        uint64_t pr[kCols / 2];  // the probabilities, in pairs
         if (!wait(&ctl->st_full[jp & 1u], (jp >> 1) & 1u)) break;
         if (tl.kind == 0) {
           const float* st = ctl->stats[jp & 1u];
           if (!wait(&ctl->x_full, jp & 1u)) break;
           tc_fence_after();
-          const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(st + g * 64);
+          const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(st + g * kCols);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            uint32_t r[32], pk[16];
-            tmem_ld32(t_self + kColX + c * 32, r);
+            uint32_t r[16], pk[8];
+            tmem_ld16(t_self + kColX + c * 16, r);
             tmem_wait_ld();
-            reg_fence32(r);
+            reg_fence16(r);
 #pragma unroll
-            for (int u = 0; u < 16; u += 2) {
-              const ulonglong2 s2 = nl[c * 8 + (u >> 1)];
-#pragma unroll
-              for (int v = 0; v < 2; ++v) {
-                const uint64_t x2 =
-                    f2_fma(f2_pack(__uint_as_float(r[2 * (u + v)]),
-                                   __uint_as_float(r[2 * (u + v) + 1])),
-                           scale2, v ? s2.y : s2.x);
-                float x0, x1;
-                f2_unpack(x2, x0, x1);
-                x0 = ex2_approx(x0);
-                x1 = ex2_approx(x1);
-                pr[c * 16 + u + v] = f2_pack(x0, x1);
-                pk[u + v] = pack_bf16x2(x0, x1);
-              }
+            for (int u = 0; u < 8; ++u) {
+              const ulonglong2 s2 = nl[c * 4 + (u >> 1)];
+              const uint64_t x2 = f2_fma(
+                  f2_pack(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])), scale2,
+                  u & 1 ? s2.y : s2.x);
+              float x0, x1;
+              f2_unpack(x2, x0, x1);
+              x0 = ex2_approx(x0);
+              x1 = ex2_approx(x1);
+              pr[c * 8 + u] = f2_pack(x0, x1);
+              pk[u] = pack_bf16x2(x0, x1);
             }
-            tmem_st16(t_self + kColX + c * 16, pk);
+            tmem_st8(t_self + kColX + c * 8, pk);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&ctl->x_done[c]);
           }
           if (!wait(&ctl->y_full[jp & 1u], (jp >> 1) & 1u)) break;
           tc_fence_after();
-          const ulonglong2* nd = reinterpret_cast<const ulonglong2*>(st + kT + g * 64);
+          const ulonglong2* nd = reinterpret_cast<const ulonglong2*>(st + kT + g * kCols);
+          uint32_t r[32], pk[16];
+          tmem_ld32(t_self + kColY, r);
+          tmem_wait_ld();
+          reg_fence32(r);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t r[32], pk[16];
-            tmem_ld32(t_self + kColY + c * 32, r);
-            tmem_wait_ld();
-            reg_fence32(r);
-#pragma unroll
-            for (int u = 0; u < 16; u += 2) {
-              const ulonglong2 s2 = nd[c * 8 + (u >> 1)];
-#pragma unroll
-              for (int v = 0; v < 2; ++v) {
-                const uint64_t d2 = f2_mul(pr[c * 16 + u + v],
-                                           f2_add(f2_pack(__uint_as_float(r[2 * (u + v)]),
-                                                          __uint_as_float(r[2 * (u + v) + 1])),
-                                                  v ? s2.y : s2.x));
-                float d0, d1;
-                f2_unpack(d2, d0, d1);
-                pk[u + v] = pack_bf16x2(d0, d1);
-              }
-            }
-            tmem_st16(t_self + kColY + c * 16, pk);
+          for (int u = 0; u < 16; ++u) {
+            const ulonglong2 s2 = nd[u >> 1];
+            const uint64_t d2 = f2_mul(
+                pr[u], f2_add(f2_pack(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])),
+                              u & 1 ? s2.y : s2.x));
+            float d0, d1;
+            f2_unpack(d2, d0, d1);
+            pk[u] = pack_bf16x2(d0, d1);
           }
+          tmem_st16(t_self + kColY, pk);
         } else {
           if (!wait(&ctl->x_full, jp & 1u)) break;
           tc_fence_after();
-          uint32_t r[2][32];
-          tmem_ld32(t_self + kColX, r[0]);
-          tmem_ld32(t_self + kColX + 32, r[1]);
+          uint32_t r[32], pk[16];
+          tmem_ld32(t_self + kColX, r);
           tmem_wait_ld();
-          reg_fence32(r[0]);
-          reg_fence32(r[1]);
+          reg_fence32(r);
           tc_fence_before();
           mbar_arrive(&ctl->x_done[0]);  // unused here, kept in step with kind 0
           mbar_arrive(&ctl->x_done[1]);
 #pragma unroll
-          for (int u = 0; u < 32; ++u) {
-            const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(r[u >> 4][2 * (u & 15)]),
-                                               __uint_as_float(r[u >> 4][2 * (u & 15) + 1])),
-                                       scale2, row_nl2);
+          for (int u = 0; u < 16; ++u) {
+            const uint64_t x2 =
+                f2_fma(f2_pack(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])), scale2,
+                       row_nl2);
             float x0, x1;
             f2_unpack(x2, x0, x1);
             pr[u] = f2_pack(ex2_approx(x0), ex2_approx(x1));
           }
           // keys past Sk: their K rows are 0, but exp(-lse) may overflow
           if (ragged && j == n - 1) {
-            const int valid = p.Sk - (p.nk - 1) * kT - g * 64;
+            const int valid = p.Sk - (p.nk - 1) * kT - g * kCols;
 #pragma unroll
-            for (int u = 0; u < 32; ++u) {
+            for (int u = 0; u < 16; ++u) {
               float x0, x1;
               f2_unpack(pr[u], x0, x1);
               pr[u] = f2_pack(2 * u < valid ? x0 : 0.f, 2 * u + 1 < valid ? x1 : 0.f);
@@ -641,24 +629,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!wait(&ctl->y_full[jp & 1u], (jp >> 1) & 1u)) break;
           tc_fence_after();
           const uint32_t y = t_self + ((j & 1) ? kColAcc1 : kColY);
+          tmem_ld32(y, r);
+          tmem_wait_ld();
+          reg_fence32(r);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t q[32], pk[16];
-            tmem_ld32(y + c * 32, q);
-            tmem_wait_ld();
-            reg_fence32(q);
-#pragma unroll
-            for (int u = 0; u < 16; ++u) {
-              const uint64_t d2 =
-                  f2_mul(pr[c * 16 + u], f2_add(f2_pack(__uint_as_float(q[2 * u]),
-                                                        __uint_as_float(q[2 * u + 1])),
-                                                row_nd2));
-              float d0, d1;
-              f2_unpack(d2, d0, d1);
-              pk[u] = pack_bf16x2(d0, d1);
-            }
-            tmem_st16(y + c * 16, pk);
+          for (int u = 0; u < 16; ++u) {
+            const uint64_t d2 = f2_mul(
+                pr[u], f2_add(f2_pack(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])),
+                              row_nd2));
+            float d0, d1;
+            f2_unpack(d2, d0, d1);
+            pk[u] = pack_bf16x2(d0, d1);
           }
+          tmem_st16(y, pk);
         }
         tmem_wait_st();
         tc_fence_before();
