@@ -40,29 +40,42 @@ constexpr int kTileBytes = kT * kT * 2;
 constexpr int kBoxBytes = kTileBytes / 2;      // one 64-column box
 constexpr int kStatBytes = 2 * kT * 4;         // -lse (log2 units) and -delta of 128 rows
 constexpr int kMaxBlocks = 1024;               // per mask row or column (S <= 131072)
+constexpr int kLeastPiece = 8;                 // blocks
 constexpr int kListReaders = 2 + kWorkers;
 constexpr uint32_t kColX = 0, kColY = 128, kColAcc1 = 256, kColAcc2 = 384;
 
+struct Mask {
+  const uint8_t* mask;
+  int64_t s0, s1, s2, s3;
+  const int32_t* head_mask_type;
+};
+
 struct Params {
   int B, H, Sq, Sk, nq, nk;
-  const uint8_t* mask;
-  int64_t ms0, ms1, ms2, ms3;
-  const int32_t* head_mask_type;
+  Mask mask;
   float scale, scale_log2;
   const float* nstat;   // [B*H][nq*128][.]: first all -lse*log2(e), then all -delta
   int64_t stat_plane;   // elements of one plane
   __nv_bfloat16 *dq, *dk, *dv;
   int64_t dqs0, dqs1, dqs2, dks0, dks1, dks2, dvs0, dvs1, dvs2;
-  int* next_tile;
+  int* next_item;
   int32_t* status;
-  int tiles0, tiles;    // kind-0 tiles come first
+  // Work items: chunk 0 of every kind-0 tile, chunk 1 of each, ..., then the
+  // same of kind 1. A tile of `count` kept blocks is cut into
+  // clamp(count / least, 1, chunks) pieces, least from the total count.
+  int tiles[2], chunks[2], items[2];
+  const int* bh_count;   // kept blocks of every (batch, head); chunks > 1 only
+  int* joined[2];        // [tile][worker warp] pieces stored so far
+  float* part[2];        // [tile][chunk] fp32 sums of a piece
 };
 
 struct __align__(16) SmemCtl {
-  float stats[2][2 * kT];          // [block parity] -lse and -delta of a query block (kind 0)
+  // [block parity] -lse and -delta of the rows of a query block: of each block
+  // of kind 0, of a kind-1 tile with its first block
+  float stats[2][2 * kT];
   uint64_t b1_full[kB1], b1_empty[kB1];
   uint64_t b2_full[kB2], b2_empty[kB2];
-  uint64_t st_full[2];             // [block parity] statistics loaded (kind 1: a bare arrival)
+  uint64_t st_full[2];             // [block parity] statistics loaded, or none to load
   uint64_t a_full[2], a_empty[2];  // [0] A1, [1] A2
   uint64_t list_full[2], list_empty[2];
   uint64_t x_full;       // X of a block computed (commit)
@@ -78,6 +91,8 @@ struct __align__(16) SmemCtl {
   int abort_flag;
   int n_blocks[2];
   int tile_id[2];
+  int pieces[2];         // of the tile; > 1: this is piece `piece`
+  int piece[2];
   uint32_t kept[2][kMaxBlocks / 32];  // [slot] bit c of word i: block 32 i + c is kept
 };
 
@@ -90,16 +105,25 @@ struct Tile {
   int kind, blk, h, b;
 };
 
+// t: kind-0 tiles, then kind-1 tiles
 __device__ __forceinline__ Tile tile_of(const Params& p, int t) {
   Tile r;
-  r.kind = t >= p.tiles0 ? 1 : 0;
-  const int u = r.kind ? t - p.tiles0 : t;
+  r.kind = t >= p.tiles[0] ? 1 : 0;
+  const int u = r.kind ? t - p.tiles[0] : t;
   const int n = r.kind ? p.nq : p.nk;
   r.blk = u % n;
   const int bh = u / n;
   r.h = bh % p.H;
   r.b = bh / p.H;
   return r;
+}
+
+__device__ __forceinline__ bool head_mask(const int32_t* type, int h, int& mh) {
+  mh = h;
+  if (type == nullptr) return false;
+  const int ty = type[h];
+  if (ty > 0) mh = ty - 1;
+  return ty <= 0;  // dense
 }
 
 // Row statistics: one 16-lane group per query row sums dO . O in fp32. Rows
@@ -110,10 +134,31 @@ __global__ void __launch_bounds__(256)
     row_stats_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ out,
                      int64_t ds0, int64_t ds1, int64_t ds2, int64_t os0, int64_t os1, int64_t os2,
                      const float* __restrict__ lse, const float* __restrict__ dlse, int H, int Sq,
-                     int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_tile) {
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next_tile = 0;
+                     int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_item,
+                     int* joined, int n_joined, int* bh_count, const Mask mask, int nk) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next_item = 0;
+  for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_joined;
+       i += gridDim.x * gridDim.y * 256)
+    joined[i] = 0;
   const int bh = blockIdx.y;
   const int h = bh % H, b = bh / H;
+  if (bh_count != nullptr && blockIdx.x == 0) {
+    // kept blocks of this head, for the cut of long tiles
+    const int n = (rows_pad / kT) * nk;
+    int mh, c = 0;
+    const bool dense = head_mask(mask.head_mask_type, h, mh);
+    const uint8_t* m = mask.mask + b * mask.s0 + mh * mask.s1;
+    if (!dense)
+      for (int i = threadIdx.x; i < n; i += 256)
+        c += m[(int64_t)(i / nk) * mask.s2 + (int64_t)(i % nk) * mask.s3] != 0;
+    __shared__ int sum;
+    if (threadIdx.x == 0) sum = dense ? n : 0;
+    __syncthreads();
+    c = __reduce_add_sync(0xffffffffu, c);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&sum, c);
+    __syncthreads();
+    if (threadIdx.x == 0) bh_count[bh] = sum;
+  }
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
   const int r0 = blockIdx.x * (16 * kPrepRows) + g;
   uint4 x[kPrepRows], y[kPrepRows];
@@ -156,31 +201,82 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Writes one 128x128 fp32 accumulator (times mul) as bf16 rows; this thread's
-// part: kCols columns of its row.
-__device__ __forceinline__ void store_acc(uint32_t taddr, float mul, __nv_bfloat16* dst,
-                                          bool write) {
-  uint32_t o[kCols];
+// This thread's part of a 128x128 fp32 accumulator: kCols columns of its row.
+__device__ __forceinline__ void load_acc(uint32_t taddr, uint32_t (&o)[kCols]) {
   tmem_ld32(taddr, o);
   tmem_wait_ld();
   reg_fence32(o);
-  if (!write) return;
-  uint4* d4 = reinterpret_cast<uint4*>(dst);
-#pragma unroll
-  for (int v = 0; v < kCols / 8; ++v) {
-    uint32_t w[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      w[u] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * u]) * mul,
-                         __uint_as_float(o[8 * v + 2 * u + 1]) * mul);
-    d4[v] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
 }
 
-__device__ __forceinline__ void store_zero(__nv_bfloat16* dst) {
-  uint4* d4 = reinterpret_cast<uint4*>(dst);
+// Writes a warp's 32 rows x kCols columns (a row per lane, fp32 times mul) as
+// bf16. dst: this warp's first row and column; rows are `pitch` elements
+// apart, `rows` of them exist. Groups of four lanes first exchange 16-byte
+// pieces, so that each store covers 64 contiguous bytes of 8 rows: with a row
+// per lane, 16 bytes of 32 rows each, the stores of a tile took 2 to 4 us.
+static_assert(kCols == 32, "four 16-byte pieces of a row per lane");
+__device__ __forceinline__ void store_rows(const uint32_t (&o)[kCols], float mul,
+                                           __nv_bfloat16* dst, int64_t pitch, int rows,
+                                           int lane) {
+  uint32_t w[4][4];  // [piece][word]
 #pragma unroll
-  for (int v = 0; v < kCols / 8; ++v) d4[v] = make_uint4(0, 0, 0, 0);
+  for (int v = 0; v < 4; ++v)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      w[v][u] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * u]) * mul,
+                            __uint_as_float(o[8 * v + 2 * u + 1]) * mul);
+  // 4x4 transpose over lanes 4a..4a+3: afterwards w[i] is piece (lane & 3) of
+  // row 4a + i
+#pragma unroll
+  for (int step = 1; step < 4; step <<= 1) {
+    const bool hi = (lane & step) != 0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      if (v & step) continue;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t give = hi ? w[v][u] : w[v + step][u];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, step);
+        if (hi) w[v][u] = got; else w[v + step][u] = got;
+      }
+    }
+  }
+  __nv_bfloat16* d = dst + (int64_t)(lane & ~3) * pitch + (lane & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if ((lane & ~3) + i < rows)
+      *reinterpret_cast<uint4*>(d + i * pitch) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+}
+
+__device__ __forceinline__ void zero_rows(__nv_bfloat16* dst, int64_t pitch, int rows, int lane) {
+  __nv_bfloat16* d = dst + (int64_t)(lane & ~3) * pitch + (lane & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if ((lane & ~3) + i < rows) *reinterpret_cast<uint4*>(d + i * pitch) = make_uint4(0, 0, 0, 0);
+}
+
+// A piece's sums in fp32, 16-byte units by lane: each warp reads back only
+// what the same warp of another CTA stored.
+__device__ __forceinline__ void keep_part(const uint32_t (&o)[kCols], float* dst, int lane) {
+#pragma unroll
+  for (int v = 0; v < kCols / 4; ++v)
+    __stcg(reinterpret_cast<uint4*>(dst) + v * 32 + lane,
+           make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]));
+}
+
+__device__ __forceinline__ void sum_parts(const float* src, int pieces, int64_t size,
+                                          uint32_t (&o)[kCols], int lane) {
+#pragma unroll
+  for (int v = 0; v < kCols; ++v) o[v] = 0u;
+  for (int i = 0; i < pieces; ++i) {
+#pragma unroll
+    for (int v = 0; v < kCols / 4; ++v) {
+      const uint4 x = __ldcg(reinterpret_cast<const uint4*>(src + i * size) + v * 32 + lane);
+      const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        o[4 * v + u] = __float_as_uint(__uint_as_float(o[4 * v + u]) + __uint_as_float(y[u]));
+    }
+  }
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -246,56 +342,87 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &ctl->abort_flag;
 
   if (warp == 2) {
-    // ---------------- tiles and their kept-block lists, two ahead ----------------
+    // ---------------- work items and their kept blocks, two ahead ----------------
+    int least = 0x7fffffff;
+    if (p.bh_count != nullptr) {
+      // pieces of about half an SM's share of the blocks of both kinds, 8 at least
+      int total = 0;
+      for (int i = lane; i < p.B * p.H; i += 32) total += p.bh_count[i];
+      total = __reduce_add_sync(0xffffffffu, total);
+      least = max(kLeastPiece, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    }
     for (int k = 0;; ++k) {
       const int slot = k & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(&ctl->list_empty[slot], ((uint32_t)(k >> 1) & 1u) ^ 1u,
                                              p.status, abort_flag)))
         break;
-      int t = 0;
-      if (lane == 0) t = atomicAdd(p.next_tile, 1);
-      t = __shfl_sync(0xffffffffu, t, 0);
-      if (t >= p.tiles) {
-        if (lane == 0) {
-          ctl->tile_id[slot] = -1;
-          ctl->n_blocks[slot] = 0;
-          mbar_arrive(&ctl->list_full[slot]);
+      int t = -1, count = 0, pieces = 1, piece = 0;
+      uint32_t word = 0;  // lane i: blocks 32 i .. 32 i + 31
+      for (;;) {
+        int it = 0;
+        if (lane == 0) it = atomicAdd(p.next_item, 1);
+        it = __shfl_sync(0xffffffffu, it, 0);
+        const int kind = it >= p.items[0] ? 1 : 0;
+        if (kind) it -= p.items[0];
+        if (it >= p.items[kind]) break;
+        piece = it / p.tiles[kind];
+        const int tile = it - piece * p.tiles[kind] + (kind ? p.tiles[0] : 0);
+        const Tile tl = tile_of(p, tile);
+        int mh;
+        const bool dense = head_mask(p.mask.head_mask_type, tl.h, mh);
+        const uint8_t* m = p.mask.mask + (int64_t)tl.b * p.mask.s0 + (int64_t)mh * p.mask.s1 +
+                           (int64_t)tl.blk * (kind ? p.mask.s2 : p.mask.s3);
+        const int64_t step = kind ? p.mask.s3 : p.mask.s2;
+        const int n = kind ? p.nk : p.nq;
+        // all mask bytes are loaded before any is used; bit i of `bits` is block
+        // 32 i + lane
+        const int nw = (n + 31) >> 5;
+        uint32_t bits = 0;
+#pragma unroll 8
+        for (int i = 0; i < nw; ++i) {
+          const int c = i * 32 + lane;
+          const bool keep = c < n && (dense || m[(int64_t)c * step] != 0);
+          bits |= (uint32_t)keep << i;
         }
+        count = 0;
+        word = 0;
+        int before = 0;  // kept blocks in the words of lower lanes
+        for (int i = 0; i < nw; ++i) {
+          const uint32_t bal = __ballot_sync(0xffffffffu, (bits >> i) & 1u);
+          if (lane == i) {
+            word = bal;
+            before = count;
+          }
+          count += __popc(bal);
+        }
+        pieces = max(1, min(p.chunks[kind], count / least));
+        if (piece >= pieces) continue;
+        if (pieces > 1) {
+          // this piece: the kept blocks number lo .. hi-1 of the tile
+          const int lo = piece * count / pieces, hi = (piece + 1) * count / pieces;
+          uint32_t rest = word;
+          word = 0;
+          for (int r = before; rest != 0u && r < hi; ++r) {
+            const uint32_t low = rest & (0u - rest);
+            rest ^= low;
+            if (r >= lo) word |= low;
+          }
+          count = hi - lo;
+        }
+        t = tile;
         break;
       }
-      const Tile tl = tile_of(p, t);
-      int mh = tl.h;
-      bool dense = false;
-      if (p.head_mask_type != nullptr) {
-        const int ty = p.head_mask_type[tl.h];
-        if (ty > 0) mh = ty - 1; else dense = true;
-      }
-      const uint8_t* m = p.mask + (int64_t)tl.b * p.ms0 + (int64_t)mh * p.ms1 +
-                         (int64_t)tl.blk * (tl.kind ? p.ms2 : p.ms3);
-      const int64_t step = tl.kind ? p.ms3 : p.ms2;
-      const int n = tl.kind ? p.nk : p.nq;
-      // all mask bytes are loaded before any is used; bit i of `bits` is block
-      // 32 i + lane
-      const int nw = (n + 31) >> 5;
-      uint32_t bits = 0;
-#pragma unroll 8
-      for (int i = 0; i < nw; ++i) {
-        const int c = i * 32 + lane;
-        const bool keep = c < n && (dense || m[(int64_t)c * step] != 0);
-        bits |= (uint32_t)keep << i;
-      }
-      int count = 0;
-      for (int i = 0; i < nw; ++i) {
-        const uint32_t bal = __ballot_sync(0xffffffffu, (bits >> i) & 1u);
-        if (lane == 0) ctl->kept[slot][i] = bal;
-        count += __popc(bal);
-      }
+      if (t >= 0) ctl->kept[slot][lane] = word;
+      __syncwarp();
       if (lane == 0) {
-        ctl->n_blocks[slot] = count;
+        ctl->n_blocks[slot] = t < 0 ? 0 : count;
+        ctl->pieces[slot] = pieces;
+        ctl->piece[slot] = piece;
         ctl->tile_id[slot] = t;
+        mbar_arrive(&ctl->list_full[slot]);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->list_full[slot]);
+      if (t < 0) break;
     }
   } else if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -349,11 +476,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++sent[3];
           // the statistics of two blocks ago have been read once their dS is written
           if (J >= 2 && !wait(&ctl->ds_full[J & 1], (uint32_t)((J - 2) >> 1) & 1u)) break;
-          if (tl.kind == 0) {
+          if (tl.kind == 0 || j == 0) {
+            const float* src = stat + (int64_t)(tl.kind ? tl.blk : blk) * kT;
             mbar_arrive_expect_tx(&ctl->st_full[J & 1], kStatBytes);
-            bulk_load(ctl->stats[J & 1], stat + (int64_t)blk * kT, kT * 4, &ctl->st_full[J & 1]);
-            bulk_load(ctl->stats[J & 1] + kT, stat + p.stat_plane + (int64_t)blk * kT, kT * 4,
-                      &ctl->st_full[J & 1]);
+            bulk_load(ctl->stats[J & 1], src, kT * 4, &ctl->st_full[J & 1]);
+            bulk_load(ctl->stats[J & 1] + kT, src + p.stat_plane, kT * 4, &ctl->st_full[J & 1]);
           } else {
             mbar_arrive(&ctl->st_full[J & 1]);
           }
@@ -423,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
         const int t = ctl->tile_id[slot];
         if (t < 0) break;
-        const int kind = t >= p.tiles0 ? 1 : 0;
+        const int kind = t >= p.tiles[0] ? 1 : 0;
         const int n = ctl->n_blocks[slot];
         if (n > 0) {
           // kind 1 has no acc1: its columns are the second Y buffer
@@ -519,33 +646,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t < 0) break;
       const Tile tl = tile_of(p, t);
       const int n = ctl->n_blocks[slot];
-      const int grow = tl.blk * kT + row;
-      const bool write = grow < (tl.kind ? p.Sq : p.Sk);
+      // this warp's first output row and column, and how many rows exist
+      const int wrow = tl.blk * kT + (warp & 3) * 32;
+      const int rows = (tl.kind ? p.Sq : p.Sk) - wrow;
       __nv_bfloat16 *o1 = nullptr, *o2;
+      int64_t pitch1 = 0, pitch2;
       if (tl.kind) {
-        o2 = p.dq + tl.b * p.dqs0 + tl.h * p.dqs1 + (int64_t)grow * p.dqs2 + g * kCols;
+        pitch2 = p.dqs2;
+        o2 = p.dq + tl.b * p.dqs0 + tl.h * p.dqs1 + wrow * pitch2 + g * kCols;
       } else {
-        o1 = p.dv + tl.b * p.dvs0 + tl.h * p.dvs1 + (int64_t)grow * p.dvs2 + g * kCols;
-        o2 = p.dk + tl.b * p.dks0 + tl.h * p.dks1 + (int64_t)grow * p.dks2 + g * kCols;
+        pitch1 = p.dvs2;
+        pitch2 = p.dks2;
+        o1 = p.dv + tl.b * p.dvs0 + tl.h * p.dvs1 + wrow * pitch1 + g * kCols;
+        o2 = p.dk + tl.b * p.dks0 + tl.h * p.dks1 + wrow * pitch2 + g * kCols;
       }
       if (n == 0) {
-        if (write) {
-          if (!tl.kind) store_zero(o1);
-          store_zero(o2);
-        }
+        if (!tl.kind) zero_rows(o1, pitch1, rows, lane);
+        zero_rows(o2, pitch2, rows, lane);
         mbar_arrive(&ctl->list_empty[slot]);
         continue;
-      }
-      float row_nl = 0.f, row_nd = 0.f;
-      if (tl.kind) {
-        const float* src = p.nstat + (int64_t)(tl.b * p.H + tl.h) * p.nq * kT + grow;
-        row_nl = src[0];
-        row_nd = src[p.stat_plane];
       }
       // the last key block of a ragged length, if it is kept
       const bool ragged = tl.kind && (p.Sk % kT) != 0 &&
                           ((ctl->kept[slot][(p.nk - 1) >> 5] >> ((p.nk - 1) & 31)) & 1u);
-      const uint64_t row_nl2 = f2_pack(row_nl, row_nl), row_nd2 = f2_pack(row_nd, row_nd);
+      uint64_t row_nl2 = 0ull, row_nd2 = 0ull;  // kind 1: this row's statistics
       for (int j = 0; j < n; ++j) {
         const uint32_t jp = (uint32_t)(J + j);
         uint64_t pr[kCols / 2];  // the probabilities, in pairs
@@ -598,6 +722,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tmem_st16(t_self + kColY, pk);
         } else {
+          if (j == 0) {
+            const float nl = ctl->stats[jp & 1u][row], nd = ctl->stats[jp & 1u][kT + row];
+            row_nl2 = f2_pack(nl, nl);
+            row_nd2 = f2_pack(nd, nd);
+          }
           if (!wait(&ctl->x_full, jp & 1u)) break;
           tc_fence_after();
           uint32_t r[32], pk[16];
@@ -650,10 +779,51 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (!wait(&ctl->acc_full, (uint32_t)e & 1u)) break;
       tc_fence_after();
-      if (!tl.kind) store_acc(t_self + kColAcc1, 1.0f, o1, write);
-      store_acc(t_self + kColAcc2, p.scale, o2, write);
-      tc_fence_before();
-      mbar_arrive(&ctl->acc_free);
+      const int pieces = ctl->pieces[slot];
+      uint32_t o[kCols];
+      if (pieces == 1) {
+        if (!tl.kind) {
+          load_acc(t_self + kColAcc1, o);
+          store_rows(o, 1.0f, o1, pitch1, rows, lane);
+        }
+        load_acc(t_self + kColAcc2, o);
+        tc_fence_before();
+        mbar_arrive(&ctl->acc_free);
+        store_rows(o, p.scale, o2, pitch2, rows, lane);
+      } else {
+        // Every warp stores its part of the piece's sums; the warp that stores
+        // the tile's last piece adds them all up in piece order, so the result
+        // does not depend on which one that is.
+        const int kind = tl.kind;
+        const int local = kind ? t - p.tiles[0] : t;
+        const int64_t size = (kind ? 1 : 2) * kT * kT;
+        float* first =
+            p.part[kind] + (int64_t)local * p.chunks[kind] * size + (warp - 4) * 32 * kCols;
+        float* mine = first + ctl->piece[slot] * size;
+        if (!kind) {
+          load_acc(t_self + kColAcc1, o);
+          keep_part(o, mine, lane);
+        }
+        load_acc(t_self + kColAcc2, o);
+        tc_fence_before();
+        mbar_arrive(&ctl->acc_free);
+        keep_part(o, mine + size - kT * kT, lane);
+        __threadfence();
+        __syncwarp();
+        int done = 0;
+        if (lane == 0)
+          done = atomicAdd(p.joined[kind] + local * (kWorkers / 32) + (warp - 4), 1) + 1;
+        done = __shfl_sync(0xffffffffu, done, 0);
+        if (done == pieces) {
+          __threadfence();
+          if (!kind) {
+            sum_parts(first, pieces, size, o, lane);
+            store_rows(o, 1.0f, o1, pitch1, rows, lane);
+          }
+          sum_parts(first + size - kT * kT, pieces, size, o, lane);
+          store_rows(o, p.scale, o2, pitch2, rows, lane);
+        }
+      }
       J += n;
       ++e;
       mbar_arrive(&ctl->list_empty[slot]);
@@ -669,11 +839,58 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace attn_bwd
 }  // namespace sa
 
+namespace {
+
+// How the tiles of each kind may be cut, and where everything lies in the
+// workspace. Tiles are cut where there are fewer than two per SM: a mask with
+// one dense column (every query keeps key block 0) then leaves one CTA working
+// on that column long after the others are done (4096 tokens, 4 heads: 32
+// blocks in a row against 14 for an SM's share). With more tiles the items
+// even out by themselves and the pieces' traffic is saved.
+struct Layout {
+  int tiles[2], chunks[2];
+  size_t joined[2], n_joined, bh_count, stats, part[2], bytes;
+};
+
+Layout layout_of(int B, int H, int Sq, int Sk, int sms) {
+  using namespace sa::attn_bwd;
+  Layout l;
+  const int64_t bh = (int64_t)B * H;
+  const int n[2] = {(Sk + kT - 1) / kT, (Sq + kT - 1) / kT};  // tiles of a head; the other's blocks
+  size_t at = 256;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  l.n_joined = 0;
+  for (int k = 0; k < 2; ++k) {
+    l.tiles[k] = (int)(n[k] * bh);
+    l.chunks[k] = 1;
+    if (n[k] * bh < 2 * sms) {
+      const int most = n[1 - k] / kLeastPiece, items = 8 * sms / l.tiles[k];
+      l.chunks[k] = most < 1 ? 1 : most < items ? most : items;
+    }
+    l.joined[k] = 256 + l.n_joined * sizeof(int);
+    if (l.chunks[k] > 1) l.n_joined += (size_t)l.tiles[k] * (kWorkers / 32);
+  }
+  take(l.n_joined * sizeof(int));
+  l.bh_count = take(bh * sizeof(int));
+  l.stats = take(2 * sizeof(float) * bh * n[1] * kT);
+  for (int k = 0; k < 2; ++k)
+    l.part[k] = l.chunks[k] > 1 ? take((size_t)l.tiles[k] * l.chunks[k] * (2 - k) * kT * kT * 4) : 0;
+  l.bytes = at;
+  return l;
+}
+
+}  // namespace
+
 extern "C" size_t sa_bsattn_bwd_workspace_size(int B, int H, int Sq, int Sk) {
   using namespace sa::attn_bwd;
-  if (B < 1 || H < 1 || Sq < 1 || Sk < 1) return 0;
-  const size_t rows = (size_t)((Sq + kT - 1) / kT) * kT;
-  return 256 + 2 * sizeof(float) * (size_t)B * H * rows;
+  if (B < 1 || H < 1 || Sq < 1 || Sk < 1 || Sq > kMaxBlocks * kT || Sk > kMaxBlocks * kT ||
+      (int64_t)B * H > 65535)
+    return 0;
+  return layout_of(B, H, Sq, Sk, sa::sm_count_current_device()).bytes;
 }
 
 extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, const void* v,
@@ -713,10 +930,11 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
                "%s: tensor base pointers must be 16-byte aligned", fn);
   SA_CHECK_ARG(Hm >= 1 && (head_mask_type != nullptr || Hm == H),
                "%s: mask has %d heads but H=%d and no head_mask_type", fn, Hm, H);
-  const size_t need = sa_bsattn_bwd_workspace_size(B, H, Sq, Sk);
-  SA_CHECK_ARG(workspace != nullptr && ws_bytes >= need && (uintptr_t)workspace % 256 == 0,
-               "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", fn, need, ws_bytes);
-
+  const int sms = sa::sm_count_current_device();
+  const Layout l = layout_of(B, H, Sq, Sk, sms);
+  SA_CHECK_ARG(workspace != nullptr && ws_bytes >= l.bytes && (uintptr_t)workspace % 256 == 0,
+               "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", fn, l.bytes,
+               ws_bytes);
   CUtensorMap tq, tk, tv, td;
   int rc;
   if ((rc = sa::tile_map_bhsd(&tq, q, q_strides, B, H, Sq, D)) != SA_OK) return rc;
@@ -726,12 +944,12 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
 
   Params p;
   p.B = B; p.H = H; p.Sq = Sq; p.Sk = Sk; p.nq = nq; p.nk = nk;
-  p.mask = block_mask;
-  p.ms0 = m_strides[0]; p.ms1 = m_strides[1]; p.ms2 = m_strides[2]; p.ms3 = m_strides[3];
-  p.head_mask_type = head_mask_type;
+  p.mask = sa::attn_bwd::Mask{block_mask, m_strides[0], m_strides[1], m_strides[2], m_strides[3],
+                              head_mask_type};
   p.scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf((float)D);
   p.scale_log2 = p.scale * 1.4426950408889634f;
-  float* nstat = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  char* ws = static_cast<char*>(workspace);
+  float* nstat = reinterpret_cast<float*>(ws + l.stats);
   p.nstat = nstat;
   p.stat_plane = (int64_t)B * H * nq * kT;
   p.dq = static_cast<__nv_bfloat16*>(dq);
@@ -740,10 +958,18 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
   p.dqs0 = dq_strides[0]; p.dqs1 = dq_strides[1]; p.dqs2 = dq_strides[2];
   p.dks0 = dk_strides[0]; p.dks1 = dk_strides[1]; p.dks2 = dk_strides[2];
   p.dvs0 = dv_strides[0]; p.dvs1 = dv_strides[1]; p.dvs2 = dv_strides[2];
-  p.next_tile = static_cast<int*>(workspace);
+  p.next_item = static_cast<int*>(workspace);
   p.status = status;
-  p.tiles0 = nk * H * B;
-  p.tiles = p.tiles0 + nq * H * B;
+  const bool cut = l.chunks[0] > 1 || l.chunks[1] > 1;
+  int* bh_count = cut ? reinterpret_cast<int*>(ws + l.bh_count) : nullptr;
+  p.bh_count = bh_count;
+  for (int k = 0; k < 2; ++k) {
+    p.tiles[k] = l.tiles[k];
+    p.chunks[k] = l.chunks[k];
+    p.items[k] = l.tiles[k] * l.chunks[k];
+    p.joined[k] = reinterpret_cast<int*>(ws + l.joined[k]);
+    p.part[k] = reinterpret_cast<float*>(ws + l.part[k]);
+  }
 
   if ((rc = sa::func_attr_once((const void*)bsattn_bwd_kernel,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes)) !=
@@ -753,11 +979,11 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
   row_stats_kernel<<<pg, 256, 0, stream>>>(
       static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
       do_strides[0], do_strides[1], do_strides[2], o_strides[0], o_strides[1], o_strides[2], lse,
-      dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_tile);
+      dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_item,
+      reinterpret_cast<int*>(ws + 256), (int)l.n_joined, bh_count, p.mask, nk);
   SA_CUDA_TRY(cudaGetLastError());
-  const int sms = sa::sm_count_current_device();
-  bsattn_bwd_kernel<<<p.tiles < sms ? p.tiles : sms, kThreads, kSmemBytes, stream>>>(tq, tk, tv,
-                                                                                  td, p);
+  const int items = p.items[0] + p.items[1];
+  bsattn_bwd_kernel<<<items < sms ? items : sms, kThreads, kSmemBytes, stream>>>(tq, tk, tv, td, p);
   SA_CUDA_TRY(cudaGetLastError());
   return SA_OK;
 }
