@@ -69,6 +69,14 @@ struct Params {
   float* part[2];        // [tile][chunk] fp32 sums of a piece
 };
 
+// A work item as the list warp publishes it: a tile, or a piece of one.
+struct __align__(16) Item {
+  int n;        // kept blocks; -1: no more items
+  int kind, blk, h, b;
+  int tile;     // of its kind
+  int pieces, piece;
+};
+
 struct __align__(16) SmemCtl {
   // [block parity] -lse and -delta of the rows of a query block: of each block
   // of kind 0, of a kind-1 tile with its first block
@@ -89,10 +97,7 @@ struct __align__(16) SmemCtl {
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
-  int n_blocks[2];
-  int tile_id[2];
-  int pieces[2];         // of the tile; > 1: this is piece `piece`
-  int piece[2];
+  Item item[2];          // [slot]
   uint32_t kept[2][kMaxBlocks / 32];  // [slot] bit c of word i: block 32 i + c is kept
 };
 
@@ -100,23 +105,6 @@ struct __align__(16) SmemCtl {
 // starts on it (checked by the kernel), so no slack is reserved.
 constexpr size_t kSmemBytes = (2 + kB1 + kB2) * kTileBytes + sizeof(SmemCtl);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
-
-struct Tile {
-  int kind, blk, h, b;
-};
-
-// t: kind-0 tiles, then kind-1 tiles
-__device__ __forceinline__ Tile tile_of(const Params& p, int t) {
-  Tile r;
-  r.kind = t >= p.tiles[0] ? 1 : 0;
-  const int u = r.kind ? t - p.tiles[0] : t;
-  const int n = r.kind ? p.nq : p.nk;
-  r.blk = u % n;
-  const int bh = u / n;
-  r.h = bh % p.H;
-  r.b = bh / p.H;
-  return r;
-}
 
 __device__ __forceinline__ bool head_mask(const int32_t* type, int h, int& mh) {
   mh = h;
@@ -356,7 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!__all_sync(0xffffffffu, mbar_wait(&ctl->list_empty[slot], ((uint32_t)(k >> 1) & 1u) ^ 1u,
                                              p.status, abort_flag)))
         break;
-      int t = -1, count = 0, pieces = 1, piece = 0;
+      Item w;
+      w.n = -1;
       uint32_t word = 0;  // lane i: blocks 32 i .. 32 i + 31
       for (;;) {
         int it = 0;
@@ -365,13 +354,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int kind = it >= p.items[0] ? 1 : 0;
         if (kind) it -= p.items[0];
         if (it >= p.items[kind]) break;
-        piece = it / p.tiles[kind];
-        const int tile = it - piece * p.tiles[kind] + (kind ? p.tiles[0] : 0);
-        const Tile tl = tile_of(p, tile);
+        w.kind = kind;
+        w.piece = it / p.tiles[kind];
+        w.tile = it - w.piece * p.tiles[kind];
+        const int per_head = kind ? p.nq : p.nk;
+        const int bh = w.tile / per_head;
+        w.blk = w.tile - bh * per_head;
+        w.b = bh / p.H;
+        w.h = bh - w.b * p.H;
         int mh;
-        const bool dense = head_mask(p.mask.head_mask_type, tl.h, mh);
-        const uint8_t* m = p.mask.mask + (int64_t)tl.b * p.mask.s0 + (int64_t)mh * p.mask.s1 +
-                           (int64_t)tl.blk * (kind ? p.mask.s2 : p.mask.s3);
+        const bool dense = head_mask(p.mask.head_mask_type, w.h, mh);
+        const uint8_t* m = p.mask.mask + (int64_t)w.b * p.mask.s0 + (int64_t)mh * p.mask.s1 +
+                           (int64_t)w.blk * (kind ? p.mask.s2 : p.mask.s3);
         const int64_t step = kind ? p.mask.s3 : p.mask.s2;
         const int n = kind ? p.nk : p.nq;
         // all mask bytes are loaded before any is used; bit i of `bits` is block
@@ -384,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool keep = c < n && (dense || m[(int64_t)c * step] != 0);
           bits |= (uint32_t)keep << i;
         }
-        count = 0;
+        int count = 0;
         word = 0;
         int before = 0;  // kept blocks in the words of lower lanes
         for (int i = 0; i < nw; ++i) {
@@ -395,11 +389,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           count += __popc(bal);
         }
-        pieces = max(1, min(p.chunks[kind], count / least));
-        if (piece >= pieces) continue;
-        if (pieces > 1) {
+        w.pieces = max(1, min(p.chunks[kind], count / least));
+        if (w.piece >= w.pieces) continue;
+        if (w.pieces > 1) {
           // this piece: the kept blocks number lo .. hi-1 of the tile
-          const int lo = piece * count / pieces, hi = (piece + 1) * count / pieces;
+          const int lo = w.piece * count / w.pieces, hi = (w.piece + 1) * count / w.pieces;
           uint32_t rest = word;
           word = 0;
           for (int r = before; rest != 0u && r < hi; ++r) {
@@ -409,20 +403,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           count = hi - lo;
         }
-        t = tile;
+        w.n = count;
         break;
       }
-      if (t >= 0) ctl->kept[slot][lane] = word;
+      ctl->kept[slot][lane] = word;
       __syncwarp();
       if (lane == 0) {
-        ctl->n_blocks[slot] = t < 0 ? 0 : count;
-        ctl->pieces[slot] = pieces;
-        ctl->piece[slot] = piece;
-        ctl->tile_id[slot] = t;
+        ctl->item[slot] = w;
         mbar_arrive(&ctl->list_full[slot]);
       }
       __syncwarp();
-      if (t < 0) break;
+      if (w.n < 0) break;
     }
   } else if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -435,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return ok;
       };
       auto load = [&](const CUtensorMap* map, uint64_t* bar, uint8_t* dst, int blk,
-                      const Tile& tl) {
+                      const Item& tl) {
         mbar_arrive_expect_tx(bar, kTileBytes);
         tma_load_4d(map, bar, dst, 0, blk * kT, tl.h, tl.b);
         tma_load_4d(map, bar, dst + kBoxBytes, 64, blk * kT, tl.h, tl.b);
@@ -443,10 +434,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; ok; ++k) {
         const int slot = k & 1;
         if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
-        const int t = ctl->tile_id[slot];
-        if (t < 0) break;
-        const Tile tl = tile_of(p, t);
-        const int n = ctl->n_blocks[slot];
+        const Item tl = ctl->item[slot];
+        const int n = tl.n;
+        if (n < 0) break;
         const CUtensorMap* ma[2] = {tl.kind ? &tm_q : &tm_k, tl.kind ? &tm_do : &tm_v};
         const CUtensorMap* mb[2] = {tl.kind ? &tm_k : &tm_q, tl.kind ? &tm_v : &tm_do};
         const float* stat = p.nstat + (int64_t)(tl.b * p.H + tl.h) * p.nq * kT;
@@ -548,10 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; ok; ++k) {
         const int slot = k & 1;
         if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
-        const int t = ctl->tile_id[slot];
-        if (t < 0) break;
-        const int kind = t >= p.tiles[0] ? 1 : 0;
-        const int n = ctl->n_blocks[slot];
+        const int n = ctl->item[slot].n, kind = ctl->item[slot].kind;
+        if (n < 0) break;
         if (n > 0) {
           // kind 1 has no acc1: its columns are the second Y buffer
           auto y_col = [&](int j) { return (kind && (j & 1)) ? kColAcc1 : kColY; };
@@ -642,10 +630,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 0; ok; ++k) {
       const int slot = k & 1;
       if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
-      const int t = ctl->tile_id[slot];
-      if (t < 0) break;
-      const Tile tl = tile_of(p, t);
-      const int n = ctl->n_blocks[slot];
+      const Item tl = ctl->item[slot];
+      const int n = tl.n;
+      if (n < 0) break;
       // this warp's first output row and column, and how many rows exist
       const int wrow = tl.blk * kT + (warp & 3) * 32;
       const int rows = (tl.kind ? p.Sq : p.Sk) - wrow;
@@ -779,7 +766,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (!wait(&ctl->acc_full, (uint32_t)e & 1u)) break;
       tc_fence_after();
-      const int pieces = ctl->pieces[slot];
+      const int pieces = tl.pieces;
       uint32_t o[kCols];
       if (pieces == 1) {
         if (!tl.kind) {
@@ -795,11 +782,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the tile's last piece adds them all up in piece order, so the result
         // does not depend on which one that is.
         const int kind = tl.kind;
-        const int local = kind ? t - p.tiles[0] : t;
+        const int local = tl.tile;
         const int64_t size = (kind ? 1 : 2) * kT * kT;
         float* first =
             p.part[kind] + (int64_t)local * p.chunks[kind] * size + (warp - 4) * 32 * kCols;
-        float* mine = first + ctl->piece[slot] * size;
+        float* mine = first + tl.piece * size;
         if (!kind) {
           load_acc(t_self + kColAcc1, o);
           keep_part(o, mine, lane);
