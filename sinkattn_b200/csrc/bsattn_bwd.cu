@@ -81,12 +81,11 @@ struct __align__(16) SmemCtl {
   // [block parity] -lse and -delta of the rows of a query block: of each block
   // of kind 0, of a kind-1 tile with its first block
   float stats[2][2 * kT];
-  uint64_t b1_full[kB1], b1_empty[kB1];
-  uint64_t b2_full[kB2], b2_empty[kB2];
+  uint64_t b1_full[kB1], b2_full[kB2];
   uint64_t st_full[2];             // [block parity] statistics loaded, or none to load
   uint64_t a_full[2], a_empty[2];  // [0] A1, [1] A2
   uint64_t list_full[2], list_empty[2];
-  uint64_t x_full;       // X of a block computed (commit)
+  uint64_t x_full[2];    // [block parity] X computed (commit)
   // kind 0: [c] half c of each warpgroup's P columns written over X; kind 1: X
   // copied out. kWorkers arrivals
   uint64_t x_done[2];
@@ -286,24 +285,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kB1; ++i) {
-      mbar_init(&ctl->b1_full[i], 1);
-      mbar_init(&ctl->b1_empty[i], 1);
-    }
-    for (int i = 0; i < kB2; ++i) {
-      mbar_init(&ctl->b2_full[i], 1);
-      mbar_init(&ctl->b2_empty[i], 1);
-    }
+    for (int i = 0; i < kB1; ++i) mbar_init(&ctl->b1_full[i], 1);
+    for (int i = 0; i < kB2; ++i) mbar_init(&ctl->b2_full[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->st_full[i], 1);
       mbar_init(&ctl->a_full[i], 1);
       mbar_init(&ctl->a_empty[i], 1);
       mbar_init(&ctl->list_full[i], 1);
       mbar_init(&ctl->list_empty[i], kListReaders);
+      mbar_init(&ctl->x_full[i], 1);
       mbar_init(&ctl->y_full[i], 1);
       mbar_init(&ctl->ds_full[i], kWorkers);
     }
-    mbar_init(&ctl->x_full, 1);
     mbar_init(&ctl->x_done[0], kWorkers);
     mbar_init(&ctl->x_done[1], kWorkers);
     mbar_init(&ctl->acc_full, 1);
@@ -420,11 +413,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int J = 0, e = 0;        // blocks and tiles loaded
       int sent[4] = {0, 0, 0, 0};  // loads issued: A1, A2, B1, B2
+      int kinds = 0;               // bit i: kind of the block i + 1 before this one
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok) ok = mbar_wait(bar, parity, p.status, abort_flag);
         return ok;
       };
+      auto wait_x = [&](int i) { return wait(&ctl->x_full[i & 1], (uint32_t)(i >> 1) & 1u); };
+      auto wait_y = [&](int i) { return wait(&ctl->y_full[i & 1], (uint32_t)(i >> 1) & 1u); };
       auto load = [&](const CUtensorMap* map, uint64_t* bar, uint8_t* dst, int blk,
                       const Item& tl) {
         mbar_arrive_expect_tx(bar, kTileBytes);
@@ -453,7 +449,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++sent[0];
           }
           const int s1 = J % kB1, s2 = J % kB2;
-          if (!wait(&ctl->b1_empty[s1], ((uint32_t)(J / kB1) & 1u) ^ 1u)) break;
+          // A slot is free once the last product that reads it is complete. The
+          // products complete in order, so a later X or Y tells: Y of J-2 follows
+          // dK of J-3, X of J-1 follows dQ of J-3 and dV of J-2.
+          if (J >= kB1 && !((kinds >> 2) & 1 ? wait_x(J - 1) : wait_y(J - 2))) break;
           load(mb[0], &ctl->b1_full[s1], b1_ring + s1 * kTileBytes, blk, tl);
           ++sent[2];
           if (j == 0) {
@@ -461,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             load(ma[1], &ctl->a_full[1], a_tile + kTileBytes, tl.blk, tl);
             ++sent[1];
           }
-          if (!wait(&ctl->b2_empty[s2], ((uint32_t)(J / kB2) & 1u) ^ 1u)) break;
+          if (J >= kB2 && !((kinds >> 1) & 1 ? wait_y(J - 2) : wait_x(J - 1))) break;
           load(mb[1], &ctl->b2_full[s2], b2_ring + s2 * kTileBytes, blk, tl);
           ++sent[3];
           // the statistics of two blocks ago have been read once their dS is written
@@ -474,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             mbar_arrive(&ctl->st_full[J & 1]);
           }
+          kinds = kinds << 1 | tl.kind;
         }
         if (!ok) break;
         if (n > 0) ++e;
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait(&ctl->b1_full[i % kB1], (uint32_t)(i / kB1) & 1u)) return;
             tc_fence_after();
             mma_x(a_desc, b1_kk + (uint64_t)(i % kB1) * kTileDesc, kColX);
-            mma_commit(&ctl->x_full);
+            mma_commit(&ctl->x_full[i & 1]);
             if (j == n - 1) mma_commit(&ctl->a_empty[0]);
           };
           auto issue_y = [&](int j) {
@@ -565,7 +565,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             mma_x(a_desc + kTileDesc, b2_kk + (uint64_t)(i % kB2) * kTileDesc, y_col(j));
             mma_commit(&ctl->y_full[i & 1]);
-            if (kind) mma_commit(&ctl->b2_empty[i % kB2]);
             if (j == n - 1) mma_commit(&ctl->a_empty[1]);
           };
           issue_x(0);
@@ -581,7 +580,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!wait(&ctl->x_done[1], (uint32_t)i & 1u)) break;
               tc_fence_after();
               mma_acc_half(1, kColX, b, kColAcc1, false);
-              mma_commit(&ctl->b2_empty[i % kB2]);
             } else {
               if (!wait(&ctl->x_done[1], (uint32_t)i & 1u)) break;
               tc_fence_after();
@@ -596,7 +594,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t b = b1_mn + (uint64_t)(i % kB1) * kTileDesc;
             mma_acc_half(0, y_col(j), b, kColAcc2, j == 0);
             mma_acc_half(1, y_col(j), b, kColAcc2, false);
-            mma_commit(&ctl->b1_empty[i % kB1]);
             if (j + 1 < n && !kind) issue_y(j + 1);
           }
           if (!ok) break;
@@ -663,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait(&ctl->st_full[jp & 1u], (jp >> 1) & 1u)) break;
         if (tl.kind == 0) {
           const float* st = ctl->stats[jp & 1u];
-          if (!wait(&ctl->x_full, jp & 1u)) break;
+          if (!wait(&ctl->x_full[jp & 1u], (jp >> 1) & 1u)) break;
           tc_fence_after();
           const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(st + g * kCols);
 #pragma unroll
@@ -714,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             row_nl2 = f2_pack(nl, nl);
             row_nd2 = f2_pack(nd, nd);
           }
-          if (!wait(&ctl->x_full, jp & 1u)) break;
+          if (!wait(&ctl->x_full[jp & 1u], (jp >> 1) & 1u)) break;
           tc_fence_after();
           uint32_t r[32], pk[16];
           tmem_ld32(t_self + kColX, r);
