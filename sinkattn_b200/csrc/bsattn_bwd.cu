@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(256)
                      const float* __restrict__ lse, const float* __restrict__ dlse, int H, int Sq,
                      int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_item,
                      int* joined, int n_joined, int* bh_count, const Mask mask, int nk) {
+  release_next_kernel();  // it waits for this one's completion all the same
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next_item = 0;
   for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_joined;
        i += gridDim.x * gridDim.y * 256)
@@ -318,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  wait_prior_kernel();  // the row statistics, the item counter and the counts
 
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   volatile int* abort_flag = &ctl->abort_flag;
@@ -967,7 +969,7 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
       reinterpret_cast<int*>(ws + 256), (int)l.n_joined, bh_count, p.mask, nk);
   SA_CUDA_TRY(cudaGetLastError());
   const int items = p.items[0] + p.items[1];
-  bsattn_bwd_kernel<<<items < sms ? items : sms, kThreads, kSmemBytes, stream>>>(tq, tk, tv, td, p);
-  SA_CUDA_TRY(cudaGetLastError());
+  SA_CUDA_TRY(sa::launch_after(bsattn_bwd_kernel, dim3(items < sms ? items : sms), dim3(kThreads),
+                               kSmemBytes, stream, tq, tk, tv, td, p));
   return SA_OK;
 }

@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, sizeof(T) == 2 ? 3 : 2) bwd_ke
                 ds2 = hd.which ? p.dks2 : p.dqs2;
   const int64_t os0 = hd.which ? p.kos0 : p.qos0, os1 = hd.which ? p.kos1 : p.qos1,
                 os2 = hd.which ? p.kos2 : p.qos2;
+  release_next_kernel();
   V8 acc = fill8(0.f);
   const float inv_d = 1.f / (float)p.D;
   if (chunk < p.chunks) {

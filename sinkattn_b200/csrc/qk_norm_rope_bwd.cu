@@ -25,6 +25,7 @@ __global__ void __launch_bounds__(32 * kChains)
     partial_rows_kernel(const float* __restrict__ part, int rows, int cols, int pitch,
                         float* __restrict__ out0, float* __restrict__ out1, int cols0) {
   __shared__ float red[kChains][33];
+  wait_prior_kernel();
   const int l = threadIdx.x & 31, chain = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + l;
   float s = 0.f;
@@ -46,9 +47,8 @@ __global__ void __launch_bounds__(32 * kChains)
 
 int sum_partial_rows(const float* part, int rows, int cols, int pitch, float* out0, float* out1,
                      int cols0, cudaStream_t stream) {
-  partial_rows_kernel<<<(cols + 31) / 32, 32 * kChains, 0, stream>>>(part, rows, cols, pitch, out0, out1,
-                                                            cols0);
-  SA_CUDA_TRY(cudaGetLastError());
+  SA_CUDA_TRY(launch_after(partial_rows_kernel, dim3((cols + 31) / 32), dim3(32 * kChains), 0,
+                           stream, part, rows, cols, pitch, out0, out1, cols0));
   return SA_OK;
 }
 
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
   const bool on = c0 < p.hidden;
   const int p0 = (c0 % p.D) >> 1;
   const float inv_n = 1.f / (float)p.hidden;
+  release_next_kernel();
   V8 acc[2] = {fill8(0.f), fill8(0.f)};
   V8 w[2];
 #pragma unroll

@@ -47,6 +47,25 @@ int tile_map_bhsd(CUtensorMap* map, const void* base, const int64_t st[4], int B
 // stride(dim) = 1 and the other strides non-negative multiples of 8 elements.
 bool strides16_ok(const int64_t st[4]);
 
+// Launches a kernel that may start while the kernel before it on the stream
+// is still ending (programmatic dependent launch): it calls wait_prior_kernel()
+// before it touches what that kernel writes.
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
+                         cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 }  // namespace sa
 
 #define SA_CHECK_ARG(cond, ...)      \
@@ -73,6 +92,16 @@ namespace sa {
 // Time limit for every spin on an mbarrier phase (nanoseconds of
 // %globaltimer). Legitimate waits in these kernels last microseconds.
 constexpr uint64_t kWaitNs = 1000000000ull;  // 1 s
+
+// Waits until the kernel before this one on the stream has completed and its
+// writes are visible (a no-op in an ordinary launch).
+__device__ __forceinline__ void wait_prior_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// Lets the kernel launched after this one start before this one has ended.
+__device__ __forceinline__ void release_next_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 __device__ __forceinline__ uint64_t global_timer_ns() {
   uint64_t t;
