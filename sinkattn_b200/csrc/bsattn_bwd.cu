@@ -48,6 +48,20 @@ struct Mask {
   const uint8_t* mask;
   int64_t s0, s1, s2, s3;
   const int32_t* head_mask_type;
+  // The mask column (kind 0) or row (kind 1) blk of a head; true when the head
+  // is dense, with nothing to read.
+  __device__ __forceinline__ bool line(int kind, int b, int h, int blk, const uint8_t*& m,
+                                       int64_t& step) const {
+    int mh = h;
+    if (head_mask_type != nullptr) {
+      const int ty = head_mask_type[h];
+      if (ty <= 0) return true;
+      mh = ty - 1;
+    }
+    m = mask + b * s0 + mh * s1 + blk * (kind ? s2 : s3);
+    step = kind ? s3 : s2;
+    return false;
+  }
 };
 
 struct Params {
@@ -60,11 +74,12 @@ struct Params {
   int64_t dqs0, dqs1, dqs2, dks0, dks1, dks2, dvs0, dvs1, dvs2;
   int* next_item;
   int32_t* status;
-  // Work items: chunk 0 of every kind-0 tile, chunk 1 of each, ..., then the
-  // same of kind 1. A tile of `count` kept blocks is cut into
-  // clamp(count / least, 1, chunks) pieces, least from the total count.
-  int tiles[2], chunks[2], items[2];
-  const int* bh_count;   // kept blocks of every (batch, head); chunks > 1 only
+  // Work items: a tile of `count` kept blocks is cut into clamp(count / least,
+  // 1, chunks) pieces, least from the total count. Pieces 1, 2, ... of the cut
+  // tiles are dealt out to the CTAs first, then every tile's piece 0 is taken
+  // from a counter, kind 0 before kind 1.
+  int tiles[2], chunks[2];
+  const int* counts[2];  // kept blocks of every tile; NULL where chunks = 1
   int* joined[2];        // [tile][worker warp] pieces stored so far
   float* part[2];        // [tile][chunk] fp32 sums of a piece
 };
@@ -105,14 +120,6 @@ struct __align__(16) SmemCtl {
 constexpr size_t kSmemBytes = (2 + kB1 + kB2) * kTileBytes + sizeof(SmemCtl);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
-__device__ __forceinline__ bool head_mask(const int32_t* type, int h, int& mh) {
-  mh = h;
-  if (type == nullptr) return false;
-  const int ty = type[h];
-  if (ty > 0) mh = ty - 1;
-  return ty <= 0;  // dense
-}
-
 // Row statistics: one 16-lane group per query row sums dO . O in fp32. Rows
 // past Sq and rows without a finite log-sum-exp (no kept key) get -inf, which
 // makes every P of theirs 0. Bound by reading dO and O once.
@@ -122,31 +129,33 @@ __global__ void __launch_bounds__(256)
                      int64_t ds0, int64_t ds1, int64_t ds2, int64_t os0, int64_t os1, int64_t os2,
                      const float* __restrict__ lse, const float* __restrict__ dlse, int H, int Sq,
                      int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_item,
-                     int* joined, int n_joined, int* bh_count, const Mask mask, int nk) {
+                     int* joined, int n_joined, int* counts0, int* counts1, const Mask mask, int B,
+                     int nk) {
   release_next_kernel();  // it waits for this one's completion all the same
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next_item = 0;
-  for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_joined;
-       i += gridDim.x * gridDim.y * 256)
-    joined[i] = 0;
+  const int nq = rows_pad / kT;
+  const int block = blockIdx.y * gridDim.x + blockIdx.x, blocks = gridDim.x * gridDim.y;
+  if (block == 0 && threadIdx.x == 0) *next_item = 0;
+  for (int i = block * 256 + threadIdx.x; i < n_joined; i += blocks * 256) joined[i] = 0;
+  // kept blocks of every tile of the kinds that may be cut, a warp per tile
+  for (int kind = 0; kind < 2; ++kind) {
+    int* counts = kind ? counts1 : counts0;
+    if (counts == nullptr) continue;
+    const int per_head = kind ? nq : nk, n = kind ? nk : nq;
+    for (int t = block * 8 + (threadIdx.x >> 5); t < B * H * per_head; t += blocks * 8) {
+      const int bh = t / per_head;
+      const uint8_t* m;
+      int64_t step;
+      int c = n;
+      if (!mask.line(kind, bh / H, bh % H, t - bh * per_head, m, step)) {
+        c = 0;
+        for (int i = threadIdx.x & 31; i < n; i += 32) c += m[i * step] != 0;
+        c = __reduce_add_sync(0xffffffffu, c);
+      }
+      if ((threadIdx.x & 31) == 0) counts[t] = c;
+    }
+  }
   const int bh = blockIdx.y;
   const int h = bh % H, b = bh / H;
-  if (bh_count != nullptr && blockIdx.x == 0) {
-    // kept blocks of this head, for the cut of long tiles
-    const int n = (rows_pad / kT) * nk;
-    int mh, c = 0;
-    const bool dense = head_mask(mask.head_mask_type, h, mh);
-    const uint8_t* m = mask.mask + b * mask.s0 + mh * mask.s1;
-    if (!dense)
-      for (int i = threadIdx.x; i < n; i += 256)
-        c += m[(int64_t)(i / nk) * mask.s2 + (int64_t)(i % nk) * mask.s3] != 0;
-    __shared__ int sum;
-    if (threadIdx.x == 0) sum = dense ? n : 0;
-    __syncthreads();
-    c = __reduce_add_sync(0xffffffffu, c);
-    if ((threadIdx.x & 31) == 0) atomicAdd(&sum, c);
-    __syncthreads();
-    if (threadIdx.x == 0) bh_count[bh] = sum;
-  }
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
   const int r0 = blockIdx.x * (16 * kPrepRows) + g;
   uint4 x[kPrepRows], y[kPrepRows];
@@ -326,14 +335,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 2) {
     // ---------------- work items and their kept blocks, two ahead ----------------
-    int least = 0x7fffffff;
-    if (p.bh_count != nullptr) {
+    int least = 0x7fffffff, extra[2] = {0, 0}, before_lane[2] = {0, 0}, span[2] = {1, 1};
+    auto pieces_of = [&](int kind, int count) {
+      return max(1, min(p.chunks[kind], count / least));
+    };
+    if (p.counts[0] != nullptr || p.counts[1] != nullptr) {
       // pieces of about half an SM's share of the blocks of both kinds, 8 at least
+      const int known = p.counts[0] != nullptr ? 0 : 1;  // the total is alike for both
       int total = 0;
-      for (int i = lane; i < p.B * p.H; i += 32) total += p.bh_count[i];
+      for (int i = lane; i < p.tiles[known]; i += 32) total += p.counts[known][i];
       total = __reduce_add_sync(0xffffffffu, total);
       least = max(kLeastPiece, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (p.counts[q] == nullptr) continue;
+        span[q] = (p.tiles[q] + 31) >> 5;  // consecutive tiles of a lane
+        int own = 0;
+        for (int i = lane * span[q]; i < min(p.tiles[q], (lane + 1) * span[q]); ++i)
+          own += pieces_of(q, p.counts[q][i]) - 1;
+        int sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += x;
+        }
+        extra[q] = __shfl_sync(0xffffffffu, sum, 31);
+        before_lane[q] = sum - own;
+      }
     }
+    int dealt = blockIdx.x;  // this CTA's next extra piece
     for (int k = 0;; ++k) {
       const int slot = k & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(&ctl->list_empty[slot], ((uint32_t)(k >> 1) & 1u) ^ 1u,
@@ -342,26 +372,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item w;
       w.n = -1;
       uint32_t word = 0;  // lane i: blocks 32 i .. 32 i + 31
-      for (;;) {
+      w.kind = -1;
+      if (dealt < extra[0] + extra[1]) {
+        // which tile the dealt-out piece belongs to: first the lane, then the
+        // tile among that lane's
+        w.kind = dealt >= extra[0] ? 1 : 0;
+        const int r = dealt - (w.kind ? extra[0] : 0);
+        const int before = w.kind ? before_lane[1] : before_lane[0];
+        const int* counts = w.kind ? p.counts[1] : p.counts[0];
+        const int owner = 31 - __clz(__ballot_sync(0xffffffffu, before <= r));
+        int left = r - __shfl_sync(0xffffffffu, before, owner);
+        for (w.tile = owner * (w.kind ? span[1] : span[0]);; ++w.tile) {
+          const int more = pieces_of(w.kind, counts[w.tile]) - 1;
+          if (left < more) break;
+          left -= more;
+        }
+        w.piece = 1 + left;
+        dealt += gridDim.x;
+      } else {
         int it = 0;
         if (lane == 0) it = atomicAdd(p.next_item, 1);
         it = __shfl_sync(0xffffffffu, it, 0);
-        const int kind = it >= p.items[0] ? 1 : 0;
-        if (kind) it -= p.items[0];
-        if (it >= p.items[kind]) break;
-        w.kind = kind;
-        w.piece = it / p.tiles[kind];
-        w.tile = it - w.piece * p.tiles[kind];
+        if (it < p.tiles[0] + p.tiles[1]) {
+          w.kind = it >= p.tiles[0] ? 1 : 0;
+          w.tile = it - (w.kind ? p.tiles[0] : 0);
+          w.piece = 0;
+        }
+      }
+      if (w.kind >= 0) {
+        const int kind = w.kind;
         const int per_head = kind ? p.nq : p.nk;
         const int bh = w.tile / per_head;
         w.blk = w.tile - bh * per_head;
         w.b = bh / p.H;
         w.h = bh - w.b * p.H;
-        int mh;
-        const bool dense = head_mask(p.mask.head_mask_type, w.h, mh);
-        const uint8_t* m = p.mask.mask + (int64_t)w.b * p.mask.s0 + (int64_t)mh * p.mask.s1 +
-                           (int64_t)w.blk * (kind ? p.mask.s2 : p.mask.s3);
-        const int64_t step = kind ? p.mask.s3 : p.mask.s2;
+        const uint8_t* m = nullptr;
+        int64_t step = 0;
+        const bool dense = p.mask.line(kind, w.b, w.h, w.blk, m, step);
         const int n = kind ? p.nk : p.nq;
         // all mask bytes are loaded before any is used; bit i of `bits` is block
         // 32 i + lane
@@ -370,11 +417,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 8
         for (int i = 0; i < nw; ++i) {
           const int c = i * 32 + lane;
-          const bool keep = c < n && (dense || m[(int64_t)c * step] != 0);
+          const bool keep = c < n && (dense || m[c * step] != 0);
           bits |= (uint32_t)keep << i;
         }
         int count = 0;
-        word = 0;
         int before = 0;  // kept blocks in the words of lower lanes
         for (int i = 0; i < nw; ++i) {
           const uint32_t bal = __ballot_sync(0xffffffffu, (bits >> i) & 1u);
@@ -384,8 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           count += __popc(bal);
         }
-        w.pieces = max(1, min(p.chunks[kind], count / least));
-        if (w.piece >= w.pieces) continue;
+        w.pieces = pieces_of(kind, count);
         if (w.pieces > 1) {
           // this piece: the kept blocks number lo .. hi-1 of the tile
           const int lo = w.piece * count / w.pieces, hi = (w.piece + 1) * count / w.pieces;
@@ -399,7 +444,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           count = hi - lo;
         }
         w.n = count;
-        break;
       }
       ctl->kept[slot][lane] = word;
       __syncwarp();
@@ -835,7 +879,7 @@ namespace {
 // even out by themselves and the pieces' traffic is saved.
 struct Layout {
   int tiles[2], chunks[2];
-  size_t joined[2], n_joined, bh_count, stats, part[2], bytes;
+  size_t joined[2], n_joined, counts[2], stats, part[2], bytes;
 };
 
 Layout layout_of(int B, int H, int Sq, int Sk, int sms) {
@@ -861,7 +905,7 @@ Layout layout_of(int B, int H, int Sq, int Sk, int sms) {
     if (l.chunks[k] > 1) l.n_joined += (size_t)l.tiles[k] * (kWorkers / 32);
   }
   take(l.n_joined * sizeof(int));
-  l.bh_count = take(bh * sizeof(int));
+  for (int k = 0; k < 2; ++k) l.counts[k] = l.chunks[k] > 1 ? take(l.tiles[k] * sizeof(int)) : 0;
   l.stats = take(2 * sizeof(float) * bh * n[1] * kT);
   for (int k = 0; k < 2; ++k)
     l.part[k] = l.chunks[k] > 1 ? take((size_t)l.tiles[k] * l.chunks[k] * (2 - k) * kT * kT * 4) : 0;
@@ -946,13 +990,13 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
   p.dvs0 = dv_strides[0]; p.dvs1 = dv_strides[1]; p.dvs2 = dv_strides[2];
   p.next_item = static_cast<int*>(workspace);
   p.status = status;
-  const bool cut = l.chunks[0] > 1 || l.chunks[1] > 1;
-  int* bh_count = cut ? reinterpret_cast<int*>(ws + l.bh_count) : nullptr;
-  p.bh_count = bh_count;
+  int* counts[2];
+  int items = 0;
   for (int k = 0; k < 2; ++k) {
     p.tiles[k] = l.tiles[k];
     p.chunks[k] = l.chunks[k];
-    p.items[k] = l.tiles[k] * l.chunks[k];
+    items += l.tiles[k] * l.chunks[k];
+    p.counts[k] = counts[k] = l.chunks[k] > 1 ? reinterpret_cast<int*>(ws + l.counts[k]) : nullptr;
     p.joined[k] = reinterpret_cast<int*>(ws + l.joined[k]);
     p.part[k] = reinterpret_cast<float*>(ws + l.part[k]);
   }
@@ -966,9 +1010,8 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
       static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
       do_strides[0], do_strides[1], do_strides[2], o_strides[0], o_strides[1], o_strides[2], lse,
       dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_item,
-      reinterpret_cast<int*>(ws + 256), (int)l.n_joined, bh_count, p.mask, nk);
+      reinterpret_cast<int*>(ws + 256), (int)l.n_joined, counts[0], counts[1], p.mask, B, nk);
   SA_CUDA_TRY(cudaGetLastError());
-  const int items = p.items[0] + p.items[1];
   SA_CUDA_TRY(sa::launch_after(bsattn_bwd_kernel, dim3(items < sms ? items : sms), dim3(kThreads),
                                kSmemBytes, stream, tq, tk, tv, td, p));
   return SA_OK;
