@@ -416,6 +416,7 @@ SA_API int sa_qk_norm_rope(const void* q_in, const void* k_in, int64_t q_in_row_
  * fixed order: equal calls give equal bits. rows may be 0 (dw = 0).
  * workspace (only for dw): sa_qk_norm_rope_bwd_workspace_size(hidden) bytes,
  *   16-byte aligned, any contents, not shared by calls that overlap.
+ * status: as sa_bsattn_fwd.
  */
 SA_API size_t sa_qk_norm_rope_bwd_workspace_size(int hidden);
 SA_API int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_row_stride,
@@ -425,7 +426,7 @@ SA_API int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_row_st
                                float eps, const float* cos_table, const float* sin_table,
                                int64_t freq_row_stride, void* dq_in, void* dk_in,
                                int64_t dqi_row_stride, int64_t dki_row_stride, float* dw_q,
-                               float* dw_k, void* workspace, size_t ws_bytes,
+                               float* dw_k, void* workspace, size_t ws_bytes, int32_t* status,
                                cudaStream_t stream);
 
 /*

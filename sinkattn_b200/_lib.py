@@ -101,7 +101,7 @@ _SIGNATURES = {
     "sa_qk_norm_rope_bwd": (
         _i,
         [_vp, _vp, _l, _l, _vp, _vp, _l, _l, _i, _i, _i, _i, _vp, _vp, _i, _f, _vp, _vp, _l, _vp,
-         _vp, _l, _l, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+         _vp, _l, _l, _vp, _vp, _vp, ctypes.c_size_t, _vp, _vp],
     ),
     "sa_qk_head_norm_rope": (
         _i,

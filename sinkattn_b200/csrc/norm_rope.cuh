@@ -125,9 +125,12 @@ __device__ __forceinline__ V8 load_weight8(const void* w, int dtype, int c0) {
   return unpack8(Raw8<float>{{__ldg(p + (c0 >> 2)), __ldg(p + (c0 >> 2) + 1)}});
 }
 
-// 1 / sqrt(v): the hardware's approximation and one Newton step.
+// 1 / sqrt(v): the hardware's approximation (within 2^-22), with one Newton
+// step where the result is fp32 as well.
+template <typename T>
 __device__ __forceinline__ float inv_sqrt(float v) {
   const float r = rsqrtf(v);
+  if (sizeof(T) == 2) return r;
   const float e = fmaf(-v * r, r, 1.f);
   // v = 0 and v = inf keep the approximation's inf and 0 (e is NaN there)
   return e == e ? fmaf(0.5f * r, e, r) : r;

@@ -9,12 +9,11 @@
 //
 // Memory-bound: x read and o written once (the gradient reads do and x and
 // writes dx). A lane holds 8 channels of a head (16 lanes a head of 128), so
-// the sums are shuffles inside a lane group. A warp takes 4 heads per lane
-// group of one token and one tensor, all loaded before the first is used, and
-// folds weight, cosine and sine into the two factors of each channel once for
-// all of them; the arithmetic is f32x2, as the scalar form was bound by its
-// instructions. Everything between the load and the store is fp32: the one
-// rounding is that of the result.
+// the sums are shuffles inside a lane group. A warp walks heads of one token
+// and one tensor, loading a few heads ahead, and folds weight, cosine and sine
+// into the two factors of each channel once for all of them; the arithmetic is
+// f32x2. Everything between the load and the store is fp32: the one rounding is
+// that of the result.
 
 #include <math.h>
 
@@ -25,21 +24,24 @@ namespace headnorm {
 
 using namespace sa::nr;
 
-constexpr int kUnroll = 4;   // heads of a lane group, loaded together
-constexpr int kUnrollBwd = 2;  // as many vectors: two tensors are read
-constexpr int kMaxWarps = 8; // warps of a block: the chunks of one token
+// Heads of a lane group in flight, about 64 KB per SM with the warps that fit.
+template <typename T>
+__host__ __device__ constexpr int ahead() { return sizeof(T) == 2 ? 3 : 2; }
+constexpr int kAheadBwd = 4;
+constexpr int kWarps = 8;        // of a block
 constexpr int kMaxHeads = 8192;  // of q and k together
-constexpr int kMaxRows = (kMaxHeads / kUnrollBwd + 2) / kMaxWarps + 1;  // blocks of one token
+
+// [0] q, [1] k. Head strides are 32-bit: a head's offset is one multiply-add.
+struct Tensors {
+  const void* base[2];
+  int64_t s0[2], s1[2];  // batch, sequence
+  int s2[2];             // head
+};
 
 struct Params {
-  const void *q, *k;
-  int64_t qs0, qs1, qs2, ks0, ks1, ks2;
-  void *qo, *ko;
-  int64_t qos0, qos1, qos2, kos0, kos1, kos2;
-  const void *dq, *dk;  // gradient only: upstream gradients
-  int64_t dqs0, dqs1, dqs2, dks0, dks1, dks2;
+  Tensors x, o, d;  // inputs, outputs, upstream gradients (gradient only)
   int B, S, Hq, Hk, D, rot;
-  const void *wq, *wk;
+  const void* w[2];
   int w_dtype;
   float eps;
   const float *cos_t, *sin_t;
@@ -48,6 +50,7 @@ struct Params {
   const void* pos;
   int pos_i64;
   int64_t ps0, ps1;
+  int steps;             // of a warp, 32 / G heads each
   int chunks_q, chunks;  // warps of a token: those of q, then those of k
   int tokens;
   float* part;     // gradient only: per-block sums of dw [blocks][2][D]
@@ -81,6 +84,11 @@ __device__ __forceinline__ Token token_of(const Params& p, int t) {
   k.bad = p.cos_t != nullptr && (k.row < 0 || k.row >= p.table_rows);
   if (k.bad) k.row = 0;
   return k;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* token_ptr(const Tensors& t, int which, const Token& k) {
+  return reinterpret_cast<const T*>(t.base[which]) + k.b * t.s0[which] + k.s * t.s1[which];
 }
 
 // Cosine and sine of a lane's 8 channels: one pair per two channels with
@@ -141,55 +149,56 @@ __device__ __forceinline__ int partner_of(const Params& p, int lane, int c0, int
   return lane + d / 8;
 }
 
-// This warp's heads: tensor (0 q, 1 k), the first head of its lane group and
-// the number of heads of the tensor.
+// This warp's heads: tensor (0 q, 1 k), those of its lane group (first, end,
+// 32 / G apart).
 struct Heads {
-  int which, h0, H;
+  int which, first, end;
 };
 
-template <int G, int U>
+template <int G>
 __device__ __forceinline__ Heads heads_of(const Params& p, int chunk, int lane) {
   Heads h;
   h.which = chunk >= p.chunks_q ? 1 : 0;
-  h.H = h.which ? p.Hk : p.Hq;
-  h.h0 = (h.which ? chunk - p.chunks_q : chunk) * (U * (32 / G)) + lane / G;
+  const int c = h.which ? chunk - p.chunks_q : chunk, per = p.steps * (32 / G);
+  h.first = c * per + lane / G;
+  h.end = min(h.which ? p.Hk : p.Hq, (c + 1) * per);
   return h;
 }
 
 // One warp per token and chunk of heads.
 template <typename T, int G, bool INTER>
-__global__ void __launch_bounds__(32 * kMaxWarps, INTER ? 4 : 3) fwd_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * kWarps, INTER ? 4 : 3) fwd_kernel(const Params p) {
+  constexpr int kAhead = ahead<T>();
   const int lane = threadIdx.x & 31;
-  const int chunk = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (chunk >= p.chunks) return;
-  const Heads hd = heads_of<G, kUnroll>(p, chunk, lane);
+  const unsigned gw = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const unsigned t = gw / (unsigned)p.chunks;
+  if (t >= (unsigned)p.tokens) return;
+  const Heads hd = heads_of<G>(p, gw - t * p.chunks, lane);
   const int c0 = (lane % G) * 8;
   const bool on = c0 < p.D;
-  const Token tk = token_of(p, blockIdx.x);
-  const T* src = hd.which
-                     ? reinterpret_cast<const T*>(p.k) + tk.b * p.ks0 + tk.s * p.ks1 + c0
-                     : reinterpret_cast<const T*>(p.q) + tk.b * p.qs0 + tk.s * p.qs1 + c0;
-  T* dst = hd.which ? reinterpret_cast<T*>(p.ko) + tk.b * p.kos0 + tk.s * p.kos1 + c0
-                    : reinterpret_cast<T*>(p.qo) + tk.b * p.qos0 + tk.s * p.qos1 + c0;
-  const int64_t hs = hd.which ? p.ks2 : p.qs2, ohs = hd.which ? p.kos2 : p.qos2;
-  Raw8<T> raw[kUnroll];
+  const Token tk = token_of(p, t);
+  const T* src = token_ptr<T>(p.x, hd.which, tk) + c0;
+  T* dst = const_cast<T*>(token_ptr<T>(p.o, hd.which, tk)) + c0;
+  const int hs = p.x.s2[hd.which], ohs = p.o.s2[hd.which];
+  auto load = [&](int h) {
+    Raw8<T> r = {};
+    if (on && h < hd.end) r = load8(src + (int64_t)h * hs);
+    return r;
+  };
+  Raw8<T> raw[kAhead];
 #pragma unroll
-  for (int i = 0; i < kUnroll; ++i) {
-    const int h = hd.h0 + i * (32 / G);
-    raw[i] = Raw8<T>{};
-    if (on && h < hd.H) raw[i] = load8(src + h * hs);
-  }
+  for (int i = 0; i < kAhead; ++i) raw[i] = load(hd.first + i * (32 / G));
   int pc0;
   const int partner = partner_of<INTER>(p, lane, c0, pc0);
-  const void* wp = hd.which ? p.wk : p.wq;
+  const void* wp = p.w[hd.which];
   const V8 w = load_weight8(wp, p.w_dtype, on ? c0 : 0);
   const Angles<INTER> ang = load_angles<INTER>(p, tk.row, c0, 1.f);
   // out = r (x a + other b) per channel, other = the pair's second channel
   V8 a, b;
   if (INTER) {
+    const uint64_t minus = f2_pack(-1.f, -1.f);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint64_t minus = f2_pack(-1.f, -1.f);
       a.v[2 * i] = f2_mul(w.v[2 * i], ang.c[i]);
       b.v[2 * i] = f2_mul(f2_mul(w.v[2 * i + 1], ang.s[i]), minus);
       a.v[2 * i + 1] = f2_mul(w.v[2 * i + 1], ang.c[i]);
@@ -205,118 +214,117 @@ __global__ void __launch_bounds__(32 * kMaxWarps, INTER ? 4 : 3) fwd_kernel(cons
   }
   if (tk.bad && lane == 0) report_status(p.status, SA_DEV_BAD_INDEX);
   const float inv_d = 1.f / (float)p.D;
+  // lane groups whose heads run out keep step with the warp
+  for (int base = hd.first - lane / G; base < hd.end; base += kAhead * (32 / G)) {
 #pragma unroll
-  for (int i = 0; i < kUnroll; ++i) {
-    const int h = hd.h0 + i * (32 / G);
-    const V8 x = unpack8(raw[i]);
-    uint64_t s2 = f2_mul(x.v[0], x.v[0]);
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = base + i * (32 / G) + lane / G;
+      const Raw8<T> cur = raw[i];
+      raw[i] = load(h + kAhead * (32 / G));
+      const V8 x = unpack8(cur);
+      uint64_t s2 = f2_mul(x.v[0], x.v[0]);
 #pragma unroll
-    for (int j = 1; j < 4; ++j) s2 = f2_fma(x.v[j], x.v[j], s2);
-    const float ss = group_sum<G>(sum2(s2));
-    float r = inv_sqrt(fmaf(ss, inv_d, p.eps));
-    if (tk.bad) r = __int_as_float(0x7fc00000);
-    const uint64_t r2 = f2_pack(r, r);
-    V8 other;
-    if (INTER) {
-      other = V8{{x.v[1], x.v[0], x.v[3], x.v[2]}};
-    } else {
-      other = unpack8(shfl8(raw[i], partner));
+      for (int j = 1; j < 4; ++j) s2 = f2_fma(x.v[j], x.v[j], s2);
+      const float ss = group_sum<G>(sum2(s2));
+      float r = inv_sqrt<T>(fmaf(ss, inv_d, p.eps));
+      if (tk.bad) r = __int_as_float(0x7fc00000);
+      const uint64_t r2 = f2_pack(r, r);
+      V8 other;
+      if (INTER) {
+        other = V8{{x.v[1], x.v[0], x.v[3], x.v[2]}};
+      } else {
+        other = unpack8(shfl8(cur, partner));
+      }
+      V8 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o.v[j] = f2_mul(f2_fma(x.v[j], a.v[j], f2_mul(other.v[j], b.v[j])), r2);
+      if (on && h < hd.end) store8(dst + (int64_t)h * ohs, o);
     }
-    V8 o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o.v[j] = f2_mul(f2_fma(x.v[j], a.v[j], f2_mul(other.v[j], b.v[j])), r2);
-    if (on && h < hd.H) store8(dst + h * ohs, o);
   }
 }
 
-// Gradient: a warp keeps its chunk of heads and walks the tokens with a stride
-// of the grid, so that its part of dw stays in registers; a block writes one
-// partial row.
+// Gradient: a warp keeps its chunk of heads and walks the tokens with a fixed
+// stride, so that its part of dw stays in registers; a block writes one partial
+// row.
 template <typename T, int G, bool INTER>
-__global__ void __launch_bounds__(32 * kMaxWarps, sizeof(T) == 2 ? 3 : 2) bwd_kernel(const Params p) {
-  __shared__ float red[kMaxWarps][G * 8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int chunk = blockIdx.y * warps + warp;
-  const Heads hd = heads_of<G, kUnrollBwd>(p, chunk, lane);
+__global__ void __launch_bounds__(32 * kWarps, 2) bwd_kernel(const Params p) {
+  __shared__ float red[kWarps][G * 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned gw = blockIdx.x * kWarps + warp;
+  const unsigned t0 = gw / (unsigned)p.chunks, step = gridDim.x * kWarps / (unsigned)p.chunks;
+  const Heads hd = heads_of<G>(p, gw - t0 * p.chunks, lane);
   const int c0 = (lane % G) * 8;
   const bool on = c0 < p.D;
   int pc0;
   const int partner = partner_of<INTER>(p, lane, c0, pc0);
-  const V8 w = load_weight8(hd.which ? p.wk : p.wq, p.w_dtype, on ? c0 : 0);
-  const T* xb = reinterpret_cast<const T*>(hd.which ? p.k : p.q) + c0;
-  const T* db = reinterpret_cast<const T*>(hd.which ? p.dk : p.dq) + c0;
-  T* ob = reinterpret_cast<T*>(hd.which ? p.ko : p.qo) + c0;
-  const int64_t xs0 = hd.which ? p.ks0 : p.qs0, xs1 = hd.which ? p.ks1 : p.qs1,
-                xs2 = hd.which ? p.ks2 : p.qs2;
-  const int64_t ds0 = hd.which ? p.dks0 : p.dqs0, ds1 = hd.which ? p.dks1 : p.dqs1,
-                ds2 = hd.which ? p.dks2 : p.dqs2;
-  const int64_t os0 = hd.which ? p.kos0 : p.qos0, os1 = hd.which ? p.kos1 : p.qos1,
-                os2 = hd.which ? p.kos2 : p.qos2;
+  const V8 w = load_weight8(p.w[hd.which], p.w_dtype, on ? c0 : 0);
+  const int xs2 = p.x.s2[hd.which], ds2 = p.d.s2[hd.which], os2 = p.o.s2[hd.which];
   release_next_kernel();
   V8 acc = fill8(0.f);
   const float inv_d = 1.f / (float)p.D;
-  if (chunk < p.chunks) {
-    for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+  if (t0 < step) {  // warps past the last whole set of chunks have no tokens
+    for (unsigned t = t0; t < (unsigned)p.tokens; t += step) {
       const Token tk = token_of(p, t);
-      const T* xt = xb + tk.b * xs0 + tk.s * xs1;
-      const T* dt = db + tk.b * ds0 + tk.s * ds1;
-      T* ot = ob + tk.b * os0 + tk.s * os1;
-      Raw8<T> rx[kUnrollBwd], rd[kUnrollBwd];
-#pragma unroll
-      for (int i = 0; i < kUnrollBwd; ++i) {
-        const int h = hd.h0 + i * (32 / G);
+      const T* xt = token_ptr<T>(p.x, hd.which, tk) + c0;
+      const T* dt = token_ptr<T>(p.d, hd.which, tk) + c0;
+      T* ot = const_cast<T*>(token_ptr<T>(p.o, hd.which, tk)) + c0;
+      Raw8<T> rx[kAheadBwd], rd[kAheadBwd];
+      auto load = [&](int i, int h) {
         rx[i] = rd[i] = Raw8<T>{};
-        if (on && h < hd.H) {
-          rx[i] = load8(xt + h * xs2);
-          rd[i] = load8(dt + h * ds2);
+        if (on && h < hd.end) {
+          rx[i] = load8(xt + (int64_t)h * xs2);
+          rd[i] = load8(dt + (int64_t)h * ds2);
         }
-      }
+      };
+#pragma unroll
+      for (int i = 0; i < kAheadBwd; ++i) load(i, hd.first + i * (32 / G));
       const Angles<INTER> ang = load_angles<INTER>(p, tk.row, c0, -1.f);
       const uint64_t minus = f2_pack(-1.f, -1.f);
       const uint64_t pos_s[2] = {f2_mul(ang.s[0], minus), f2_mul(ang.s[1], minus)};
       if (tk.bad && lane == 0) report_status(p.status, SA_DEV_BAD_INDEX);
+      for (int base = hd.first - lane / G; base < hd.end; base += kAheadBwd * (32 / G)) {
 #pragma unroll
-      for (int i = 0; i < kUnrollBwd; ++i) {
-        const int h = hd.h0 + i * (32 / G);
-        const V8 x = unpack8(rx[i]), d = unpack8(rd[i]);
-        V8 g;
-        if (INTER) {
+        for (int i = 0; i < kAheadBwd; ++i) {
+          const int h = base + i * (32 / G) + lane / G;
+          const V8 x = unpack8(rx[i]), d = unpack8(rd[i]);
+          V8 g;
+          if (INTER) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            // the sine comes negated: g_e = d_e c + d_o s, g_o = d_o c - d_e s
-            g.v[2 * j] = f2_fma(d.v[2 * j], ang.c[j], f2_mul(d.v[2 * j + 1], pos_s[j]));
-            g.v[2 * j + 1] = f2_fma(d.v[2 * j + 1], ang.c[j], f2_mul(d.v[2 * j], ang.s[j]));
+            for (int j = 0; j < 2; ++j) {
+              // the sine comes negated: g_e = d_e c + d_o s, g_o = d_o c - d_e s
+              g.v[2 * j] = f2_fma(d.v[2 * j], ang.c[j], f2_mul(d.v[2 * j + 1], pos_s[j]));
+              g.v[2 * j + 1] = f2_fma(d.v[2 * j + 1], ang.c[j], f2_mul(d.v[2 * j], ang.s[j]));
+            }
+          } else {
+            const V8 other = unpack8(shfl8(rd[i], partner));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              g.v[j] = f2_fma(d.v[j], ang.c[j], f2_mul(other.v[j], ang.s[j]));
           }
-        } else {
-          const V8 other = unpack8(shfl8(rd[i], partner));
+          load(i, h + kAheadBwd * (32 / G));
+          uint64_t s2 = f2_mul(x.v[0], x.v[0]);
+          uint64_t t2 = f2_mul(f2_mul(g.v[0], w.v[0]), x.v[0]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            g.v[j] = f2_fma(d.v[j], ang.c[j], f2_mul(other.v[j], ang.s[j]));
-        }
-        V8 u;
-        uint64_t s2 = f2_mul(x.v[0], x.v[0]);
-        u.v[0] = f2_mul(g.v[0], w.v[0]);
-        uint64_t t2 = f2_mul(u.v[0], x.v[0]);
-#pragma unroll
-        for (int j = 1; j < 4; ++j) {
-          s2 = f2_fma(x.v[j], x.v[j], s2);
-          u.v[j] = f2_mul(g.v[j], w.v[j]);
-          t2 = f2_fma(u.v[j], x.v[j], t2);
-        }
-        const float ss = group_sum<G>(sum2(s2)), dot = group_sum<G>(sum2(t2));
-        float r = inv_sqrt(fmaf(ss, inv_d, p.eps));
-        if (tk.bad) r = __int_as_float(0x7fc00000);
-        const float m = -r * r * r * dot * inv_d;
-        const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
-        if (on && h < hd.H) {
-          V8 o;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            acc.v[j] = f2_fma(f2_mul(g.v[j], r2), x.v[j], acc.v[j]);
-            o.v[j] = f2_fma(x.v[j], m2, f2_mul(u.v[j], r2));
+          for (int j = 1; j < 4; ++j) {
+            s2 = f2_fma(x.v[j], x.v[j], s2);
+            t2 = f2_fma(f2_mul(g.v[j], w.v[j]), x.v[j], t2);
           }
-          store8(ot + h * os2, o);
+          const float ss = group_sum<G>(sum2(s2)), dot = group_sum<G>(sum2(t2));
+          float r = inv_sqrt<T>(fmaf(ss, inv_d, p.eps));
+          if (tk.bad) r = __int_as_float(0x7fc00000);
+          const float m = -r * r * r * dot * inv_d;
+          const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
+          if (on && h < hd.end) {
+            V8 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint64_t gr = f2_mul(g.v[j], r2);
+              acc.v[j] = f2_fma(gr, x.v[j], acc.v[j]);
+              o.v[j] = f2_fma(x.v[j], m2, f2_mul(gr, w.v[j]));
+            }
+            store8(ot + (int64_t)h * os2, o);
+          }
         }
       }
     }
@@ -331,27 +339,28 @@ __global__ void __launch_bounds__(32 * kMaxWarps, sizeof(T) == 2 ? 3 : 2) bwd_ke
     for (int o = 16; o >= G; o >>= 1) a8[j] += __shfl_xor_sync(0xffffffffu, a8[j], o);
     if (lane < G) red[warp][c0 + j] = a8[j];
   }
+  __shared__ int tensor[kWarps];
+  if (lane == 0) tensor[warp] = hd.which;
   __syncthreads();
-  float* row = p.part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.D;
-  const int first_k = p.chunks_q - blockIdx.y * warps;  // the first warp on k
-  for (int c = threadIdx.x; c < 2 * p.D; c += blockDim.x) {
+  float* row = p.part + (int64_t)blockIdx.x * 2 * p.D;
+  for (int c = threadIdx.x; c < 2 * p.D; c += 32 * kWarps) {
     const int which = c >= p.D, cc = which ? c - p.D : c;
     float s = 0.f;
-    for (int v = 0; v < warps; ++v)
-      if ((v >= first_k) == (which != 0)) s += red[v][cc];
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v)
+      if (tensor[v] == which) s += red[v][cc];
     row[c] = s;
   }
 }
 
 template <typename T, int G>
-void launch_g(const Params& p, bool inter, bool bwd, dim3 grid, int threads,
-              cudaStream_t stream) {
+void launch_g(const Params& p, bool inter, bool bwd, int grid, cudaStream_t stream) {
   if (bwd) {
-    if (inter) bwd_kernel<T, G, true><<<grid, threads, 0, stream>>>(p);
-    else bwd_kernel<T, G, false><<<grid, threads, 0, stream>>>(p);
+    if (inter) bwd_kernel<T, G, true><<<grid, 32 * kWarps, 0, stream>>>(p);
+    else bwd_kernel<T, G, false><<<grid, 32 * kWarps, 0, stream>>>(p);
   } else {
-    if (inter) fwd_kernel<T, G, true><<<grid, threads, 0, stream>>>(p);
-    else fwd_kernel<T, G, false><<<grid, threads, 0, stream>>>(p);
+    if (inter) fwd_kernel<T, G, true><<<grid, 32 * kWarps, 0, stream>>>(p);
+    else fwd_kernel<T, G, false><<<grid, 32 * kWarps, 0, stream>>>(p);
   }
 }
 
@@ -359,45 +368,55 @@ void launch_g(const Params& p, bool inter, bool bwd, dim3 grid, int threads,
 int group_of(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
 template <typename T>
-void launch_t(const Params& p, bool inter, bool bwd, dim3 grid, int threads,
-              cudaStream_t stream) {
+void launch_t(const Params& p, bool inter, bool bwd, int grid, cudaStream_t stream) {
   switch (group_of(p.D)) {
-    case 4: launch_g<T, 4>(p, inter, bwd, grid, threads, stream); break;
-    case 8: launch_g<T, 8>(p, inter, bwd, grid, threads, stream); break;
-    case 16: launch_g<T, 16>(p, inter, bwd, grid, threads, stream); break;
-    default: launch_g<T, 32>(p, inter, bwd, grid, threads, stream); break;
+    case 4: launch_g<T, 4>(p, inter, bwd, grid, stream); break;
+    case 8: launch_g<T, 8>(p, inter, bwd, grid, stream); break;
+    case 16: launch_g<T, 16>(p, inter, bwd, grid, stream); break;
+    default: launch_g<T, 32>(p, inter, bwd, grid, stream); break;
   }
 }
 
-int dispatch(const Params& p, int dtype, bool inter, bool bwd, dim3 grid, int threads,
-             cudaStream_t stream) {
-  if (dtype == SA_DTYPE_BF16) launch_t<__nv_bfloat16>(p, inter, bwd, grid, threads, stream);
-  else if (dtype == SA_DTYPE_FP16) launch_t<__half>(p, inter, bwd, grid, threads, stream);
-  else launch_t<float>(p, inter, bwd, grid, threads, stream);
+int dispatch(const Params& p, int dtype, bool inter, bool bwd, int grid, cudaStream_t stream) {
+  if (dtype == SA_DTYPE_BF16) launch_t<__nv_bfloat16>(p, inter, bwd, grid, stream);
+  else if (dtype == SA_DTYPE_FP16) launch_t<__half>(p, inter, bwd, grid, stream);
+  else launch_t<float>(p, inter, bwd, grid, stream);
   SA_CUDA_TRY(cudaGetLastError());
   return SA_OK;
 }
 
-// Blocks take the chunks of one token, split evenly over as few as possible.
-void shape(const Params& p, int& warps, int& rows) {
-  rows = (p.chunks + kMaxWarps - 1) / kMaxWarps;
-  warps = (p.chunks + rows - 1) / rows;
+// Chunks of heads: as long as leaves `want` warps over all tokens (the angles
+// and factors of a token are then worked out by fewer warps), at least `ahead`
+// steps.
+void shape(Params& p, int ahead, int64_t want) {
+  const int per = 32 / group_of(p.D);
+  const int sq = (p.Hq + per - 1) / per, sk = (p.Hk + per - 1) / per;
+  const auto chunks = [&](int steps) {
+    return (sq + steps - 1) / steps + (sk + steps - 1) / steps;
+  };
+  p.steps = ahead;
+  while (p.steps < (sq > sk ? sq : sk) && p.tokens * (int64_t)chunks(2 * p.steps) >= want)
+    p.steps *= 2;
+  p.chunks_q = (sq + p.steps - 1) / p.steps;
+  p.chunks = chunks(p.steps);
 }
 
-// Tokens in flight of the gradient kernel (grid.x): 24 warps per SM, a
-// partial row of dw from each block.
-constexpr int kBwdWarpsPerSm = 24;
-int bwd_grid(int tokens, int warps, int rows) {
-  const int64_t most =
-      ((int64_t)sa::sm_count_current_device() * kBwdWarpsPerSm + warps * rows - 1) / (warps * rows);
-  return (int)(tokens < most ? tokens : most);
+// The gradient's blocks, each a partial row of dw: 16 warps per SM, in whole
+// sets of chunks (the last few warps may have no tokens).
+constexpr int kBwdBlocksPerSm = 2;
+int bwd_grid(const Params& p) {
+  const int64_t want = ((int64_t)p.tokens * p.chunks + kWarps - 1) / kWarps;
+  const int64_t least = (p.chunks + kWarps - 1) / kWarps;  // a warp for every chunk
+  int64_t most = (int64_t)sa::sm_count_current_device() * kBwdBlocksPerSm;
+  if (most < least) most = least;
+  return (int)(want < most ? want : most);
 }
 
 bool aligned_ok(const void* base, const int64_t st[4], int dtype) {
   if (base == nullptr) return true;
   const int64_t mult = dtype == SA_DTYPE_FP32 ? 4 : 8;
   return (uintptr_t)base % 16 == 0 && st != nullptr && st[3] == 1 && st[0] >= 0 && st[1] >= 0 &&
-         st[2] >= 0 && st[0] % mult == 0 && st[1] % mult == 0 && st[2] % mult == 0;
+         st[2] >= 0 && st[0] % mult == 0 && st[1] % mult == 0 && st[2] % mult == 0 && st[2] <= 0x7fffffff;
 }
 
 // Arguments that the forward and the gradient share.
@@ -433,28 +452,26 @@ int check(const char* fn, int B, int S, int Hq, int Hk, int D, int dtype, const 
   return SA_OK;
 }
 
+Tensors tensors(const void* q, const void* k, const int64_t* qs, const int64_t* ks) {
+  return Tensors{{q, k}, {qs[0], ks[0]}, {qs[1], ks[1]}, {(int)qs[2], (int)ks[2]}};
+}
+
 void common(Params& p, const void* q, const void* k, const int64_t* qs, const int64_t* ks, int B,
             int S, int Hq, int Hk, int D, const void* w_q, const void* w_k, int w_dtype, float eps,
             const float* cos_t, const float* sin_t, int64_t fs, int table_rows, int rot,
             const void* positions, int pos_i64, const int64_t* pos_strides, void* qo, void* ko,
-            const int64_t* qos, const int64_t* kos, int unroll, int32_t* status) {
+            const int64_t* qos, const int64_t* kos, int32_t* status) {
   static const int64_t zero[4] = {0, 0, 0, 1};
   if (Hk == 0) ks = kos = zero;
   p = Params{};
-  p.q = q; p.k = k; p.qo = qo; p.ko = ko;
-  p.qs0 = qs[0]; p.qs1 = qs[1]; p.qs2 = qs[2];
-  p.ks0 = ks[0]; p.ks1 = ks[1]; p.ks2 = ks[2];
-  p.qos0 = qos[0]; p.qos1 = qos[1]; p.qos2 = qos[2];
-  p.kos0 = kos[0]; p.kos1 = kos[1]; p.kos2 = kos[2];
+  p.x = tensors(q, k, qs, ks);
+  p.o = tensors(qo, ko, qos, kos);
   p.B = B; p.S = S; p.Hq = Hq; p.Hk = Hk; p.D = D;
   p.rot = cos_t != nullptr ? rot : 0;
-  p.wq = w_q; p.wk = w_k; p.w_dtype = w_dtype; p.eps = eps;
+  p.w[0] = w_q; p.w[1] = w_k; p.w_dtype = w_dtype; p.eps = eps;
   p.cos_t = cos_t; p.sin_t = sin_t; p.fs = fs; p.table_rows = table_rows;
   p.pos = positions; p.pos_i64 = pos_i64;
   if (positions != nullptr) { p.ps0 = pos_strides[0]; p.ps1 = pos_strides[1]; }
-  const int per = unroll * (32 / group_of(D));
-  p.chunks_q = (Hq + per - 1) / per;
-  p.chunks = p.chunks_q + (Hk + per - 1) / per;
   p.tokens = B * S;
   p.status = status;
 }
@@ -483,18 +500,18 @@ extern "C" int sa_qk_head_norm_rope(
   Params p;
   common(p, q, k, q_strides, k_strides, B, S, Hq, Hk, D, w_q, w_k, w_dtype, eps, cos_table,
          sin_table, freq_row_stride, table_rows, rot_dim, positions, positions_i64, pos_strides,
-         q_out, k_out, qo_strides, ko_strides, kUnroll, status);
-  int warps, rows;
-  shape(p, warps, rows);
-  return dispatch(p, dtype, interleaved != 0, false, dim3((unsigned)p.tokens, (unsigned)rows),
-                  32 * warps, stream);
+         q_out, k_out, qo_strides, ko_strides, status);
+  shape(p, dtype == SA_DTYPE_FP32 ? ahead<float>() : ahead<__half>(), (int64_t)sa::sm_count_current_device() * 64);
+  const int64_t blocks = ((int64_t)p.tokens * p.chunks + kWarps - 1) / kWarps;
+  SA_CHECK_ARG(blocks <= 0x7fffffff / kWarps, "%s: too many tokens", fn);
+  return dispatch(p, dtype, interleaved != 0, false, (int)blocks, stream);
 }
 
 extern "C" size_t sa_qk_head_norm_rope_bwd_workspace_size(int D) {
   if (D < 8) return 0;
-  // at most kBwdWarpsPerSm blocks (of one warp) per SM, or one per block row
-  return (size_t)(sa::sm_count_current_device() * sa::headnorm::kBwdWarpsPerSm +
-                  sa::headnorm::kMaxRows) * 2 * D * sizeof(float);
+  const int64_t most = (int64_t)sa::sm_count_current_device() * sa::headnorm::kBwdBlocksPerSm;
+  const int64_t least = sa::headnorm::kMaxHeads / (sa::headnorm::kAheadBwd * sa::headnorm::kWarps) + 1;
+  return (size_t)(most > least ? most : least) * 2 * D * sizeof(float);
 }
 
 extern "C" int sa_qk_head_norm_rope_bwd(
@@ -532,17 +549,13 @@ extern "C" int sa_qk_head_norm_rope_bwd(
     Params p;
     common(p, q, k, q_strides, k_strides, B, S, Hq, Hk, D, w_q, w_k, w_dtype, eps, cos_table,
            sin_table, freq_row_stride, table_rows, rot_dim, positions, positions_i64, pos_strides,
-           dq_in, dk_in, dqi_strides, dki_strides, kUnrollBwd, status);
-    p.dq = dq; p.dk = dk;
-    p.dqs0 = dq_strides[0]; p.dqs1 = dq_strides[1]; p.dqs2 = dq_strides[2];
-    if (Hk > 0) { p.dks0 = dk_strides[0]; p.dks1 = dk_strides[1]; p.dks2 = dk_strides[2]; }
+           dq_in, dk_in, dqi_strides, dki_strides, status);
+    p.d = tensors(dq, dk, dq_strides, Hk > 0 ? dk_strides : dq_strides);
     p.part = weights ? part : nullptr;
-    int warps, rows;
-    shape(p, warps, rows);
-    const int gx = bwd_grid(p.tokens, warps, rows);
-    blocks = gx * rows;
-    rc = dispatch(p, dtype, interleaved != 0, true, dim3((unsigned)gx, (unsigned)rows), 32 * warps,
-                  stream);
+    shape(p, kAheadBwd, (int64_t)sa::sm_count_current_device() * kBwdBlocksPerSm * kWarps * 2);
+    SA_CHECK_ARG((int64_t)p.tokens * p.chunks <= 0x7fffffff, "%s: too many tokens", fn);
+    blocks = bwd_grid(p);
+    rc = dispatch(p, dtype, interleaved != 0, true, blocks, stream);
     if (rc != SA_OK) return rc;
   }
   if (!weights) return SA_OK;

@@ -7,9 +7,10 @@
 // Memory-bound: x and the upstream gradient are read and dx written once
 // (6 bf16 values per hidden channel of Q and K together). A block takes whole
 // rows, one 8-channel vector of Q and one of K per thread, so that the angles
-// are read once for both, dw needs 16 registers and the next row's vectors are
-// loaded before the current row's sums are reduced. (A warp per row, 48
-// channels a lane, needed 158 registers and reached 28% of the copy rate.)
+// are read once for both and dw needs 16 registers. The rows come through a
+// ring of bulk copies, three rows ahead. (A warp per row with 48 channels a
+// lane needed 158 registers and reached 28% of the copy rate; rows loaded one
+// ahead into registers spilled and reached 55%.)
 
 #include <math.h>
 
@@ -60,19 +61,21 @@ using namespace sa::nr;
 
 constexpr int kMaxHidden = 4096;
 constexpr int kMaxThreads = kMaxHidden / 8;
+constexpr int kRing = 3;  // rows in flight per block
 
 struct Params {
-  const __nv_bfloat16* d[2];  // upstream gradients of q, k
-  const __nv_bfloat16* x[2];
+  const __nv_bfloat16* src[4];  // q, k, and the upstream gradients of both
+  int64_t ss[4];
   __nv_bfloat16* o[2];
+  int64_t os[2];
   const void* w[2];
-  int64_t ds[2], xs[2], os[2];
   int rows, S, hidden, D;
   int w_dtype;
   float eps;
   const float *cos_t, *sin_t;
   int64_t fs;
-  float* part;  // [partial rows][2][hidden], NULL without dw
+  float* part;  // [block][2][hidden], NULL without dw
+  int32_t* status;
 };
 
 // Four sums over a warp at once: after two exchange steps a lane carries one
@@ -90,49 +93,54 @@ __device__ __forceinline__ float warp_sum4(float a, float b, float c, float d, i
   return z;
 }
 
-struct Row {
-  Raw8<__nv_bfloat16> x[2], d[2];
-};
-
-__device__ __forceinline__ Row load_row(const Params& p, int64_t row, int c0, bool on) {
-  Row r;
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    r.x[w] = r.d[w] = Raw8<__nv_bfloat16>{};
-    if (on) {
-      r.x[w] = load8(p.x[w] + row * p.xs[w] + c0);
-      r.d[w] = load8(p.d[w] + row * p.ds[w] + c0);
-    }
-  }
-  return r;
-}
-
 // One thread per 8 channels; rows blockIdx.x, + gridDim.x, ... Registers are
 // capped so that 768 threads fit an SM.
 template <int MAXT>
 __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
-  __shared__ __align__(16) float sums[2][MAXT / 32][4];
+  __shared__ float sums[2][MAXT / 32 * 4];
+  __shared__ __align__(8) uint64_t full[kRing];
+  extern __shared__ __align__(16) uint8_t ring[];  // [kRing][4][hidden] bf16
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int c0 = threadIdx.x * 8;
   const bool on = c0 < p.hidden;
+  const uint32_t row_bytes = p.hidden * 2;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
+  release_next_kernel();
+  __syncthreads();
+  auto fetch = [&](int slot, int row) {
+    mbar_arrive_expect_tx(&full[slot], 4 * row_bytes);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      bulk_load(ring + (slot * 4 + i) * row_bytes, p.src[i] + (int64_t)row * p.ss[i], row_bytes,
+                &full[slot]);
+  };
+  if (threadIdx.x == 0)
+    for (int i = 0; i < kRing; ++i)
+      if ((int64_t)blockIdx.x + (int64_t)i * gridDim.x < p.rows)
+        fetch(i, blockIdx.x + i * gridDim.x);
   const int p0 = (c0 % p.D) >> 1;
   const float inv_n = 1.f / (float)p.hidden;
-  release_next_kernel();
   V8 acc[2] = {fill8(0.f), fill8(0.f)};
   V8 w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) w[i] = load_weight8(p.w[i], p.w_dtype, on ? c0 : 0);
-  Row next = load_row(p, blockIdx.x, c0, on);
-  int turn = 0;
-  for (int row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-    const Row cur = next;
+  const int s_step = gridDim.x % p.S;
+  int s = blockIdx.x % p.S;  // position of the row
+  int n = 0;                 // rows done
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, ++n) {
+    const int slot = n % kRing;
     float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.cos_t != nullptr && on) {
-      const int64_t s = (unsigned)row % (unsigned)p.S;
       c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t + s * p.fs + p0));
       s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t + s * p.fs + p0));
     }
-    if (p.rows - row > (int)gridDim.x) next = load_row(p, (int64_t)row + gridDim.x, c0, on);
+    s += s_step;
+    if (s >= p.S) s -= p.S;
+    // the rows arrive by themselves: a copy that does not leaves NaN behind
+    const bool there = mbar_wait(&full[slot], (uint32_t)(n / kRing) & 1u, p.status, nullptr);
     const uint64_t c2[2] = {f2_pack(c4.x, c4.y), f2_pack(c4.z, c4.w)};
     const uint64_t s2[2] = {f2_pack(s4.x, s4.y), f2_pack(s4.z, s4.w)};
     const uint64_t n2[2] = {f2_pack(-s4.x, -s4.y), f2_pack(-s4.z, -s4.w)};
@@ -140,8 +148,14 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
     float ss[2], dot[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x[i] = unpack8(cur.x[i]);
-      const V8 d = unpack8(cur.d[i]);
+      Raw8<__nv_bfloat16> rx = {}, rd = {};
+      if (on) {
+        rx.v[0] = reinterpret_cast<const uint4*>(ring + (slot * 4 + i) * row_bytes)[threadIdx.x];
+        rd.v[0] =
+            reinterpret_cast<const uint4*>(ring + (slot * 4 + 2 + i) * row_bytes)[threadIdx.x];
+      }
+      x[i] = unpack8(rx);
+      const V8 d = unpack8(rd);
       uint64_t a2 = 0ull, b2 = 0ull;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -159,17 +173,26 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
     const float z = warp_sum4(ss[0], dot[0], ss[1], dot[1], lane);
     // two buffers in turn: a warp writes a row's sums only after the block has
     // passed the barrier of the row before, so the row before that has been read
-    if (lane < 4) sums[turn][warp][lane] = z;
+    float* turn = sums[n & 1];
+    if (lane < 4) turn[warp * 4 + lane] = z;
     __syncthreads();
-    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int v = 0; v < warps; ++v) {
-      const float4 q = *reinterpret_cast<const float4*>(sums[turn][v]);
-      t.x += q.x; t.y += q.y; t.z += q.z; t.w += q.w;
+    // every thread has its part of the row in registers: the slot is free
+    if (threadIdx.x == 0 && row + (int64_t)kRing * gridDim.x < p.rows) {
+      fence_proxy_async_smem();
+      fetch(slot, (int)(row + (int64_t)kRing * gridDim.x));
     }
+    // lane l sums value l & 3 of every eighth warp, then over the lanes
+    float t = 0.f;
+    for (int v = lane; v < warps * 4; v += 32) t += turn[v];
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float r = inv_sqrt(fmaf(i ? t.z : t.x, inv_n, p.eps));
-      const float m = -r * r * r * (i ? t.w : t.y) * inv_n;
+      const float sq = __shfl_sync(0xffffffffu, t, 2 * i);
+      const float dt = __shfl_sync(0xffffffffu, t, 2 * i + 1);
+      float r = inv_sqrt<__nv_bfloat16>(fmaf(sq, inv_n, p.eps));
+      if (!there) r = __int_as_float(0x7fc00000);
+      const float m = -r * r * r * dt * inv_n;
       const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
       V8 o;
 #pragma unroll
@@ -178,7 +201,7 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
         acc[i].v[j] = f2_fma(gr, x[i].v[j], acc[i].v[j]);
         o.v[j] = f2_fma(x[i].v[j], m2, f2_mul(gr, w[i].v[j]));
       }
-      if (on) store8(p.o[i] + (int64_t)row * p.os[i] + c0, o);
+      if (on) store8(p.o[i] + row * p.os[i] + c0, o);
     }
   }
   if (p.part == nullptr || !on) return;
@@ -215,7 +238,7 @@ extern "C" int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_ro
                                    const float* sin_table, int64_t freq_row_stride, void* dq_in,
                                    void* dk_in, int64_t dqi_row_stride, int64_t dki_row_stride,
                                    float* dw_q, float* dw_k, void* workspace, size_t ws_bytes,
-                                   cudaStream_t stream) {
+                                   int32_t* status, cudaStream_t stream) {
   using namespace sa::qkrope_bwd;
   const char* fn = "sa_qk_norm_rope_bwd";
   SA_CHECK_ARG(rows >= 0 && S >= 1 && D >= 8 && D % 8 == 0,
@@ -247,13 +270,13 @@ extern "C" int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_ro
   float* part = static_cast<float*>(workspace);
   if (rows > 0) {
     Params p;
-    p.d[0] = static_cast<const __nv_bfloat16*>(dq); p.d[1] = static_cast<const __nv_bfloat16*>(dk);
-    p.x[0] = static_cast<const __nv_bfloat16*>(q); p.x[1] = static_cast<const __nv_bfloat16*>(k);
-    p.o[0] = static_cast<__nv_bfloat16*>(dq_in); p.o[1] = static_cast<__nv_bfloat16*>(dk_in);
+    p.src[0] = static_cast<const __nv_bfloat16*>(q); p.ss[0] = q_row_stride;
+    p.src[1] = static_cast<const __nv_bfloat16*>(k); p.ss[1] = k_row_stride;
+    p.src[2] = static_cast<const __nv_bfloat16*>(dq); p.ss[2] = dq_row_stride;
+    p.src[3] = static_cast<const __nv_bfloat16*>(dk); p.ss[3] = dk_row_stride;
+    p.o[0] = static_cast<__nv_bfloat16*>(dq_in); p.os[0] = dqi_row_stride;
+    p.o[1] = static_cast<__nv_bfloat16*>(dk_in); p.os[1] = dki_row_stride;
     p.w[0] = w_q; p.w[1] = w_k;
-    p.ds[0] = dq_row_stride; p.ds[1] = dk_row_stride;
-    p.xs[0] = q_row_stride; p.xs[1] = k_row_stride;
-    p.os[0] = dqi_row_stride; p.os[1] = dki_row_stride;
     p.rows = rows; p.S = S; p.hidden = hidden; p.D = D;
     p.w_dtype = w_is_bf16 ? SA_DTYPE_BF16 : SA_DTYPE_FP32;
     p.eps = eps;
@@ -261,8 +284,14 @@ extern "C" int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_ro
     p.part = dw_q != nullptr ? part : nullptr;
     const int threads = threads_of(hidden);
     part_rows = blocks_of(rows, threads);
-    if (threads <= 256) kernel<256><<<part_rows, threads, 0, stream>>>(p);
-    else kernel<kMaxThreads><<<part_rows, threads, 0, stream>>>(p);
+    p.status = status;
+    const size_t smem = (size_t)kRing * 4 * hidden * 2;
+    const void* fn_ptr = threads <= 256 ? (const void*)kernel<256> : (const void*)kernel<kMaxThreads>;
+    const int rc = sa::func_attr_once(fn_ptr, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kRing * 4 * 2 * 8 * (threads <= 256 ? 256 : kMaxThreads));
+    if (rc != SA_OK) return rc;
+    if (threads <= 256) kernel<256><<<part_rows, threads, smem, stream>>>(p);
+    else kernel<kMaxThreads><<<part_rows, threads, smem, stream>>>(p);
     SA_CUDA_TRY(cudaGetLastError());
   }
   if (dw_q == nullptr) return SA_OK;

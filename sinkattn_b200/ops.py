@@ -978,7 +978,7 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
            _meta(w_q), _meta(w_k), _meta(cos), _meta(sin), _meta(dq), _meta(dk))
     plan = _PLANS.get(key) or _remember(key, _qk_norm_rope_bwd_plan(
         dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, sin, dq, dk))
-    idx, dev, fits, in_rows, sizes, w_bf16, fs, out_rows, need = plan
+    idx, dev, fits, in_rows, sizes, w_bf16, fs, out_rows, need, status = plan
     ptrs = [_ptr(t) for t in (dq_out, dk_out, q, k, w_q, w_k, cos, sin)]
     if not fits or any(x is not None and x & 15 for x in ptrs):
         def rows(t):
@@ -1008,7 +1008,7 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
     _launch(idx, "sa_qk_norm_rope_bwd", _lib.load().sa_qk_norm_rope_bwd, ptrs[0], ptrs[1],
             in_rows[0], in_rows[1], ptrs[2], ptrs[3], in_rows[2], in_rows[3], *sizes, ptrs[4],
             ptrs[5], w_bf16, eps, ptrs[6], ptrs[7], fs, dq.data_ptr(), dk.data_ptr(), *out_rows,
-            _ptr(dw_q), _ptr(dw_k), *ws)
+            _ptr(dw_q), _ptr(dw_k), *ws, status)
     return dq, dk, dw_q, dw_k
 
 
@@ -1052,7 +1052,8 @@ def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, s
     return (dev.index, dev, fits, [t.stride(1) for t in (dq_out, dk_out, q, k)],
             (B * S, max(S, 1), hidden, int(head_dim)), w_bf16,
             0 if cos is None else head_dim // 2,
-            [hidden if t is None else t.stride(1) for t in (dq, dk)], need)
+            [hidden if t is None else t.stride(1) for t in (dq, dk)], need,
+            DeviceStatus.pointer(dev))
 
 
 _DTYPES = {torch.bfloat16: _lib.SA_DTYPE_BF16, torch.float16: _lib.SA_DTYPE_FP16,
