@@ -7,8 +7,8 @@
 // Memory-bound: x and the upstream gradient are read and dx written once
 // (6 bf16 values per hidden channel of Q and K together). A block takes whole
 // rows, one 8-channel vector of Q and one of K per thread, so that the angles
-// are read once for both and dw needs 16 registers. The rows come through a
-// ring of bulk copies, three rows ahead. (A warp per row with 48 channels a
+// are read once for both and dw needs 16 registers. The rows and their angles
+// come through a ring of bulk copies, three rows ahead. (A warp per row with 48 channels a
 // lane needed 158 registers and reached 28% of the copy rate; rows loaded one
 // ahead into registers spilled and reached 55%.)
 
@@ -99,11 +99,13 @@ template <int MAXT>
 __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
   __shared__ float sums[2][MAXT / 32 * 4];
   __shared__ __align__(8) uint64_t full[kRing];
-  extern __shared__ __align__(16) uint8_t ring[];  // [kRing][4][hidden] bf16
+  // [kRing] slots: four rows of bf16, then the position's cosines and sines
+  extern __shared__ __align__(16) uint8_t ring[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int c0 = threadIdx.x * 8;
   const bool on = c0 < p.hidden;
-  const uint32_t row_bytes = p.hidden * 2;
+  const uint32_t row_bytes = p.hidden * 2, angle_bytes = p.cos_t != nullptr ? p.D * 2 : 0;
+  const uint32_t slot_bytes = 4 * row_bytes + 2 * angle_bytes;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -111,11 +113,16 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
   release_next_kernel();
   __syncthreads();
   auto fetch = [&](int slot, int row) {
-    mbar_arrive_expect_tx(&full[slot], 4 * row_bytes);
+    uint8_t* dst = ring + slot * slot_bytes;
+    mbar_arrive_expect_tx(&full[slot], slot_bytes);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      bulk_load(ring + (slot * 4 + i) * row_bytes, p.src[i] + (int64_t)row * p.ss[i], row_bytes,
-                &full[slot]);
+      bulk_load(dst + i * row_bytes, p.src[i] + (int64_t)row * p.ss[i], row_bytes, &full[slot]);
+    if (p.cos_t != nullptr) {
+      const int64_t at = (int64_t)((unsigned)row % (unsigned)p.S) * p.fs;
+      bulk_load(dst + 4 * row_bytes, p.cos_t + at, angle_bytes, &full[slot]);
+      bulk_load(dst + 4 * row_bytes + angle_bytes, p.sin_t + at, angle_bytes, &full[slot]);
+    }
   };
   if (threadIdx.x == 0)
     for (int i = 0; i < kRing; ++i)
@@ -127,20 +134,18 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
   V8 w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) w[i] = load_weight8(p.w[i], p.w_dtype, on ? c0 : 0);
-  const int s_step = gridDim.x % p.S;
-  int s = blockIdx.x % p.S;  // position of the row
-  int n = 0;                 // rows done
+  int n = 0;  // rows done
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, ++n) {
     const int slot = n % kRing;
-    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.cos_t != nullptr && on) {
-      c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t + s * p.fs + p0));
-      s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t + s * p.fs + p0));
-    }
-    s += s_step;
-    if (s >= p.S) s -= p.S;
+    const uint8_t* src = ring + slot * slot_bytes;
     // the rows arrive by themselves: a copy that does not leaves NaN behind
     const bool there = mbar_wait(&full[slot], (uint32_t)(n / kRing) & 1u, p.status, nullptr);
+    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.cos_t != nullptr && on) {
+      const uint8_t* angles = src + 4 * row_bytes + p0 * 4;
+      c4 = *reinterpret_cast<const float4*>(angles);
+      s4 = *reinterpret_cast<const float4*>(angles + angle_bytes);
+    }
     const uint64_t c2[2] = {f2_pack(c4.x, c4.y), f2_pack(c4.z, c4.w)};
     const uint64_t s2[2] = {f2_pack(s4.x, s4.y), f2_pack(s4.z, s4.w)};
     const uint64_t n2[2] = {f2_pack(-s4.x, -s4.y), f2_pack(-s4.z, -s4.w)};
@@ -150,9 +155,8 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
     for (int i = 0; i < 2; ++i) {
       Raw8<__nv_bfloat16> rx = {}, rd = {};
       if (on) {
-        rx.v[0] = reinterpret_cast<const uint4*>(ring + (slot * 4 + i) * row_bytes)[threadIdx.x];
-        rd.v[0] =
-            reinterpret_cast<const uint4*>(ring + (slot * 4 + 2 + i) * row_bytes)[threadIdx.x];
+        rx.v[0] = reinterpret_cast<const uint4*>(src + i * row_bytes)[threadIdx.x];
+        rd.v[0] = reinterpret_cast<const uint4*>(src + (2 + i) * row_bytes)[threadIdx.x];
       }
       x[i] = unpack8(rx);
       const V8 d = unpack8(rd);
@@ -285,10 +289,11 @@ extern "C" int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_ro
     const int threads = threads_of(hidden);
     part_rows = blocks_of(rows, threads);
     p.status = status;
-    const size_t smem = (size_t)kRing * 4 * hidden * 2;
+    const size_t smem = (size_t)kRing * (4 * hidden * 2 + (cos_table != nullptr ? 4 * D : 0));
     const void* fn_ptr = threads <= 256 ? (const void*)kernel<256> : (const void*)kernel<kMaxThreads>;
     const int rc = sa::func_attr_once(fn_ptr, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kRing * 4 * 2 * 8 * (threads <= 256 ? 256 : kMaxThreads));
+                                      // rows and angles of the widest head, D = hidden
+                                      kRing * (4 * 2 + 4) * 8 * (threads <= 256 ? 256 : kMaxThreads));
     if (rc != SA_OK) return rc;
     if (threads <= 256) kernel<256><<<part_rows, threads, smem, stream>>>(p);
     else kernel<kMaxThreads><<<part_rows, threads, smem, stream>>>(p);
