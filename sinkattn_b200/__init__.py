@@ -8,10 +8,14 @@ CUDA behind a C ABI (include/sinkattn.h, libsinkattn.so):
 * the calibration chain: mean pooling of Q/K, pooled-score softmax, batch
   mean / accumulation and the 0.85-coverage block-mask build.
 
+Both have gradients: :mod:`sinkattn_b200.autograd` holds the differentiable
+attention and the differentiable Q/K norm + rotation (per head, or over the
+hidden dimension) in front of it.
+
 ``install()`` binds the drop-in functions of :mod:`sinkattn_b200.reference_api`
 into the reference's modules; :mod:`sinkattn_b200.ops` is the tensor-level API.
 """
-from . import ops
+from . import autograd, ops
 from ._lib import load as load_library
 from .reference_api import (
     _block_sparse_attn,
@@ -23,6 +27,7 @@ from .reference_api import (
 
 __all__ = [
     "ops",
+    "autograd",
     "load_library",
     "install",
     "block_sparse_attn_func",

@@ -1,0 +1,119 @@
+"""Differentiable forms of the tensor-level operators.
+
+Each function runs the same kernel as its namesake in :mod:`sinkattn_b200.ops`
+and records what its gradient kernel needs; without a differentiable input
+(or under torch.no_grad()) nothing is recorded. The gradients are first-order
+only. reference_api's drop-ins call these where an input requires a gradient.
+
+A backward pass may be captured into a CUDA graph like any other torch one:
+warm it up on a side stream and let no graph of the same leaves that was
+recorded eagerly stay alive beside it (torch ties a leaf's accumulation to the
+stream it was first recorded on).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call on these tensors has to be recorded."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _BlockSparseAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, block_mask, softmax_scale, head_mask_type):
+        out, lse = ops.bsattn_fwd(q, k, v, block_mask, softmax_scale=softmax_scale,
+                                  head_mask_type=head_mask_type)
+        ctx.save_for_backward(q, k, v, out, lse, block_mask, head_mask_type)
+        ctx.softmax_scale = softmax_scale
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlse):
+        if dout is None and dlse is None:
+            return (None,) * 6
+        q, k, v, out, lse, block_mask, head_mask_type = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros_like(out)
+        dq, dk, dv = ops.bsattn_bwd(dout, q, k, v, out, lse, block_mask,
+                                    softmax_scale=ctx.softmax_scale,
+                                    head_mask_type=head_mask_type, dlse=dlse)
+        return dq, dk, dv, None, None, None
+
+
+def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           block_mask: torch.Tensor, softmax_scale: Optional[float] = None,
+                           head_mask_type: Optional[torch.Tensor] = None):
+    """ops.bsattn_fwd with gradients for q, k and v, through both results.
+
+    Arguments as for ops.bsattn_fwd. Returns (out [B,H,Sq,D] bf16, lse fp32
+    [B,H,Sq]). Keys and values broadcast over heads (expanded views) get their
+    gradients summed over them by autograd."""
+    return _BlockSparseAttention.apply(q, k, v, block_mask, softmax_scale, head_mask_type)
+
+
+def _like(grad: Optional[torch.Tensor], w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if grad is None or w is None else grad.to(w.dtype)
+
+
+class _QKHeadNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, eps, w_q, w_k, cos, sin, positions, interleaved):
+        out_q, out_k = ops.qk_head_norm_rope(q, k, eps, w_q, w_k, cos, sin, positions=positions,
+                                             interleaved=interleaved)
+        ctx.save_for_backward(q, k, w_q, w_k, cos, sin, positions)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return out_q, out_k
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, w_q, w_k, cos, sin, positions = ctx.saved_tensors
+        dq, dk, dw_q, dw_k = ops.qk_head_norm_rope_bwd(
+            dq, None if k is None else dk, q, k, ctx.eps, w_q, w_k, cos, sin,
+            positions=positions, interleaved=ctx.interleaved)
+        return dq, dk, None, _like(dw_q, w_q), _like(dw_k, w_k), None, None, None, None
+
+
+def qk_head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], eps: float,
+                      w_q: Optional[torch.Tensor] = None, w_k: Optional[torch.Tensor] = None,
+                      cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None, interleaved: bool = True):
+    """ops.qk_head_norm_rope with gradients for q, k, w_q and w_k (the tables
+    get none). The weights' gradients are summed in fp32 and returned in the
+    weights' type."""
+    return _QKHeadNormRope.apply(q, k, eps, w_q, w_k, cos, sin, positions, interleaved)
+
+
+class _QKNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, head_dim, eps, w_q, w_k, cos, sin):
+        out_q, out_k = ops.qk_norm_rope(q, k, head_dim, eps, w_q, w_k, cos, sin)
+        ctx.save_for_backward(q, k, w_q, w_k, cos, sin)
+        ctx.head_dim, ctx.eps = head_dim, eps
+        return out_q, out_k
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, w_q, w_k, cos, sin = ctx.saved_tensors
+        dq, dk, dw_q, dw_k = ops.qk_norm_rope_bwd(dq, dk, q, k, ctx.head_dim, ctx.eps, w_q, w_k,
+                                                  cos, sin)
+        return dq, dk, None, None, _like(dw_q, w_q), _like(dw_k, w_k), None, None
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, head_dim: int, eps: float,
+                 w_q: Optional[torch.Tensor] = None, w_k: Optional[torch.Tensor] = None,
+                 cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None):
+    """ops.qk_norm_rope (out of place) with gradients for q, k, w_q and w_k
+    (the tables get none); the bf16 rounding between the norm and the rotation
+    counts as the identity."""
+    return _QKNormRope.apply(q, k, head_dim, eps, w_q, w_k, cos, sin)

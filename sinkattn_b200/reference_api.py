@@ -29,7 +29,7 @@ from typing import Optional
 
 import torch
 
-from . import ops
+from . import autograd, ops
 
 # How head_mask_type is read by block_sparse_attn_func.
 #   "per_head" (default): a mask with one slice per head is applied per head;
@@ -102,7 +102,8 @@ def block_sparse_attn_func(
     packing described by cu_seqlens_*), base_blockmask bool
     [B, Hm, ceil(max_seqlen_q/128), ceil(max_seqlen_k/128)].
     Returns out [total_q, H, D], or (out, softmax_lse fp32 [B, H, max_seqlen_q],
-    None) when return_attn_probs.
+    None) when return_attn_probs. Where q, k or v requires a gradient both are
+    differentiable.
     """
     if p_dropout != 0.0:
         raise NotImplementedError("sinkattn_b200: dropout is not supported (forward inference only)")
@@ -126,7 +127,14 @@ def block_sparse_attn_func(
         if any(t < 0 for t in hv):
             raise NotImplementedError("sinkattn_b200: streaming heads (head_mask_type < 0)")
         hmt = head_mask_type.to(torch.int32)
-    if total_q == B * Sq and total_k == B * Sk:
+    record = autograd.needs_grad(q_unpad, k_unpad, v_unpad)
+    if total_q == B * Sq and total_k == B * Sk and record:
+        q = q_unpad.view(B, Sq, H, D).permute(0, 2, 1, 3)
+        k = k_unpad.view(B, Sk, H, D).permute(0, 2, 1, 3)
+        v = v_unpad.view(B, Sk, H, D).permute(0, 2, 1, 3)
+        out, lse = autograd.block_sparse_attention(q, k, v, base_blockmask, softmax_scale, hmt)
+        out = out.permute(0, 2, 1, 3).reshape(total_q, H, D)
+    elif total_q == B * Sq and total_k == B * Sk:
         # uniform batch: every sequence has the maximum length (the reference's case)
         q = q_unpad.view(B, Sq, H, D).permute(0, 2, 1, 3)
         k = k_unpad.view(B, Sk, H, D).permute(0, 2, 1, 3)
@@ -139,6 +147,10 @@ def block_sparse_attn_func(
         # ragged varlen batch: one launch per sequence on its own slice
         cq = [int(x) for x in cu_seqlens_q.detach().cpu().tolist()]
         ck = [int(x) for x in cu_seqlens_k.detach().cpu().tolist()]
+        if record:
+            out, lse = _ragged_recorded(q_unpad, k_unpad, v_unpad, cq, ck, base_blockmask, Sq,
+                                        softmax_scale, hmt)
+            return (out, lse, None) if return_attn_probs else out
         out = torch.empty_like(q_unpad)
         lse = (torch.full((B, H, Sq), float("-inf"), dtype=torch.float32, device=q_unpad.device)
                if return_attn_probs else None)
@@ -163,6 +175,31 @@ def block_sparse_attn_func(
     return out
 
 
+def _ragged_recorded(q_unpad, k_unpad, v_unpad, cq, ck, base_blockmask, max_q, softmax_scale, hmt):
+    """The ragged batch of block_sparse_attn_func, differentiable: one launch
+    per sequence, joined. Returns (out [total_q, H, D], lse [B, H, max_q])."""
+    H = q_unpad.shape[1]
+    outs, lses = [], []
+    for b in range(len(cq) - 1):
+        sq, sk = cq[b + 1] - cq[b], ck[b + 1] - ck[b]
+        if sq == 0 or sk == 0:
+            outs.append(torch.zeros_like(q_unpad[cq[b]:cq[b + 1]]))
+            lses.append(torch.full((H, max_q), float("-inf"), dtype=torch.float32,
+                                   device=q_unpad.device))
+            continue
+        qb, kb, vb = (t[c[b]:c[b + 1]].unsqueeze(0).permute(0, 2, 1, 3)
+                      for t, c in ((q_unpad, cq), (k_unpad, ck), (v_unpad, ck)))
+        mb = base_blockmask[b:b + 1, :, : math.ceil(sq / _BLOCK), : math.ceil(sk / _BLOCK)]
+        ob, lb = autograd.block_sparse_attention(qb, kb, vb, mb, softmax_scale, hmt)
+        outs.append(ob[0].permute(1, 0, 2))
+        lses.append(torch.nn.functional.pad(lb[0], (0, max_q - sq), value=float("-inf")))
+    out = torch.cat(outs)
+    rest = q_unpad.shape[0] - out.shape[0]  # rows behind the last sequence
+    if rest:
+        out = torch.cat([out, torch.zeros_like(q_unpad[:rest])])
+    return out, torch.stack(lses)
+
+
 @_reports_device_failures
 def _block_sparse_attn(
     q: torch.Tensor,
@@ -174,15 +211,20 @@ def _block_sparse_attn(
     """sparse_attention.py:710-776 without the three transpose copies: the
     kernel reads the strided [B,H,S,D] views directly through TMA. Returns
     out as a [B,S,H,D]-contiguous tensor viewed [B,H,S,D] (the reference's
-    layout) and lse [B,H,S,1] in q.dtype (line 776)."""
+    layout) and lse [B,H,S,1] in q.dtype (line 776). Differentiable where q, k
+    or v requires a gradient."""
     B, H, Sq, D = q.shape
     if HEAD_MASK_TYPE_MODE == "upstream":
         # the reference passes ones(H): every head reads mask slice 0
         hmt = torch.ones(H, dtype=torch.int32, device=q.device)
     else:
         hmt = None
-    out, lse = ops.bsattn_fwd(q, k, v, block_mask.contiguous(), head_mask_type=hmt,
-                              return_lse=return_lse)
+    if autograd.needs_grad(q, k, v):
+        out, lse = autograd.block_sparse_attention(q, k, v, block_mask.contiguous(), None, hmt)
+        lse = lse if return_lse else None
+    else:
+        out, lse = ops.bsattn_fwd(q, k, v, block_mask.contiguous(), head_mask_type=hmt,
+                                  return_lse=return_lse)
     if lse is None:
         return out, None
     return out, lse.unsqueeze(-1).to(device=q.device, dtype=q.dtype)
@@ -387,7 +429,8 @@ def fused_prepare_attention_tensors(attn, hidden_states, encoder_hidden_states=N
     self-attention with RMS-normalised Q/K and a rotary embedding: the Q/K
     RMSNorm and the rotation run as one kernel (sa_qk_norm_rope) on the
     projections' outputs. Q, K and V come back as [B,H,S,D] views of the
-    [B,S,H*D] projections, the layout the attention kernel reads. Other
+    [B,S,H*D] projections, the layout the attention kernel reads. With
+    gradients enabled it is differentiable (sa_qk_norm_rope_bwd). Other
     configurations run the reference's own function."""
     norm_q, norm_k = getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)
     fusable = (encoder_hidden_states is None and rotary_emb is not None
@@ -406,11 +449,16 @@ def fused_prepare_attention_tensors(attn, hidden_states, encoder_hidden_states=N
     D = query.shape[-1] // attn.heads
     with (timing.section("qk_norm") if timing is not None and timing.is_enabled else nullcontext()):
         cos, sin = _rotary_tables(rotary_emb, S, D)
-        in_place = not (query.requires_grad or key.requires_grad)
-        query, key = ops.qk_norm_rope(query, key, D, float(norm_q.eps), norm_q.weight,
-                                      norm_k.weight, cos.to(query.device), sin.to(query.device),
-                                      out_q=query if in_place else None,
-                                      out_k=key if in_place else None)
+        cos, sin = cos.to(query.device), sin.to(query.device)
+        if autograd.needs_grad(query, key, norm_q.weight, norm_k.weight):
+            query, key = autograd.qk_norm_rope(query, key, D, float(norm_q.eps), norm_q.weight,
+                                               norm_k.weight, cos, sin)
+        else:
+            in_place = not (query.requires_grad or key.requires_grad)
+            query, key = ops.qk_norm_rope(query, key, D, float(norm_q.eps), norm_q.weight,
+                                          norm_k.weight, cos, sin,
+                                          out_q=query if in_place else None,
+                                          out_k=key if in_place else None)
     query = query.unflatten(2, (attn.heads, -1)).transpose(1, 2)
     key = key.unflatten(2, (attn.heads, -1)).transpose(1, 2)
     value = value.unflatten(2, (attn.heads, -1)).transpose(1, 2)

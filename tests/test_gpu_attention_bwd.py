@@ -282,3 +282,65 @@ def test_gradient_against_differences():
     _, bound = reference(q, k, v, dout, keep, 1 / math.sqrt(128))
     tol = 6 * math.sqrt(sum(float((b * d).square().sum()) for b, d in zip(bound, dirs)))
     assert abs(slope - want) <= tol, (slope, want, tol)
+
+
+def test_refusals():
+    from sinkattn_b200 import ops
+
+    q, k, v, dout, mask = make(1, 2, 200, 300, 1.0, 19)
+    out, lse = ops.bsattn_fwd(q, k, v, mask)
+    ok = (dout, q, k, v, out, lse, mask)
+
+    def refuse(match, **kw):
+        names = ("dout", "q", "k", "v", "out", "lse", "block_mask")
+        args = {**dict(zip(names, ok)), **kw}
+        with pytest.raises(RuntimeError, match=match):
+            ops.bsattn_bwd(**args)
+
+    refuse("dout must be bf16", dout=dout.float())
+    refuse("v must be bf16", v=v[:, :, :299])
+    refuse("out must be bf16", out=out[:, :1])
+    refuse("lse must be fp32", lse=lse.bfloat16())
+    refuse("dlse must be fp32", dlse=lse[..., :100])
+    refuse("block_mask must be", block_mask=mask[..., :1])
+    refuse("block_mask must be bool", block_mask=mask.float())
+    refuse("head_mask_type must be int32", head_mask_type=torch.ones(2, device="cuda"))
+    refuse("dq must", dq=torch.empty(1, 2, 200, 136, device="cuda", dtype=torch.bfloat16)[..., 4:132])
+    refuse("dk must be bf16", dk=torch.empty_like(k, dtype=torch.float32))
+    refuse("workspace", workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    refuse("CUDA tensors only", q=q.cpu())
+    refuse("mask has 1 heads", block_mask=mask[:, :1])
+
+
+def test_from_a_thread_without_a_context():
+    """A thread whose first CUDA call is ours (an autograd worker may be one):
+    through the C entry point, as torch's own calls would bind the context."""
+    import ctypes
+    import threading
+
+    from sinkattn_b200 import _lib, ops
+
+    q, k, v, dout, mask = make(1, 2, 300, 300, 0.6, 20)
+    want = run(q, k, v, dout, mask)
+    out, lse = ops.bsattn_fwd(q, k, v, mask)
+    lib = _lib.load()
+    size = lib.sa_bsattn_bwd_workspace_size(1, 2, 300, 300)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    got = [torch.empty_like(t) for t in want]
+    torch.cuda.synchronize()
+    st = [_lib.strides4(t) for t in (dout, q, k, v, out, *got)]
+    ms = (ctypes.c_int64 * 4)(*mask.stride())
+    rcs = []
+
+    def work():
+        rcs.append(lib.sa_bsattn_bwd(
+            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *st[:5],
+            lse.data_ptr(), None, 1, 2, 300, 300, 128, mask.data_ptr(), ms, 2, None, -1.0,
+            *(t.data_ptr() for t in got), *st[5:], ws.data_ptr(), size, None, None))
+
+    t = threading.Thread(target=work)
+    t.start(), t.join()
+    torch.cuda.synchronize()
+    assert rcs == [_lib.SA_OK]
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)

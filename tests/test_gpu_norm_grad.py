@@ -362,3 +362,53 @@ def test_gradients_against_differences():
                for g, n in ((q, "q"), (k, "k"), (dwq, "wq"), (dwk, "wk")))
     # 2^-16 of every term (above); the difference's own error is h^2 of third derivatives
     assert abs(got - want) <= 2.0 ** -16 * size + 1e-6 * size, (got, want, size)
+
+
+def test_refusals():
+    from sinkattn_b200 import ops
+
+    a, w, cos, sin, pos = make(2, 5, 4, 2, 128, 128, torch.bfloat16, T=9)
+
+    def refuse(match, fn="qk_head_norm_rope", exc=RuntimeError, **kw):
+        args = dict(q=a["q"], k=a["k"], eps=1e-6, w_q=w[0], w_k=w[1], cos=cos, sin=sin,
+                    positions=pos)
+        if fn.endswith("bwd"):
+            args.update(dq_out=a["dq"], dk_out=a["dk"])
+        args.update(kw)
+        with pytest.raises(exc, match=match):
+            getattr(ops, fn)(**args)
+
+    refuse("expects q, k of", q=a["q"][0])
+    refuse("k must be", k=a["k"].float())
+    refuse("k must be", k=a["k"][:, :4])
+    refuse("bf16, fp16 or fp32", q=a["q"].double(), k=a["k"].double())
+    refuse("go together", w_k=None)
+    refuse("go together", sin=None)
+    refuse("128 elements", w_q=w[0][:64])
+    refuse("cos and sin must be fp32", cos=cos.double(), sin=sin.double())
+    refuse("cos and sin must be fp32", sin=sin[:, :32])
+    refuse("positions must be", positions=pos.float())
+    refuse("positions must be", positions=pos[:, :4])
+    refuse("positions need", cos=None, sin=None)
+    refuse("table rows", cos=cos[:4], sin=sin[:4], positions=None)
+    refuse("multiple of 16", cos=cos[:, :12], sin=sin[:, :12], interleaved=False)
+    refuse("out_q must", out_q=torch.empty(2, 5, 4, 132, dtype=torch.bfloat16, device="cuda")[..., 4:])
+    refuse("out_k without k", k=None, w_k=None, out_k=a["k"])
+    refuse("CUDA tensors only", cos=cos.cpu(), sin=sin.cpu())
+    refuse("multiple of 8 up to 256", q=a["q"][..., :100], k=a["k"][..., :100], w_q=None, w_k=None,
+           cos=None, sin=None, positions=None)
+    refuse("dk_out is missing", fn="qk_head_norm_rope_bwd", dk_out=None)
+    refuse("dq_out must be", fn="qk_head_norm_rope_bwd", dq_out=a["dq"].float())
+    refuse("workspace", fn="qk_head_norm_rope_bwd",
+           workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    x = torch.zeros(2, 5, 256, dtype=torch.bfloat16, device="cuda")
+    h = dict(dq_out=x, dk_out=x, q=x, k=x, head_dim=128, eps=1e-6)
+    for match, exc, kw in (("must be bf16", RuntimeError, dict(q=x.float())),
+                           ("must be bf16", RuntimeError, dict(dk_out=x[:, :4])),
+                           ("256 elements", RuntimeError, dict(w_q=w[0], w_k=w[1])),
+                           ("go together", RuntimeError, dict(w_q=x[0, 0])),
+                           ("frequency shape", ValueError, dict(cos=cos, sin=sin)),
+                           ("uniform rows", RuntimeError, dict(dq=x.transpose(0, 1).contiguous()
+                                                               .transpose(0, 1)))):
+        with pytest.raises(exc, match=match):
+            ops.qk_norm_rope_bwd(**{**h, **kw})
