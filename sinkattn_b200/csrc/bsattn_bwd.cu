@@ -276,6 +276,23 @@ __device__ __forceinline__ void sum_parts(const float* src, int pieces, int64_t 
   }
 }
 
+__device__ __forceinline__ const uint32_t (&first16(const uint32_t (&r)[32]))[16] {
+  return reinterpret_cast<const uint32_t(&)[16]>(r);
+}
+
+// x = hi + lo in bf16 each, two values: 16 significant bits instead of 8.
+__device__ __forceinline__ void split_bf16x2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(x0, x1);
+  lo = pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+}
+
+// P and dS enter their products as bf16, which with fp32 sums leaves an error
+// like that of the bf16 results (1.4 times it together). Over a few tokens
+// single roundings show, up to twice that, so FINE keeps P and dS as two bf16
+// halves, each a product of its own in the columns that X and Y leave free.
+// The launch takes it where the blocks do not fill the GPU once and the extra
+// products hide behind latencies (300 tokens, 2 heads: 12.1 us become 13.0).
+template <bool FINE>
 __global__ void __launch_bounds__(kThreads, 1)
     bsattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                       const __grid_constant__ CUtensorMap tm_k,
@@ -579,6 +596,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int kk = (u / (per / 2)) * per + c * (per / 2) + u % (per / 2);
           mma_ts(d, a + (kk / per) * kCols + (kk % per) * 8, b + ((kk * 2048) >> 4), idesc_mn,
                  u > 0 || !first ? 1u : 0u);
+          if (FINE)
+            mma_ts(d, a + (kk / per) * kCols + kCols / 2 + (kk % per) * 8, b + ((kk * 2048) >> 4),
+                   idesc_mn, 1u);
         }
       };
       for (int k = 0; ok; ++k) {
@@ -709,12 +729,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!wait(&ctl->x_full[jp & 1u], (jp >> 1) & 1u)) break;
           tc_fence_after();
           const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(st + g * kCols);
+          uint32_t later[16];  // FINE writes over all columns: read them first
+          if (FINE) tmem_ld16(t_self + kColX + 16, later);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            uint32_t r[16], pk[8];
-            tmem_ld16(t_self + kColX + c * 16, r);
-            tmem_wait_ld();
-            reg_fence16(r);
+            uint32_t r[16], pk[8], pl[8];
+            if (FINE && c == 1) {
+#pragma unroll
+              for (int u = 0; u < 16; ++u) r[u] = later[u];
+            } else {
+              tmem_ld16(t_self + kColX + c * 16, r);
+              tmem_wait_ld();
+              reg_fence16(r);
+              if (FINE) reg_fence16(later);
+            }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
               const ulonglong2 s2 = nl[c * 4 + (u >> 1)];
@@ -726,9 +754,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               x0 = ex2_approx(x0);
               x1 = ex2_approx(x1);
               pr[c * 8 + u] = f2_pack(x0, x1);
-              pk[u] = pack_bf16x2(x0, x1);
+              if (FINE) split_bf16x2(x0, x1, pk[u], pl[u]);
+              else pk[u] = pack_bf16x2(x0, x1);
             }
             tmem_st8(t_self + kColX + c * 8, pk);
+            if (FINE) tmem_st8(t_self + kColX + kCols / 2 + c * 8, pl);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&ctl->x_done[c]);
@@ -748,9 +778,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                               u & 1 ? s2.y : s2.x));
             float d0, d1;
             f2_unpack(d2, d0, d1);
-            pk[u] = pack_bf16x2(d0, d1);
+            if (FINE) split_bf16x2(d0, d1, pk[u], r[u]);
+            else pk[u] = pack_bf16x2(d0, d1);
           }
           tmem_st16(t_self + kColY, pk);
+          if (FINE) tmem_st16(t_self + kColY + kCols / 2, first16(r));
         } else {
           if (j == 0) {
             const float nl = ctl->stats[jp & 1u][row], nd = ctl->stats[jp & 1u][kT + row];
@@ -798,9 +830,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                               row_nd2));
             float d0, d1;
             f2_unpack(d2, d0, d1);
-            pk[u] = pack_bf16x2(d0, d1);
+            if (FINE) split_bf16x2(d0, d1, pk[u], r[u]);
+            else pk[u] = pack_bf16x2(d0, d1);
           }
           tmem_st16(y, pk);
+          if (FINE) tmem_st16(y + kCols / 2, first16(r));
         }
         tmem_wait_st();
         tc_fence_before();
@@ -1001,7 +1035,9 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
     p.part[k] = reinterpret_cast<float*>(ws + l.part[k]);
   }
 
-  if ((rc = sa::func_attr_once((const void*)bsattn_bwd_kernel,
+  const bool fine = (int64_t)nq * nk * B * H <= sms;
+  const auto kernel = fine ? bsattn_bwd_kernel<true> : bsattn_bwd_kernel<false>;
+  if ((rc = sa::func_attr_once((const void*)kernel,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes)) !=
       SA_OK)
     return rc;
@@ -1012,7 +1048,7 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
       dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_item,
       reinterpret_cast<int*>(ws + 256), (int)l.n_joined, counts[0], counts[1], p.mask, B, nk);
   SA_CUDA_TRY(cudaGetLastError());
-  SA_CUDA_TRY(sa::launch_after(bsattn_bwd_kernel, dim3(items < sms ? items : sms), dim3(kThreads),
+  SA_CUDA_TRY(sa::launch_after(kernel, dim3(items < sms ? items : sms), dim3(kThreads),
                                kSmemBytes, stream, tq, tk, tv, td, p));
   return SA_OK;
 }
