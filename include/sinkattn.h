@@ -51,7 +51,7 @@ extern "C" {
 /* Device status codes written into `status` by kernels. */
 #define SA_DEV_OK 0
 #define SA_DEV_WAIT_TIMEOUT 1 /* an mbarrier wait exceeded its iteration limit */
-#define SA_DEV_BAD_INDEX 2    /* a position outside the rotary tables */
+#define SA_DEV_BAD_INDEX 2    /* a rotary position or head_mask_type entry out of range */
 
 /* Element types of the entry points that take one. */
 #define SA_DTYPE_BF16 0
@@ -149,8 +149,10 @@ SA_API int sa_sink_dynamic_attn_fwd(
  *   to lse. dq, dk and dv are written whole: rows whose mask row (key blocks
  *   whose mask column) keeps nothing get 0, whatever their lse and dout hold.
  * block_mask, m_strides, Hm, head_mask_type, softmax_scale, status: as for
- *   sa_bsattn_fwd. Sq, Sk <= 131072. P and dS enter their products as bf16;
- *   the sums, dP and the row statistics are fp32.
+ *   sa_bsattn_fwd (an entry t > Hm is not followed: the head is computed dense
+ *   and *status becomes SA_DEV_BAD_INDEX). Sq, Sk <= 131072. P and dS enter
+ *   their products as bf16 (as two bf16 halves each where the call has no more
+ *   blocks than the GPU has SMs); the sums, dP and the row statistics are fp32.
  * Every sum is formed by one CTA in block order (no atomics on data), so equal
  *   calls give equal bits.
  * workspace: sa_bsattn_bwd_workspace_size(B, H, Sq, Sk) bytes, 256-byte

@@ -48,6 +48,7 @@ struct Mask {
   const uint8_t* mask;
   int64_t s0, s1, s2, s3;
   const int32_t* head_mask_type;
+  int heads;
   // The mask column (kind 0) or row (kind 1) blk of a head; true when the head
   // is dense, with nothing to read.
   __device__ __forceinline__ bool line(int kind, int b, int h, int blk, const uint8_t*& m,
@@ -55,7 +56,9 @@ struct Mask {
     int mh = h;
     if (head_mask_type != nullptr) {
       const int ty = head_mask_type[h];
-      if (ty <= 0) return true;
+      // an entry past the mask's heads has no slice to read: dense, and reported
+      // by the row statistics
+      if (ty <= 0 || ty > heads) return true;
       mh = ty - 1;
     }
     m = mask + b * s0 + mh * s1 + blk * (kind ? s2 : s3);
@@ -130,11 +133,14 @@ __global__ void __launch_bounds__(256)
                      const float* __restrict__ lse, const float* __restrict__ dlse, int H, int Sq,
                      int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_item,
                      int* joined, int n_joined, int* counts0, int* counts1, const Mask mask, int B,
-                     int nk) {
+                     int nk, int32_t* status) {
   release_next_kernel();  // it waits for this one's completion all the same
   const int nq = rows_pad / kT;
   const int block = blockIdx.y * gridDim.x + blockIdx.x, blocks = gridDim.x * gridDim.y;
   if (block == 0 && threadIdx.x == 0) *next_item = 0;
+  if (block == 0 && mask.head_mask_type != nullptr)
+    for (int i = threadIdx.x; i < H; i += 256)
+      if (mask.head_mask_type[i] > mask.heads) report_status(status, SA_DEV_BAD_INDEX);
   for (int i = block * 256 + threadIdx.x; i < n_joined; i += blocks * 256) joined[i] = 0;
   // kept blocks of every tile of the kinds that may be cut, a warp per tile
   for (int kind = 0; kind < 2; ++kind) {
@@ -1009,7 +1015,7 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
   Params p;
   p.B = B; p.H = H; p.Sq = Sq; p.Sk = Sk; p.nq = nq; p.nk = nk;
   p.mask = sa::attn_bwd::Mask{block_mask, m_strides[0], m_strides[1], m_strides[2], m_strides[3],
-                              head_mask_type};
+                              head_mask_type, Hm};
   p.scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf((float)D);
   p.scale_log2 = p.scale * 1.4426950408889634f;
   char* ws = static_cast<char*>(workspace);
@@ -1046,7 +1052,7 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
       static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
       do_strides[0], do_strides[1], do_strides[2], o_strides[0], o_strides[1], o_strides[2], lse,
       dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_item,
-      reinterpret_cast<int*>(ws + 256), (int)l.n_joined, counts[0], counts[1], p.mask, B, nk);
+      reinterpret_cast<int*>(ws + 256), (int)l.n_joined, counts[0], counts[1], p.mask, B, nk, status);
   SA_CUDA_TRY(cudaGetLastError());
   SA_CUDA_TRY(sa::launch_after(kernel, dim3(items < sms ? items : sms), dim3(kThreads),
                                kSmemBytes, stream, tq, tk, tv, td, p));

@@ -59,7 +59,9 @@ extern "C" int sa_check_status(int32_t* status) {
   *reinterpret_cast<volatile int32_t*>(status) = SA_DEV_OK;
   if (v == SA_DEV_BAD_INDEX) {
     sa::set_error(
-        "a kernel met a position outside the rotary tables: the rows of those tokens are NaN");
+        "a kernel met an index outside what it selects from: a position outside the rotary "
+        "tables (the rows of those tokens are NaN) or a head_mask_type entry past the mask's "
+        "heads (those heads are computed dense)");
     return SA_EINVAL;
   }
   sa::set_error(

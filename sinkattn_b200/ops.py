@@ -73,6 +73,35 @@ def _meta(t: Optional[torch.Tensor]):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
+def _strides16_ok(t: torch.Tensor) -> bool:
+    """Whole 16-byte vectors along the last dimension, and from element to
+    element of the others (a dimension of size 1 is never stepped along)."""
+    n = 16 // t.element_size()
+    return t.stride(-1) == 1 and not any(
+        s % n for s, size in zip(t.stride()[:-1], t.shape[:-1]) if size > 1)
+
+
+def _view16_ok(t: torch.Tensor) -> bool:
+    return _strides16_ok(t) and t.data_ptr() % 16 == 0
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t itself when contiguous on a 16-byte boundary, else a copy that is."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _kernel_strides(t: torch.Tensor):
+    """t's strides for the C ABI; those of dimensions of size 1, which may be
+    anything in torch, as 8."""
+    return (_lib.ctypes.c_int64 * t.dim())(
+        *(s if size > 1 else 8 for s, size in zip(t.stride()[:-1], t.shape[:-1])), 1)
+
+
+def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 
@@ -260,8 +289,9 @@ def bsattn_bwd(
                           None if head_mask_type is None else head_mask_type.contiguous(),
                           None if dlse is None else dlse.contiguous(), dq, dk, dv, workspace)
     # each gradient by default [B,S,H,D]-contiguous, viewed [B,H,S,D]
-    dq, dk, dv = (torch.empty_strided(*g, dtype=torch.bfloat16, device=dev) if t is None else t
-                  for t, g in zip((dq, dk, dv), grads))
+    dq = q.new_empty_strided(*grads[0]) if dq is None else dq
+    dk = k.new_empty_strided(*grads[1]) if dk is None else dk
+    dv = v.new_empty_strided(*grads[1]) if dv is None else dv
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif workspace.get_device() != idx:
@@ -287,7 +317,7 @@ def _bsattn_bwd_plan(dout, q, k, v, out, lse, block_mask, softmax_scale, head_ma
         if t.dtype != torch.bfloat16 or t.shape != (B, H, S, D):
             raise RuntimeError(f"bsattn_bwd: {name} must be bf16 {(B, H, S, D)}, got {t.dtype} "
                                f"{tuple(t.shape)}")
-        if name in ("dq", "dk", "dv") and not _bf16_view_ok(t):
+        if name in ("dq", "dk", "dv") and not _view16_ok(t):
             raise RuntimeError(f"bsattn_bwd: {name} must have stride(-1)=1, 16-byte strides and "
                                "alignment")
     for name, t in (("lse", lse), ("dlse", dlse)):
@@ -295,18 +325,18 @@ def _bsattn_bwd_plan(dout, q, k, v, out, lse, block_mask, softmax_scale, head_ma
             raise RuntimeError(f"bsattn_bwd: {name} must be fp32 {(B, H, Sq)}, got {t.dtype} "
                                f"{tuple(t.shape)}")
     _check_block_mask("bsattn_bwd", block_mask, head_mask_type, B, H, Sq, Sk)
-    fits = (all(t.stride(-1) == 1 and not any(x % 8 for x in t.stride()[:-1])
-                for t in (dout, q, k, v, out))
+    fits = (all(_strides16_ok(t) for t in (dout, q, k, v, out))
             and all(t is None or t.is_contiguous() for t in (lse, dlse, head_mask_type)))
-    need = int(_lib.load().sa_bsattn_bwd_workspace_size(B, H, Sq, Sk))
+    with torch.cuda.device(dev):
+        need = int(_lib.load().sa_bsattn_bwd_workspace_size(B, H, Sq, Sk))
     ms = list(block_mask.stride())
     if block_mask.shape[0] == 1:
         ms[0] = 0
     i64x4 = _lib.ctypes.c_int64 * 4
-    grads = [((B, H, S, D), (S * H * D, D, H * D, 1)) for S in (Sq, Sk, Sk)]
-    out_strides = [i64x4(*(g[1] if t is None else t.stride()))
-                   for t, g in zip((dq, dk, dv), grads)]
-    return (dev.index, dev, fits, [_lib.strides4(t) for t in (dout, q, k, v, out)],
+    grads = [((B, H, S, D), (S * H * D, D, H * D, 1)) for S in (Sq, Sk)]
+    out_strides = [i64x4(*g[1]) if t is None else _kernel_strides(t)
+                   for t, g in zip((dq, dk, dv), grads + grads[1:])]
+    return (dev.index, dev, fits, [_kernel_strides(t) for t in (dout, q, k, v, out)],
             ((B, H, Sq, Sk, D), (i64x4(*ms), block_mask.shape[1]),
              -1.0 if softmax_scale is None else float(softmax_scale)),
             grads, out_strides, need, DeviceStatus.pointer(dev))
@@ -974,15 +1004,15 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
     without weights). Equal calls give equal bits. Calls sharing a `workspace`
     (uint8, sa_qk_norm_rope_bwd_workspace_size bytes) must not overlap.
     """
-    key = ("qk_norm_rope_bwd", _meta(dq_out), _meta(dk_out), _meta(q), _meta(k), head_dim, eps,
+    key = ("qk_norm_rope_bwd", _meta(dq_out), _meta(dk_out), _meta(q), _meta(k), head_dim,
            _meta(w_q), _meta(w_k), _meta(cos), _meta(sin), _meta(dq), _meta(dk))
     plan = _PLANS.get(key) or _remember(key, _qk_norm_rope_bwd_plan(
-        dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, sin, dq, dk))
+        dq_out, dk_out, q, k, head_dim, w_q, w_k, cos, sin, dq, dk))
     idx, dev, fits, in_rows, sizes, w_bf16, fs, out_rows, need, status = plan
     ptrs = [_ptr(t) for t in (dq_out, dk_out, q, k, w_q, w_k, cos, sin)]
     if not fits or any(x is not None and x & 15 for x in ptrs):
         def rows(t):
-            return t if _uniform_rows(t) and t.data_ptr() % 16 == 0 else _aligned(t)
+            return t if _row_stride(t) is not None and t.data_ptr() % 16 == 0 else _aligned(t)
 
         def weight(w):
             return w if w is None else _aligned(w if w_bf16 else w.float())
@@ -993,8 +1023,8 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
         return qk_norm_rope_bwd(rows(dq_out), rows(dk_out), rows(q), rows(k), head_dim, eps,
                                 weight(w_q), weight(w_k), table(cos), table(sin), dq, dk,
                                 workspace)
-    dq = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if dq is None else dq
-    dk = torch.empty(q.shape, dtype=torch.bfloat16, device=dev) if dk is None else dk
+    dq = _contiguous_like(q) if dq is None else dq
+    dk = _contiguous_like(q) if dk is None else dk
     dw_q = dw_k = None
     if need:
         dw_q = torch.empty(sizes[2], dtype=torch.float32, device=dev)
@@ -1007,18 +1037,25 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
         else (None, 0)
     _launch(idx, "sa_qk_norm_rope_bwd", _lib.load().sa_qk_norm_rope_bwd, ptrs[0], ptrs[1],
             in_rows[0], in_rows[1], ptrs[2], ptrs[3], in_rows[2], in_rows[3], *sizes, ptrs[4],
-            ptrs[5], w_bf16, eps, ptrs[6], ptrs[7], fs, dq.data_ptr(), dk.data_ptr(), *out_rows,
+            ptrs[5], w_bf16, float(eps), ptrs[6], ptrs[7], fs, dq.data_ptr(), dk.data_ptr(), *out_rows,
             _ptr(dw_q), _ptr(dw_k), *ws, status)
     return dq, dk, dw_q, dw_k
 
 
-def _uniform_rows(t: torch.Tensor) -> bool:
-    """[B, S, hidden] whose B * S rows lie at one stride of whole 16-byte vectors."""
-    return t.numel() == 0 or (t.stride(-1) == 1 and t.stride(1) % 8 == 0
-                              and (t.shape[0] == 1 or t.stride(0) == t.shape[1] * t.stride(1)))
+def _row_stride(t: torch.Tensor) -> Optional[int]:
+    """The one stride at which the B * S rows of [B, S, hidden] lie, in whole
+    16-byte vectors; None if there is none."""
+    B, S, hidden = t.shape
+    if t.numel() == 0 or B * S == 1:
+        st = hidden
+    elif S == 1:
+        st = t.stride(0)
+    else:
+        st = t.stride(1) if B == 1 or t.stride(0) == S * t.stride(1) else None
+    return st if st is not None and t.stride(-1) == 1 and st % 8 == 0 else None
 
 
-def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, sin, dq, dk):
+def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, w_q, w_k, cos, sin, dq, dk):
     dev = _require_cuda(dq_out, dk_out, q, k, w_q, w_k, cos, sin, dq, dk)
     if q.dim() != 3:
         raise RuntimeError("qk_norm_rope_bwd expects [B, S, hidden] tensors")
@@ -1028,11 +1065,11 @@ def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, s
         if t is not None and (t.dtype != torch.bfloat16 or t.shape != (B, S, hidden)):
             raise RuntimeError(f"qk_norm_rope_bwd: {name} must be bf16 {(B, S, hidden)}, got "
                                f"{t.dtype} {tuple(t.shape)}")
-        if t is not None and name in ("dq", "dk") and not _uniform_rows(t):
+        if t is not None and name in ("dq", "dk") and _row_stride(t) is None:
             raise RuntimeError("qk_norm_rope_bwd outputs need uniform rows, 16-byte aligned")
     if (w_q is None) != (w_k is None) or (cos is None) != (sin is None):
         raise RuntimeError("qk_norm_rope_bwd: w_q and w_k, cos and sin go together")
-    fits = all(_uniform_rows(t) for t in (dq_out, dk_out, q, k))
+    fits = all(_row_stride(t) is not None for t in (dq_out, dk_out, q, k))
     w_bf16 = 1
     if w_q is not None:
         if w_q.shape != (hidden,) or w_k.shape != (hidden,):
@@ -1049,27 +1086,15 @@ def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, s
     if w_q is not None:
         with torch.cuda.device(dev):
             need = int(_lib.load().sa_qk_norm_rope_bwd_workspace_size(hidden))
-    return (dev.index, dev, fits, [t.stride(1) for t in (dq_out, dk_out, q, k)],
+    return (dev.index, dev, fits, [_row_stride(t) or 0 for t in (dq_out, dk_out, q, k)],
             (B * S, max(S, 1), hidden, int(head_dim)), w_bf16,
             0 if cos is None else head_dim // 2,
-            [hidden if t is None else t.stride(1) for t in (dq, dk)], need,
+            [hidden if t is None else _row_stride(t) for t in (dq, dk)], need,
             DeviceStatus.pointer(dev))
 
 
 _DTYPES = {torch.bfloat16: _lib.SA_DTYPE_BF16, torch.float16: _lib.SA_DTYPE_FP16,
            torch.float32: _lib.SA_DTYPE_FP32}
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """t itself when contiguous on a 16-byte boundary, else a copy that is."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _view16_ok(t: torch.Tensor) -> bool:
-    n = 16 // t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and not any(s % n for s in t.stride()[:-1]))
 
 
 def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, outs):
@@ -1121,9 +1146,9 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
                                f", got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} "
                                f"{tuple(sin.shape)}")
         rows, rot = cos.shape[0], 2 * cos.shape[1]
-        fs = cos.stride(0)
-        fits = fits and _strides16_ok(cos) and _strides16_ok(sin) and fs == sin.stride(0) \
-            and fs >= rot // 2
+        fs = cos.stride(0) if rows > 1 else (rot // 2 + 3) // 4 * 4
+        fits = fits and _strides16_ok(cos) and _strides16_ok(sin) and (
+            rows == 1 or fs == sin.stride(0) >= rot // 2)
     pst = None
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
@@ -1146,18 +1171,13 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
         if t is None:
             b, s, h, d = like.shape
             return i64x4(s * h * d, h * d, d, 1)
-        return _lib.strides4(t)
+        return _kernel_strides(t)
 
     return (dev.index, dev, fits, (st(q, q), st(k, k)), [st(t, like) for _, t, like in more],
             [st(t, like) for _, t, like in outs], (B, S, Hq, Hk, D, _DTYPES[q.dtype]), w_dtype,
             (fs, rows, rot, int(bool(interleaved))),
             int(positions is not None and positions.dtype == torch.int64), pst, need,
             DeviceStatus.pointer(dev))
-
-
-def _strides16_ok(t: torch.Tensor) -> bool:
-    n = 16 // t.element_size()
-    return t.stride(-1) == 1 and not any(s % n for s in t.stride()[:-1])
 
 
 def _head_norm_copies(w_q, w_k, cos, sin, tensors):
@@ -1168,8 +1188,8 @@ def _head_norm_copies(w_q, w_k, cos, sin, tensors):
     if w_q is not None:
         same = w_q.dtype in _DTYPES and (w_k is None or w_k.dtype == w_q.dtype)
         w_q, w_k = (None if w is None else _aligned(w if same else w.float()) for w in (w_q, w_k))
-    if cos is not None and not (_view16_ok(cos) and _view16_ok(sin)
-                                and cos.stride(0) == sin.stride(0) >= cos.shape[1]):
+    if cos is not None and not (_view16_ok(cos) and _view16_ok(sin) and (
+            cos.shape[0] == 1 or cos.stride(0) == sin.stride(0) >= cos.shape[1])):
         cos, sin = _aligned(cos), _aligned(sin)
     return [fit(t) for t in tensors], w_q, w_k, cos, sin
 
@@ -1203,11 +1223,11 @@ def qk_head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], eps: float,
         return qk_head_norm_rope(q, k, eps, w_q, w_k, cos, sin, positions, interleaved, out_q,
                                  out_k)
     if out_q is None:
-        out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out_q = _contiguous_like(q)
     if out_k is None and k is not None:
-        out_k = torch.empty(k.shape, dtype=q.dtype, device=dev)
+        out_k = _contiguous_like(k)
     _launch(idx, "sa_qk_head_norm_rope", _lib.load().sa_qk_head_norm_rope, pq, pk, *st, *sizes,
-            pwq, pwk, w_dtype, eps, pc, ps, *tab, _ptr(positions), pos64, pst, out_q.data_ptr(),
+            pwq, pwk, w_dtype, float(eps), pc, ps, *tab, _ptr(positions), pos64, pst, out_q.data_ptr(),
             _ptr(out_k), *ost, status)
     return out_q, out_k
 
@@ -1241,9 +1261,9 @@ def qk_head_norm_rope_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], 
         return qk_head_norm_rope_bwd(dq_out, dk_out, q, k, eps, w_q, w_k, cos, sin, positions,
                                      interleaved, dq, dk, workspace)
     if dq is None:
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        dq = _contiguous_like(q)
     if dk is None and k is not None:
-        dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
+        dk = _contiguous_like(k)
     dw_q = dw_k = None
     if need:
         dw_q = torch.empty(sizes[4], dtype=torch.float32, device=dev)
@@ -1255,7 +1275,7 @@ def qk_head_norm_rope_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], 
     ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if need \
         else (None, 0)
     _launch(idx, "sa_qk_head_norm_rope_bwd", _lib.load().sa_qk_head_norm_rope_bwd, ptrs[0],
-            ptrs[1], *dst, ptrs[2], ptrs[3], *st, *sizes, ptrs[4], ptrs[5], w_dtype, eps, ptrs[6],
+            ptrs[1], *dst, ptrs[2], ptrs[3], *st, *sizes, ptrs[4], ptrs[5], w_dtype, float(eps), ptrs[6],
             ptrs[7], *tab, _ptr(positions), pos64, pst, dq.data_ptr(), _ptr(dk), *ost,
             _ptr(dw_q), _ptr(dw_k), *ws, status)
     return dq, dk, dw_q, dw_k

@@ -344,3 +344,51 @@ def test_from_a_thread_without_a_context():
     assert rcs == [_lib.SA_OK]
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+def test_odd_strides_of_dimensions_of_size_one():
+    q, k, v, dout, mask = make(1, 1, 1, 300, 1.0, 21, layout="bhsd")
+    want = run(q, k, v, dout, mask)
+
+    def odd(t):
+        st = [s if n > 1 else 13 for s, n in zip(t.stride(), t.shape)]
+        return torch.as_strided(t, t.shape, st)
+
+    from sinkattn_b200 import ops
+
+    out, lse = ops.bsattn_fwd(q, k, v, mask)
+    got = ops.bsattn_bwd(odd(dout), odd(q), odd(k), odd(v), odd(out), lse, mask,
+                         dq=odd(torch.empty_like(q)))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
+def test_head_mask_type_past_the_mask_is_reported():
+    from sinkattn_b200 import ops
+
+    q, k, v, dout, mask = make(1, 3, 300, 300, 0.5, 22)
+    mask = mask[:, :2]
+    good = torch.tensor([1, 2, 0], dtype=torch.int32, device="cuda")
+    want = run(q, k, v, dout, mask, hmt=good)
+    out, lse = ops.bsattn_fwd(q, k, v, mask, head_mask_type=good)
+    bad = torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda")
+    got = ops.bsattn_bwd(dout, q, k, v, out, lse, mask, head_mask_type=bad)
+    with pytest.raises(RuntimeError, match="head_mask_type entry"):
+        ops.DeviceStatus.check()
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
+def test_on_a_stream_of_its_own():
+    from sinkattn_b200 import ops
+
+    q, k, v, dout, mask = make(1, 2, 900, 900, 0.5, 23)
+    want = run(q, k, v, dout, mask)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out, lse = ops.bsattn_fwd(q, k, v, mask)
+        got = ops.bsattn_bwd(dout, q, k, v, out, lse, mask)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)

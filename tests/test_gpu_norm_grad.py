@@ -231,11 +231,11 @@ def test_positions_outside_the_table_are_reported_and_nothing_else_changes():
     hit = torch.zeros(2, 8, dtype=torch.bool, device="cuda")
     hit[0, 3] = hit[1, 7] = True
     got = ops.qk_head_norm_rope(a["q"], a["k"], 1e-6, *w, cos, sin, positions=bad)
-    with pytest.raises(RuntimeError, match="outside the rotary tables"):
+    with pytest.raises(RuntimeError, match="position outside the rotary"):
         ops.DeviceStatus.check()
     back = ops.qk_head_norm_rope_bwd(a["dq"], a["dk"], a["q"], a["k"], 1e-6, *w, cos, sin,
                                      positions=bad)
-    with pytest.raises(RuntimeError, match="outside the rotary tables"):
+    with pytest.raises(RuntimeError, match="position outside the rotary"):
         ops.DeviceStatus.check()
     for x, y in zip(got + back[:2], want + good[:2]):
         assert torch.isnan(x[hit]).all() and torch.equal(x[~hit], y[~hit])
@@ -362,6 +362,31 @@ def test_gradients_against_differences():
                for g, n in ((q, "q"), (k, "k"), (dwq, "wq"), (dwk, "wk")))
     # 2^-16 of every term (above); the difference's own error is h^2 of third derivatives
     assert abs(got - want) <= 2.0 ** -16 * size + 1e-6 * size, (got, want, size)
+
+
+def test_odd_strides_of_dimensions_of_size_one():
+    from sinkattn_b200 import ops
+
+    def odd(t):
+        st = [s if n > 1 else 13 for s, n in zip(t.stride(), t.shape)]
+        return torch.as_strided(t, t.shape, st)
+
+    a, w, cos, sin, _ = make(1, 1, 1, 1, 128, 128, torch.bfloat16)
+    want = ops.qk_head_norm_rope(a["q"], a["k"], 1e-6, *w, cos, sin)
+    want += ops.qk_head_norm_rope_bwd(a["dq"], a["dk"], a["q"], a["k"], 1e-6, *w, cos, sin)
+    o = {n: odd(t) for n, t in a.items()}
+    got = ops.qk_head_norm_rope(o["q"], o["k"], 1e-6, *w, odd(cos), odd(sin))
+    got += ops.qk_head_norm_rope_bwd(o["dq"], o["dk"], o["q"], o["k"], 1e-6, *w, odd(cos), odd(sin))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    for B, S in ((1, 1), (3, 1), (1, 5)):
+        g = torch.Generator(device="cuda").manual_seed(B + S)
+        x = [torch.randn(B, S, 256, generator=g, device="cuda").bfloat16() for _ in range(4)]
+        wide = [torch.cat([t, t], dim=-1)[..., 256:] for t in x]
+        want = ops.qk_norm_rope_bwd(*x, 128, 1e-6)
+        for y in ([odd(t) for t in x], wide, [odd(t) for t in wide]):
+            got = ops.qk_norm_rope_bwd(*y, 128, 1e-6)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 def test_refusals():

@@ -152,7 +152,7 @@ def test_bad_index_status_is_told_from_a_timeout(lib):
 
     word = ctypes.c_int32(_lib.SA_DEV_BAD_INDEX)
     assert lib.sa_check_status(ctypes.addressof(word)) == _lib.SA_EINVAL
-    assert "outside the rotary tables" in _lib.last_error() and word.value == 0
+    assert "outside the rotary" in _lib.last_error() and word.value == 0
     word.value = _lib.SA_DEV_WAIT_TIMEOUT
     assert lib.sa_check_status(ctypes.addressof(word)) == _lib.SA_ETIMEOUT and word.value == 0
     assert lib.sa_check_status(ctypes.addressof(word)) == _lib.SA_OK
