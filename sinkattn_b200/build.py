@@ -3,8 +3,9 @@
 Usage: python -m sinkattn_b200.build [--verbose] [--force]
 
 Each csrc/*.cu file is compiled to an object under sinkattn_b200/_build/ and
-linked into sinkattn_b200/libsinkattn.so. The build is incremental on file
-modification times (sources and headers) and needs no GPU.
+linked into sinkattn_b200/libsinkattn.so; csrc/fast.cpp becomes the extension
+module sinkattn_b200/_fast.so, against the installed torch. The build is
+incremental on file modification times (sources and headers) and needs no GPU.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libsinkattn.so"
+FAST = PKG / "_fast.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = [
@@ -60,6 +62,39 @@ def _compile(nvcc: str, src: Path, obj: Path, extra: list[str], verbose: bool) -
         print(res.stdout + res.stderr, flush=True)
 
 
+def build_fast(verbose: bool = False, force: bool = False) -> Path:
+    """Compile the extension module that shortens the Python calls."""
+    import sysconfig
+
+    import torch
+
+    src = CSRC / "fast.cpp"
+    stamp = BUILD / "fast.txt"
+    made_for = f"{torch.__version__} {sys.version}"
+    newest = max(src.stat().st_mtime, max(p.stat().st_mtime for p in INCLUDE.glob("*.h")))
+    if not force and FAST.exists() and FAST.stat().st_mtime >= newest and stamp.exists() \
+            and stamp.read_text() == made_for:
+        return FAST
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    tmp = FAST.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", str(src), "-o", str(tmp),
+           f"-L{root}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+           "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compiling {src.name} failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, FAST)
+    stamp.write_text(made_for)
+    return FAST
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
     """Compile every CUDA source and link the shared library; returns its path."""
     nvcc = find_nvcc()
@@ -92,6 +127,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    build_fast(verbose, force)
     return LIB
 
 

@@ -160,18 +160,25 @@ __global__ void __launch_bounds__(256)
       if ((threadIdx.x & 31) == 0) counts[t] = c;
     }
   }
-  const int bh = blockIdx.y;
+  const int bh = blockIdx.x;
   const int h = bh % H, b = bh / H;
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int r0 = blockIdx.x * (16 * kPrepRows) + g;
+  const int r0 = blockIdx.y * (16 * kPrepRows) + g;
   uint4 x[kPrepRows], y[kPrepRows];
+  float row_lse[kPrepRows], row_dlse[kPrepRows];
 #pragma unroll
   for (int i = 0; i < kPrepRows; ++i) {
     const int r = r0 + 16 * i;
     x[i] = y[i] = make_uint4(0, 0, 0, 0);
+    row_lse[i] = -INFINITY;
+    row_dlse[i] = 0.f;
     if (r < Sq) {
+      if (l == 0) {
+        row_lse[i] = lse[(int64_t)bh * Sq + r];
+        if (dlse != nullptr) row_dlse[i] = dlse[(int64_t)bh * Sq + r];
+      }
       x[i] = __ldg(reinterpret_cast<const uint4*>(dout + b * ds0 + h * ds1 + (int64_t)r * ds2) + l);
-      y[i] = __ldg(reinterpret_cast<const uint4*>(out + b * os0 + h * os1 + (int64_t)r * os2) + l);
+      y[i] = __ldcs(reinterpret_cast<const uint4*>(out + b * os0 + h * os1 + (int64_t)r * os2) + l);
     }
   }
 #pragma unroll
@@ -189,13 +196,9 @@ __global__ void __launch_bounds__(256)
     for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (l == 0 && r < rows_pad) {
       float nl = -INFINITY, nd = 0.f;
-      if (r < Sq) {
-        const int64_t i0 = (int64_t)bh * Sq + r;
-        const float v = lse[i0];
-        if (v != -INFINITY) {
-          nl = -v * 1.4426950408889634f;
-          nd = (dlse != nullptr ? dlse[i0] : 0.f) - s;
-        }
+      if (row_lse[i] != -INFINITY) {
+        nl = -row_lse[i] * 1.4426950408889634f;
+        nd = row_dlse[i] - s;
       }
       const int64_t o0 = (int64_t)bh * rows_pad + r;
       nstat[o0] = nl;
@@ -1047,7 +1050,9 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes)) !=
       SA_OK)
     return rc;
-  const dim3 pg((unsigned)((nq * kT + 16 * kPrepRows - 1) / (16 * kPrepRows)), (unsigned)(B * H));
+  // heads run fastest: with the heads of a token side by side in memory, blocks
+  // that run together then read it in order
+  const dim3 pg((unsigned)(B * H), (unsigned)((nq * kT + 16 * kPrepRows - 1) / (16 * kPrepRows)));
   row_stats_kernel<<<pg, 256, 0, stream>>>(
       static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
       do_strides[0], do_strides[1], do_strides[2], o_strides[0], o_strides[1], o_strides[2], lse,

@@ -14,6 +14,11 @@ import torch
 
 from . import _lib
 
+try:  # the short way into the library for calls that need nothing laid out
+    from . import _fast
+except ImportError:  # not built for this torch: every call goes the long way
+    _fast = None
+
 BLOCK = 128
 
 
@@ -56,23 +61,6 @@ def _as_kernel_layout(t: torch.Tensor) -> torch.Tensor:
     return t if _bf16_view_ok(t) else t.contiguous()
 
 
-# Checks and ctypes arguments that follow from the tensors' metadata alone
-# (shapes, strides, types, devices) are worked out once per combination and
-# kept: what a call still does is pointers, alignment, buffers and the launch.
-_PLANS: dict = {}
-
-
-def _remember(key, plan):
-    if len(_PLANS) >= 4096:
-        _PLANS.clear()
-    _PLANS[key] = plan
-    return plan
-
-
-def _meta(t: Optional[torch.Tensor]):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
-
-
 def _strides16_ok(t: torch.Tensor) -> bool:
     """Whole 16-byte vectors along the last dimension, and from element to
     element of the others (a dimension of size 1 is never stepped along)."""
@@ -102,19 +90,34 @@ def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda idx: torch.cuda.current_stream(idx).cuda_stream)
-
-
 def _launch(idx: int, name: str, fn, *args) -> None:
     """Calls an entry point whose last argument is the stream, on device idx."""
-    if torch.cuda.current_device() == idx:
-        rc = fn(*args, _raw_stream(idx))
-    else:
-        with torch.cuda.device(idx):
-            rc = fn(*args, _raw_stream(idx))
-    if rc != _lib.SA_OK:
-        _lib.check(rc, name)
+    with torch.cuda.device(idx):
+        rc = fn(*args, _stream(torch.device("cuda", idx)))
+    _lib.check(rc, name)
+
+
+_FAST_NAMES = ("sa_bsattn_bwd", "sa_bsattn_bwd_workspace_size", "sa_qk_norm_rope_bwd",
+               "sa_qk_norm_rope_bwd_workspace_size", "sa_qk_head_norm_rope",
+               "sa_qk_head_norm_rope_bwd", "sa_qk_head_norm_rope_bwd_workspace_size")
+
+
+def _open_fast(idx: int, status: int) -> None:
+    """Lets device idx's calls go the short way: the loaded library's addresses
+    and the device's status word."""
+    if _fast is not None:
+        lib = _lib.load()
+        _fast.bind(*(_lib.ctypes.cast(getattr(lib, n), _lib.ctypes.c_void_p).value
+                     for n in _FAST_NAMES))
+        _fast.set_status(idx, status)
+
+
+def _short(name: str, *args):
+    """The results of a call that went the short way, else None."""
+    got = getattr(_fast, name)(*args) if _fast is not None else None
+    if type(got) is int:
+        _lib.check(got, "sa_" + name)
+    return got
 
 
 class DeviceStatus:
@@ -140,6 +143,7 @@ class DeviceStatus:
                        "sa_status_device_pointer")
             w = (int(host), int(dev_ptr.value))
             cls._words[idx] = w
+            _open_fast(idx, w[1])
         return w
 
     @staticmethod
@@ -275,11 +279,12 @@ def bsattn_bwd(
     sa_bsattn_bwd_workspace_size bytes) may hold anything; calls sharing one
     must not overlap on the GPU.
     """
-    key = ("bsattn_bwd", _meta(dout), _meta(q), _meta(k), _meta(v), _meta(out), _meta(lse),
-           _meta(block_mask), softmax_scale, _meta(head_mask_type), _meta(dlse), _meta(dq),
-           _meta(dk), _meta(dv))
-    plan = _PLANS.get(key) or _remember(key, _bsattn_bwd_plan(
-        dout, q, k, v, out, lse, block_mask, softmax_scale, head_mask_type, dlse, dq, dk, dv))
+    got = _short("bsattn_bwd", dout, q, k, v, out, lse, block_mask, softmax_scale, head_mask_type,
+                 dlse, dq, dk, dv, workspace)
+    if got is not None:
+        return got
+    plan = _bsattn_bwd_plan(dout, q, k, v, out, lse, block_mask, softmax_scale, head_mask_type,
+                            dlse, dq, dk, dv)
     idx, dev, fits, in_strides, middle, grads, out_strides, need, status = plan
     ins = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
     if not fits or (ins[0] | ins[1] | ins[2] | ins[3] | ins[4]) & 15:
@@ -1004,10 +1009,11 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
     without weights). Equal calls give equal bits. Calls sharing a `workspace`
     (uint8, sa_qk_norm_rope_bwd_workspace_size bytes) must not overlap.
     """
-    key = ("qk_norm_rope_bwd", _meta(dq_out), _meta(dk_out), _meta(q), _meta(k), head_dim,
-           _meta(w_q), _meta(w_k), _meta(cos), _meta(sin), _meta(dq), _meta(dk))
-    plan = _PLANS.get(key) or _remember(key, _qk_norm_rope_bwd_plan(
-        dq_out, dk_out, q, k, head_dim, w_q, w_k, cos, sin, dq, dk))
+    got = _short("qk_norm_rope_bwd", dq_out, dk_out, q, k, head_dim, eps, w_q, w_k, cos, sin, dq,
+                 dk, workspace)
+    if got is not None:
+        return got
+    plan = _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, w_q, w_k, cos, sin, dq, dk)
     idx, dev, fits, in_rows, sizes, w_bf16, fs, out_rows, need, status = plan
     ptrs = [_ptr(t) for t in (dq_out, dk_out, q, k, w_q, w_k, cos, sin)]
     if not fits or any(x is not None and x & 15 for x in ptrs):
@@ -1098,8 +1104,7 @@ _DTYPES = {torch.bfloat16: _lib.SA_DTYPE_BF16, torch.float16: _lib.SA_DTYPE_FP16
 
 
 def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, outs):
-    """What qk_head_norm_rope and its gradient derive from their tensors'
-    metadata. more: further (name, tensor, like) inputs; outs: the same of
+    """What qk_head_norm_rope and its gradient derive from their tensors. more: further (name, tensor, like) inputs; outs: the same of
     outputs, None for one to be allocated."""
     dev = _require_cuda(q, k, w_q, w_k, cos, sin, positions, *(t for _, t, _ in more + outs))
     if q.dim() != 4 or (k is not None and k.dim() != 4):
@@ -1211,11 +1216,11 @@ def qk_head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], eps: float,
     the input type; out_q/out_k may alias q/k or be views of a larger buffer.
     """
     fn = "qk_head_norm_rope"
-    key = (fn, _meta(q), _meta(k), _meta(w_q), _meta(w_k), _meta(cos), _meta(sin),
-           _meta(positions), interleaved, _meta(out_q), _meta(out_k))
-    plan = _PLANS.get(key) or _remember(key, _head_norm_plan(
-        fn, q, k, w_q, w_k, cos, sin, positions, interleaved, [],
-        [("out_q", out_q, q), ("out_k", out_k, k)]))
+    got = _short(fn, q, k, eps, w_q, w_k, cos, sin, positions, interleaved, out_q, out_k)
+    if got is not None:
+        return got
+    plan = _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, [],
+                           [("out_q", out_q, q), ("out_k", out_k, k)])
     idx, dev, fits, st, _, ost, sizes, w_dtype, tab, pos64, pst, _, status = plan
     pq, pk, pwq, pwk, pc, ps = (_ptr(t) for t in (q, k, w_q, w_k, cos, sin))
     if not fits or (pq | (pk or 0) | (pwq or 0) | (pwk or 0) | (pc or 0) | (ps or 0)) & 15:
@@ -1248,11 +1253,13 @@ def qk_head_norm_rope_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], 
     (uint8, sa_qk_head_norm_rope_bwd_workspace_size bytes) must not overlap.
     """
     fn = "qk_head_norm_rope_bwd"
-    key = (fn, _meta(dq_out), _meta(dk_out), _meta(q), _meta(k), _meta(w_q), _meta(w_k),
-           _meta(cos), _meta(sin), _meta(positions), interleaved, _meta(dq), _meta(dk))
-    plan = _PLANS.get(key) or _remember(key, _head_norm_plan(
-        fn, q, k, w_q, w_k, cos, sin, positions, interleaved,
-        [("dq_out", dq_out, q), ("dk_out", dk_out, k)], [("dq", dq, q), ("dk", dk, k)]))
+    got = _short(fn, q, k, eps, w_q, w_k, cos, sin, positions, interleaved, dq_out, dk_out, dq,
+                 dk, workspace)
+    if got is not None:
+        return got
+    plan = _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved,
+                           [("dq_out", dq_out, q), ("dk_out", dk_out, k)],
+                           [("dq", dq, q), ("dk", dk, k)])
     idx, dev, fits, st, dst, ost, sizes, w_dtype, tab, pos64, pst, need, status = plan
     ptrs = [_ptr(t) for t in (dq_out, dk_out, q, k, w_q, w_k, cos, sin)]
     if not fits or any(x is not None and x & 15 for x in ptrs):

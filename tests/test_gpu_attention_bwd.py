@@ -392,3 +392,32 @@ def test_on_a_stream_of_its_own():
     torch.cuda.current_stream().wait_stream(side)
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+def test_the_short_way_is_taken_and_agrees_with_the_long_one(monkeypatch):
+    from sinkattn_b200 import ops
+
+    assert ops._fast is not None, "the extension module is not built"
+    q, k, v, dout, mask = make(2, 3, 500, 400, 0.5, 24)
+    hmt = torch.tensor([1, 0, 3], dtype=torch.int32, device="cuda")
+    dlse = torch.randn(2, 3, 500, device="cuda")
+    out, lse = ops.bsattn_fwd(q, k, v, mask, head_mask_type=hmt)
+    args = (dout, q, k, v, out, lse, mask)
+    ops.DeviceStatus.pointer(q.device)
+    taken = []
+    real = ops._short
+
+    def spy(name, *a):
+        got = real(name, *a)
+        taken.append(got is not None)
+        return got
+
+    monkeypatch.setattr(ops, "_short", spy)
+    kws = (dict(), dict(head_mask_type=hmt, dlse=dlse, softmax_scale=0.1),
+           dict(dq=torch.empty_like(q), dk=torch.empty_like(k), dv=torch.empty_like(v)))
+    fast = [ops.bsattn_bwd(*args, **kw) for kw in kws]
+    assert taken == [True] * 3
+    monkeypatch.setattr(ops, "_short", lambda *a: None)
+    for kw, want in zip(kws, fast):
+        for x, y in zip(ops.bsattn_bwd(*args, **kw), want):
+            assert torch.equal(x, y) and x.stride() == y.stride()

@@ -437,3 +437,45 @@ def test_refusals():
                                                                .transpose(0, 1)))):
         with pytest.raises(exc, match=match):
             ops.qk_norm_rope_bwd(**{**h, **kw})
+
+
+def test_the_short_way_is_taken_and_agrees_with_the_long_one(monkeypatch):
+    from sinkattn_b200 import ops
+
+    assert ops._fast is not None, "the extension module is not built"
+    a, w, cos, sin, pos = make(2, 40, 6, 3, 128, 128, torch.bfloat16, T=99)
+    ops.DeviceStatus.pointer(cos.device)
+    x = [torch.randn(2, 40, 768, device="cuda").bfloat16() for _ in range(4)]
+    wh = torch.randn(768, device="cuda")
+    th = [t[:40].contiguous() for t in (cos, sin)]
+    packed = torch.cat([a["q"].flatten(2), a["k"].flatten(2)], dim=-1)
+    pq, pk = packed[..., :768].unflatten(2, (6, 128)), packed[..., 768:].unflatten(2, (3, 128))
+    calls = [
+        lambda: ops.qk_head_norm_rope(a["q"], a["k"], 1e-6, *w, cos, sin, positions=pos),
+        lambda: ops.qk_head_norm_rope(pq, pk, 1e-6, *w, cos, sin, positions=pos[0].int()),
+        lambda: ops.qk_head_norm_rope(a["q"], None, 1e-6, w[0], None, cos, sin, interleaved=False),
+        lambda: ops.qk_head_norm_rope(a["q"].float(), a["k"].float(), 1e-6),
+        lambda: ops.qk_head_norm_rope_bwd(a["dq"], a["dk"], a["q"], a["k"], 1e-6, *w, cos, sin,
+                                          positions=pos),
+        lambda: ops.qk_head_norm_rope_bwd(a["dq"], None, pq, None, 1e-6, w[0].float(), None),
+        lambda: ops.qk_norm_rope_bwd(*x, 128, 1e-6, wh, wh, *th),
+        lambda: ops.qk_norm_rope_bwd(*x, 128, 1e-6, wh.bfloat16(), wh.bfloat16()),
+        lambda: ops.qk_norm_rope_bwd(*x, 128, 1e-6, dq=torch.empty_like(x[0])),
+    ]
+    taken = []
+    real = ops._short
+
+    def spy(name, *args):
+        got = real(name, *args)
+        taken.append(got is not None)
+        return got
+
+    monkeypatch.setattr(ops, "_short", spy)
+    fast = [c() for c in calls]
+    assert taken == [True] * len(calls)
+    monkeypatch.setattr(ops, "_short", lambda *args: None)
+    for c, want in zip(calls, fast):
+        got = c()
+        assert len(got) == len(want)
+        for p, q in zip(got, want):
+            assert (p is None and q is None) or (torch.equal(p, q) and p.stride() == q.stride())
