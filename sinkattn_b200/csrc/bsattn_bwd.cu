@@ -41,6 +41,7 @@ constexpr int kBoxBytes = kTileBytes / 2;      // one 64-column box
 constexpr int kStatBytes = 2 * kT * 4;         // -lse (log2 units) and -delta of 128 rows
 constexpr int kMaxBlocks = 1024;               // per mask row or column (S <= 131072)
 constexpr int kLeastPiece = 8;                 // blocks
+constexpr int kJoin = 8;                       // pieces added up at a time
 constexpr int kListReaders = 2 + kWorkers;
 constexpr uint32_t kColX = 0, kColY = 128, kColAcc1 = 256, kColAcc2 = 384;
 
@@ -77,22 +78,33 @@ struct Params {
   int64_t dqs0, dqs1, dqs2, dks0, dks1, dks2, dvs0, dvs1, dvs2;
   int* next_item;
   int32_t* status;
-  // Work items: a tile of `count` kept blocks is cut into clamp(count / least,
-  // 1, chunks) pieces, least from the total count. Pieces 1, 2, ... of the cut
-  // tiles are dealt out to the CTAs first, then every tile's piece 0 is taken
-  // from a counter, kind 0 before kind 1.
-  int tiles[2], chunks[2];
-  const int* counts[2];  // kept blocks of every tile; NULL where chunks = 1
-  int* joined[2];        // [tile][worker warp] pieces stored so far
-  float* part[2];        // [tile][chunk] fp32 sums of a piece
+  // Work items: where tiles may be cut, one of `count` kept blocks is cut into
+  // max(1, count / least) pieces, least from the total count. Pieces 1, 2, ...
+  // of the cut tiles are dealt out to the CTAs first, then every tile's piece 0
+  // is taken from a counter, kind 0 before kind 1.
+  int tiles[2];
+  const int* counts[2];  // kept blocks of every tile; NULL where none is cut
+  const int* eights;     // the same of every eight tiles: sum * 2048 + largest; by kind
+  // Pieces are numbered over all cut tiles of a kind. A piece has at least
+  // 1 / SMs of the kind's blocks, so there are max_extra <= SMs of the pieces
+  // 1, 2, ...; with f of them before the tile's, its piece i > 0 is kept in slot
+  // f + i - 1, its piece 0 in slot max_extra + f.
+  int max_extra;
+  float* part[2];  // [slot] fp32 sums of a piece
+  int* joined[2];  // [slot][worker warp] arrivals of pieces or of groups of them
 };
 
 // A work item as the list warp publishes it: a tile, or a piece of one.
 struct __align__(16) Item {
   int n;        // kept blocks; -1: no more items
   int kind, blk, h, b;
-  int tile;     // of its kind
-  int pieces, piece;
+  int pieces, piece, first;  // first: slot of piece 1
+  // The tile of acc 0 (dV) and 1 (dK or dQ): first row, row pitch, and the rows
+  // that exist. Looked up ahead of the epilogue, where first reads of these
+  // parameters took 2 us of a launch.
+  __nv_bfloat16* out[2];
+  int64_t pitch[2];
+  int rows;
 };
 
 struct __align__(16) SmemCtl {
@@ -132,8 +144,8 @@ __global__ void __launch_bounds__(256)
                      int64_t ds0, int64_t ds1, int64_t ds2, int64_t os0, int64_t os1, int64_t os2,
                      const float* __restrict__ lse, const float* __restrict__ dlse, int H, int Sq,
                      int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_item,
-                     int* joined, int n_joined, int* counts0, int* counts1, const Mask mask, int B,
-                     int nk, int32_t* status) {
+                     int* joined, int n_joined, int* counts0, int* counts1, int* eights,
+                     const Mask mask, int B, int nk, int32_t* status) {
   release_next_kernel();  // it waits for this one's completion all the same
   const int nq = rows_pad / kT;
   const int block = blockIdx.y * gridDim.x + blockIdx.x, blocks = gridDim.x * gridDim.y;
@@ -142,23 +154,42 @@ __global__ void __launch_bounds__(256)
     for (int i = threadIdx.x; i < H; i += 256)
       if (mask.head_mask_type[i] > mask.heads) report_status(status, SA_DEV_BAD_INDEX);
   for (int i = block * 256 + threadIdx.x; i < n_joined; i += blocks * 256) joined[i] = 0;
-  // kept blocks of every tile of the kinds that may be cut, a warp per tile
+  // kept blocks of every tile of the kinds that may be cut, a warp per tile, and
+  // of eight tiles together, as one number: sum * 2048 + largest
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int of_warp[8];
   for (int kind = 0; kind < 2; ++kind) {
     int* counts = kind ? counts1 : counts0;
     if (counts == nullptr) continue;
-    const int per_head = kind ? nq : nk, n = kind ? nk : nq;
-    for (int t = block * 8 + (threadIdx.x >> 5); t < B * H * per_head; t += blocks * 8) {
-      const int bh = t / per_head;
+    const int per_head = kind ? nq : nk, n = kind ? nk : nq, tiles = B * H * per_head;
+    for (int e = block; e * 8 < tiles; e += blocks) {
+      const int t = e * 8 + warp, bh = t / per_head;
       const uint8_t* m;
       int64_t step;
-      int c = n;
-      if (!mask.line(kind, bh / H, bh % H, t - bh * per_head, m, step)) {
-        c = 0;
-        for (int i = threadIdx.x & 31; i < n; i += 32) c += m[i * step] != 0;
-        c = __reduce_add_sync(0xffffffffu, c);
+      int c = 0;
+      if (t < tiles) {
+        c = n;
+        if (!mask.line(kind, bh / H, bh % H, t - bh * per_head, m, step)) {
+          c = 0;
+#pragma unroll 8
+          for (int i = lane; i < n; i += 32) c += m[i * step] != 0;
+          c = __reduce_add_sync(0xffffffffu, c);
+        }
+        if (lane == 0) counts[t] = c;
       }
-      if ((threadIdx.x & 31) == 0) counts[t] = c;
+      if (lane == 0) of_warp[warp] = c;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int sum = 0, most = 0;
+        for (int w = 0; w < 8; ++w) {
+          sum += of_warp[w];
+          most = max(most, of_warp[w]);
+        }
+        eights[e] = sum * 2048 + most;
+      }
+      __syncthreads();
     }
+    eights += (tiles + 7) / 8;
   }
   const int bh = blockIdx.x;
   const int h = bh % H, b = bh / H;
@@ -269,19 +300,14 @@ __device__ __forceinline__ void keep_part(const uint32_t (&o)[kCols], float* dst
            make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]));
 }
 
-__device__ __forceinline__ void sum_parts(const float* src, int pieces, int64_t size,
-                                          uint32_t (&o)[kCols], int lane) {
+__device__ __forceinline__ void add_part(uint32_t (&o)[kCols], const float* src, int lane) {
 #pragma unroll
-  for (int v = 0; v < kCols; ++v) o[v] = 0u;
-  for (int i = 0; i < pieces; ++i) {
+  for (int v = 0; v < kCols / 4; ++v) {
+    const uint4 x = __ldcg(reinterpret_cast<const uint4*>(src) + v * 32 + lane);
+    const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int v = 0; v < kCols / 4; ++v) {
-      const uint4 x = __ldcg(reinterpret_cast<const uint4*>(src + i * size) + v * 32 + lane);
-      const uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        o[4 * v + u] = __float_as_uint(__uint_as_float(o[4 * v + u]) + __uint_as_float(y[u]));
-    }
+    for (int u = 0; u < 4; ++u)
+      o[4 * v + u] = __float_as_uint(__uint_as_float(o[4 * v + u]) + __uint_as_float(y[u]));
   }
 }
 
@@ -301,7 +327,9 @@ __device__ __forceinline__ void split_bf16x2(float x0, float x1, uint32_t& hi, u
 // halves, each a product of its own in the columns that X and Y leave free.
 // The launch takes it where the blocks do not fill the GPU once and the extra
 // products hide behind latencies (300 tokens, 2 heads: 12.1 us become 13.0).
-template <bool FINE>
+// CUT: tiles may be cut into pieces. Without that code a launch of a few tiles is
+// 2 us shorter (300 tokens, 2 heads, cold caches: 19.3 and 17.4 us).
+template <bool FINE, bool CUT>
 __global__ void __launch_bounds__(kThreads, 1)
     bsattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                       const __grid_constant__ CUtensorMap tm_k,
@@ -362,23 +390,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 2) {
     // ---------------- work items and their kept blocks, two ahead ----------------
     int least = 0x7fffffff, extra[2] = {0, 0}, before_lane[2] = {0, 0}, span[2] = {1, 1};
-    auto pieces_of = [&](int kind, int count) {
-      return max(1, min(p.chunks[kind], count / least));
-    };
-    if (p.counts[0] != nullptr || p.counts[1] != nullptr) {
+    const auto extras_of = [&](int count) { return max(1, count / least) - 1; };
+    if (CUT) {
       // pieces of about half an SM's share of the blocks of both kinds, 8 at least
-      const int known = p.counts[0] != nullptr ? 0 : 1;  // the total is alike for both
-      int total = 0;
-      for (int i = lane; i < p.tiles[known]; i += 32) total += p.counts[known][i];
+      const int n0 = p.counts[0] != nullptr ? (p.tiles[0] + 7) / 8 : 0;
+      const int n = n0 + (p.counts[1] != nullptr ? (p.tiles[1] + 7) / 8 : 0);
+      int most[2] = {0, 0}, total = 0;
+#pragma unroll 6
+      for (int i = lane * 4; i < n; i += 128) {
+        const int4 x = *reinterpret_cast<const int4*>(p.eights + i);
+        const int y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = i + e < n ? y[e] : 0;
+          total += c >> 11;
+          if (i + e < n0) most[0] = max(most[0], c & 2047);
+          else most[1] = max(most[1], c & 2047);
+        }
+      }
       total = __reduce_add_sync(0xffffffffu, total);
+      if (n0 > 0 && n > n0) total >>= 1;  // of one kind: both have the same
+      most[0] = __reduce_max_sync(0xffffffffu, most[0]);
+      most[1] = __reduce_max_sync(0xffffffffu, most[1]);
       least = max(kLeastPiece, (total + (int)gridDim.x - 1) / (int)gridDim.x);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        if (p.counts[q] == nullptr) continue;
+        if (most[q] < 2 * least) continue;
         span[q] = (p.tiles[q] + 31) >> 5;  // consecutive tiles of a lane
         int own = 0;
         for (int i = lane * span[q]; i < min(p.tiles[q], (lane + 1) * span[q]); ++i)
-          own += pieces_of(q, p.counts[q][i]) - 1;
+          own += extras_of(p.counts[q][i]);
         int sum = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -399,7 +440,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       w.n = -1;
       uint32_t word = 0;  // lane i: blocks 32 i .. 32 i + 31
       w.kind = -1;
-      if (dealt < extra[0] + extra[1]) {
+      int tile = 0;
+      w.piece = w.first = 0;
+      if (CUT && dealt < extra[0] + extra[1]) {
         // which tile the dealt-out piece belongs to: first the lane, then the
         // tile among that lane's
         w.kind = dealt >= extra[0] ? 1 : 0;
@@ -407,13 +450,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int before = w.kind ? before_lane[1] : before_lane[0];
         const int* counts = w.kind ? p.counts[1] : p.counts[0];
         const int owner = 31 - __clz(__ballot_sync(0xffffffffu, before <= r));
-        int left = r - __shfl_sync(0xffffffffu, before, owner);
-        for (w.tile = owner * (w.kind ? span[1] : span[0]);; ++w.tile) {
-          const int more = pieces_of(w.kind, counts[w.tile]) - 1;
-          if (left < more) break;
-          left -= more;
+        int first = __shfl_sync(0xffffffffu, before, owner);
+        for (int t = owner * (w.kind ? span[1] : span[0]);; t += 32) {
+          const int more = t + lane < p.tiles[w.kind] ? extras_of(counts[t + lane]) : 0;
+          int sum = more;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+          }
+          const uint32_t past = __ballot_sync(0xffffffffu, r < first + sum);
+          if (past != 0u) {
+            const int i = __ffs(past) - 1;
+            tile = t + i;
+            first += __shfl_sync(0xffffffffu, sum - more, i);
+            break;
+          }
+          first += __shfl_sync(0xffffffffu, sum, 31);
         }
-        w.piece = 1 + left;
+        w.piece = 1 + r - first;
+        w.first = first;
         dealt += gridDim.x;
       } else {
         int it = 0;
@@ -421,15 +477,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         it = __shfl_sync(0xffffffffu, it, 0);
         if (it < p.tiles[0] + p.tiles[1]) {
           w.kind = it >= p.tiles[0] ? 1 : 0;
-          w.tile = it - (w.kind ? p.tiles[0] : 0);
-          w.piece = 0;
+          tile = it - (w.kind ? p.tiles[0] : 0);
+          const int* counts = w.kind ? p.counts[1] : p.counts[0];
+          if (CUT && (w.kind ? extra[1] : extra[0]) > 0 && counts[tile] >= 2 * least) {
+            const int width = w.kind ? span[1] : span[0], owner = tile / width;
+            int sum = 0;
+            for (int i = owner * width + lane; i < tile; i += 32) sum += extras_of(counts[i]);
+            w.first = __shfl_sync(0xffffffffu, w.kind ? before_lane[1] : before_lane[0], owner) +
+                      __reduce_add_sync(0xffffffffu, sum);
+          }
         }
       }
       if (w.kind >= 0) {
         const int kind = w.kind;
         const int per_head = kind ? p.nq : p.nk;
-        const int bh = w.tile / per_head;
-        w.blk = w.tile - bh * per_head;
+        const int bh = tile / per_head;
+        w.blk = tile - bh * per_head;
         w.b = bh / p.H;
         w.h = bh - w.b * p.H;
         const uint8_t* m = nullptr;
@@ -456,10 +519,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           count += __popc(bal);
         }
-        w.pieces = pieces_of(kind, count);
-        if (w.pieces > 1) {
+        w.pieces = 1;
+        if (CUT && (kind ? extra[1] : extra[0]) > 0) w.pieces += extras_of(count);
+        if (CUT && w.pieces > 1) {
           // this piece: the kept blocks number lo .. hi-1 of the tile
-          const int lo = w.piece * count / w.pieces, hi = (w.piece + 1) * count / w.pieces;
+          const int lo = (int)((int64_t)w.piece * count / w.pieces);
+          const int hi = (int)((int64_t)(w.piece + 1) * count / w.pieces);
           uint32_t rest = word;
           word = 0;
           for (int r = before; rest != 0u && r < hi; ++r) {
@@ -470,6 +535,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           count = hi - lo;
         }
         w.n = count;
+        const int64_t row = (int64_t)w.blk * kT;
+        w.rows = (kind ? p.Sq : p.Sk) - (int)row;
+        w.pitch[0] = p.dvs2;
+        w.pitch[1] = kind ? p.dqs2 : p.dks2;
+        w.out[0] = p.dv + w.b * p.dvs0 + w.h * p.dvs1 + row * p.dvs2;
+        w.out[1] = (kind ? p.dq + w.b * p.dqs0 + w.h * p.dqs1 : p.dk + w.b * p.dks0 + w.h * p.dks1) +
+                   row * w.pitch[1];
       }
       ctl->kept[slot][lane] = word;
       __syncwarp();
@@ -702,38 +774,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 0; ok; ++k) {
       const int slot = k & 1;
       if (!wait(&ctl->list_full[slot], (uint32_t)(k >> 1) & 1u)) break;
-      const Item tl = ctl->item[slot];
-      const int n = tl.n;
+      const int n = ctl->item[slot].n, kind = ctl->item[slot].kind;
       if (n < 0) break;
-      // this warp's first output row and column, and how many rows exist
-      const int wrow = tl.blk * kT + (warp & 3) * 32;
-      const int rows = (tl.kind ? p.Sq : p.Sk) - wrow;
-      __nv_bfloat16 *o1 = nullptr, *o2;
-      int64_t pitch1 = 0, pitch2;
-      if (tl.kind) {
-        pitch2 = p.dqs2;
-        o2 = p.dq + tl.b * p.dqs0 + tl.h * p.dqs1 + wrow * pitch2 + g * kCols;
-      } else {
-        pitch1 = p.dvs2;
-        pitch2 = p.dks2;
-        o1 = p.dv + tl.b * p.dvs0 + tl.h * p.dvs1 + wrow * pitch1 + g * kCols;
-        o2 = p.dk + tl.b * p.dks0 + tl.h * p.dks1 + wrow * pitch2 + g * kCols;
-      }
+      // this warp's part of an output
+      const auto output = [&](int acc, auto&& write) {
+        const Item& t = ctl->item[slot];
+        const int r = (warp & 3) * 32;
+        write(t.out[acc] + r * t.pitch[acc] + g * kCols, t.pitch[acc], t.rows - r);
+      };
+      const auto store = [&](int acc, const uint32_t(&o)[kCols]) {
+        output(acc, [&](__nv_bfloat16* to, int64_t pitch, int rows) {
+          store_rows(o, acc ? p.scale : 1.0f, to, pitch, rows, lane);
+        });
+      };
       if (n == 0) {
-        if (!tl.kind) zero_rows(o1, pitch1, rows, lane);
-        zero_rows(o2, pitch2, rows, lane);
+        for (int acc = kind; acc < 2; ++acc)
+          output(acc, [&](__nv_bfloat16* to, int64_t pitch, int rows) {
+            zero_rows(to, pitch, rows, lane);
+          });
         mbar_arrive(&ctl->list_empty[slot]);
         continue;
       }
       // the last key block of a ragged length, if it is kept
-      const bool ragged = tl.kind && (p.Sk % kT) != 0 &&
+      const bool ragged = kind && (p.Sk % kT) != 0 &&
                           ((ctl->kept[slot][(p.nk - 1) >> 5] >> ((p.nk - 1) & 31)) & 1u);
       uint64_t row_nl2 = 0ull, row_nd2 = 0ull;  // kind 1: this row's statistics
       for (int j = 0; j < n; ++j) {
         const uint32_t jp = (uint32_t)(J + j);
         uint64_t pr[kCols / 2];  // the probabilities, in pairs
         if (!wait(&ctl->st_full[jp & 1u], (jp >> 1) & 1u)) break;
-        if (tl.kind == 0) {
+        if (!kind) {
           const float* st = ctl->stats[jp & 1u];
           if (!wait(&ctl->x_full[jp & 1u], (jp >> 1) & 1u)) break;
           tc_fence_after();
@@ -852,49 +922,64 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (!wait(&ctl->acc_full, (uint32_t)e & 1u)) break;
       tc_fence_after();
-      const int pieces = tl.pieces;
       uint32_t o[kCols];
-      if (pieces == 1) {
-        if (!tl.kind) {
-          load_acc(t_self + kColAcc1, o);
-          store_rows(o, 1.0f, o1, pitch1, rows, lane);
-        }
-        load_acc(t_self + kColAcc2, o);
-        tc_fence_before();
-        mbar_arrive(&ctl->acc_free);
-        store_rows(o, p.scale, o2, pitch2, rows, lane);
-      } else {
-        // Every warp stores its part of the piece's sums; the warp that stores
-        // the tile's last piece adds them all up in piece order, so the result
-        // does not depend on which one that is.
-        const int kind = tl.kind;
-        const int local = tl.tile;
-        const int64_t size = (kind ? 1 : 2) * kT * kT;
-        float* first =
-            p.part[kind] + (int64_t)local * p.chunks[kind] * size + (warp - 4) * 32 * kCols;
-        float* mine = first + tl.piece * size;
+      const Item& tl = ctl->item[slot];
+      if (!CUT || tl.pieces == 1) {
         if (!kind) {
           load_acc(t_self + kColAcc1, o);
-          keep_part(o, mine, lane);
+          store(0, o);
         }
         load_acc(t_self + kColAcc2, o);
         tc_fence_before();
         mbar_arrive(&ctl->acc_free);
-        keep_part(o, mine + size - kT * kT, lane);
-        __threadfence();
-        __syncwarp();
-        int done = 0;
-        if (lane == 0)
-          done = atomicAdd(p.joined[kind] + local * (kWorkers / 32) + (warp - 4), 1) + 1;
-        done = __shfl_sync(0xffffffffu, done, 0);
-        if (done == pieces) {
+        store(1, o);
+      } else {
+        // Every warp stores its part of the piece's sums. The warp that stores
+        // the last of a group of kJoin pieces adds them up in piece order; the
+        // warp that finishes the last group adds the groups' sums in order. So
+        // the result does not depend on who comes last, and no warp reads more
+        // than a few pieces after the other (128 pieces of one tile, added by
+        // one warp per part, took 200 us).
+        const int64_t size = (kind ? 1 : 2) * kT * kT;
+        float* parts = p.part[kind] + (warp - 4) * 32 * kCols;
+        const auto slot_of = [&](int i) { return i > 0 ? tl.first + i - 1 : p.max_extra + tl.first; };
+#pragma unroll 1
+        for (int acc = kind; acc < 2; ++acc) {
+          load_acc(t_self + (acc ? kColAcc2 : kColAcc1), o);
+          keep_part(o, parts + slot_of(tl.piece) * size + (acc - kind) * kT * kT, lane);
+        }
+        tc_fence_before();
+        mbar_arrive(&ctl->acc_free);
+        int* joined = p.joined[kind] + (warp - 4);
+        const int group = tl.piece / kJoin * kJoin;  // its first piece
+        int from = group, step = 1, n_parts = min(kJoin, tl.pieces - group);
+        // arrivals: of a group at its first piece's slot, of the groups at
+        // piece 1's, which begins no group
+        int at = slot_of(group);
+#pragma unroll 1
+        for (bool last = tl.pieces <= kJoin;; last = true) {
           __threadfence();
-          if (!kind) {
-            sum_parts(first, pieces, size, o, lane);
-            store_rows(o, 1.0f, o1, pitch1, rows, lane);
+          __syncwarp();
+          int done = 0;
+          if (lane == 0) done = atomicAdd(joined + at * (kWorkers / 32), 1) + 1;
+          done = __shfl_sync(0xffffffffu, done, 0);
+          if (done != n_parts) break;
+          __threadfence();
+#pragma unroll 1
+          for (int acc = kind; acc < 2; ++acc) {
+            float* of_acc = parts + (acc - kind) * kT * kT;
+#pragma unroll
+            for (int v = 0; v < kCols; ++v) o[v] = 0u;
+            for (int i = 0; i < n_parts; ++i)
+              add_part(o, of_acc + slot_of(from + i * step) * size, lane);
+            if (last) store(acc, o);
+            else keep_part(o, of_acc + slot_of(group) * size, lane);
           }
-          sum_parts(first + size - kT * kT, pieces, size, o, lane);
-          store_rows(o, p.scale, o2, pitch2, rows, lane);
+          if (last) break;
+          from = 0;
+          step = kJoin;
+          n_parts = (tl.pieces + kJoin - 1) / kJoin;
+          at = slot_of(1);
         }
       }
       J += n;
@@ -914,15 +999,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 namespace {
 
-// How the tiles of each kind may be cut, and where everything lies in the
-// workspace. Tiles are cut where there are fewer than two per SM: a mask with
-// one dense column (every query keeps key block 0) then leaves one CTA working
-// on that column long after the others are done (4096 tokens, 4 heads: 32
-// blocks in a row against 14 for an SM's share). With more tiles the items
-// even out by themselves and the pieces' traffic is saved.
+// Which kinds of tiles may be cut, and where everything lies in the workspace.
+// Few tiles do not fill the GPU, and among more of them a long one (a key block
+// that every query keeps) holds one SM after the others are done: one head of
+// 65536 tokens, a twentieth of its blocks kept, took 976 us without cutting
+// and takes 360. With 16 tiles per SM and a sixteenth of the blocks kept a full
+// line is within an SM's share, and the counting is saved.
 struct Layout {
-  int tiles[2], chunks[2];
-  size_t joined[2], n_joined, counts[2], stats, part[2], bytes;
+  int tiles[2], max_extra, n_joined, n_eights;
+  bool cut[2];
+  size_t counts[2], eights, joined[2], stats, part[2], bytes;
 };
 
 Layout layout_of(int B, int H, int Sq, int Sk, int sms) {
@@ -931,27 +1017,27 @@ Layout layout_of(int B, int H, int Sq, int Sk, int sms) {
   const int64_t bh = (int64_t)B * H;
   const int n[2] = {(Sk + kT - 1) / kT, (Sq + kT - 1) / kT};  // tiles of a head; the other's blocks
   size_t at = 256;
-  auto take = [&](size_t bytes) {
+  auto take = [&](bool needed, size_t bytes) {
     const size_t o = at;
-    at += (bytes + 255) / 256 * 256;
+    if (needed) at += (bytes + 255) / 256 * 256;
     return o;
   };
-  l.n_joined = 0;
+  const int64_t pieces = (int64_t)n[0] * n[1] * bh / kLeastPiece;
+  l.max_extra = pieces < sms ? (int)pieces : sms;
+  l.n_joined = l.n_eights = 0;
   for (int k = 0; k < 2; ++k) {
     l.tiles[k] = (int)(n[k] * bh);
-    l.chunks[k] = 1;
-    if (n[k] * bh < 2 * sms) {
-      const int most = n[1 - k] / kLeastPiece, items = 8 * sms / l.tiles[k];
-      l.chunks[k] = most < 1 ? 1 : most < items ? most : items;
-    }
+    l.cut[k] = n[k] * bh < 16 * sms && n[1 - k] >= 2 * kLeastPiece;
     l.joined[k] = 256 + l.n_joined * sizeof(int);
-    if (l.chunks[k] > 1) l.n_joined += (size_t)l.tiles[k] * (kWorkers / 32);
+    if (l.cut[k]) l.n_joined += 2 * l.max_extra * (kWorkers / 32);
   }
-  take(l.n_joined * sizeof(int));
-  for (int k = 0; k < 2; ++k) l.counts[k] = l.chunks[k] > 1 ? take(l.tiles[k] * sizeof(int)) : 0;
-  l.stats = take(2 * sizeof(float) * bh * n[1] * kT);
+  take(true, l.n_joined * sizeof(int));
+  for (int k = 0; k < 2; ++k) l.counts[k] = take(l.cut[k], l.tiles[k] * sizeof(int));
+  for (int k = 0; k < 2; ++k) l.n_eights += l.cut[k] ? (l.tiles[k] + 7) / 8 : 0;
+  l.eights = take(true, l.n_eights * sizeof(int));
+  l.stats = take(true, 2 * sizeof(float) * bh * n[1] * kT);
   for (int k = 0; k < 2; ++k)
-    l.part[k] = l.chunks[k] > 1 ? take((size_t)l.tiles[k] * l.chunks[k] * (2 - k) * kT * kT * 4) : 0;
+    l.part[k] = take(l.cut[k], (size_t)2 * l.max_extra * (2 - k) * kT * kT * 4);
   l.bytes = at;
   return l;
 }
@@ -1034,32 +1120,38 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
   p.next_item = static_cast<int*>(workspace);
   p.status = status;
   int* counts[2];
-  int items = 0;
   for (int k = 0; k < 2; ++k) {
     p.tiles[k] = l.tiles[k];
-    p.chunks[k] = l.chunks[k];
-    items += l.tiles[k] * l.chunks[k];
-    p.counts[k] = counts[k] = l.chunks[k] > 1 ? reinterpret_cast<int*>(ws + l.counts[k]) : nullptr;
+    p.counts[k] = counts[k] = l.cut[k] ? reinterpret_cast<int*>(ws + l.counts[k]) : nullptr;
     p.joined[k] = reinterpret_cast<int*>(ws + l.joined[k]);
     p.part[k] = reinterpret_cast<float*>(ws + l.part[k]);
   }
+  const bool cut = l.cut[0] || l.cut[1];
+  int* eights = reinterpret_cast<int*>(ws + l.eights);
+  p.eights = eights;
+  p.max_extra = l.max_extra;
 
   const bool fine = (int64_t)nq * nk * B * H <= sms;
-  const auto kernel = fine ? bsattn_bwd_kernel<true> : bsattn_bwd_kernel<false>;
+  const auto kernel = fine ? cut ? bsattn_bwd_kernel<true, true> : bsattn_bwd_kernel<true, false>
+                           : cut ? bsattn_bwd_kernel<false, true> : bsattn_bwd_kernel<false, false>;
   if ((rc = sa::func_attr_once((const void*)kernel,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes)) !=
       SA_OK)
     return rc;
   // heads run fastest: with the heads of a token side by side in memory, blocks
-  // that run together then read it in order
-  const dim3 pg((unsigned)(B * H), (unsigned)((nq * kT + 16 * kPrepRows - 1) / (16 * kPrepRows)));
+  // that run together then read it in order; at least a block for eight counted tiles
+  const int64_t chunks = (nq * kT + 16 * kPrepRows - 1) / (16 * kPrepRows);
+  const int64_t counting = (l.n_eights + (int64_t)B * H - 1) / ((int64_t)B * H);
+  const dim3 pg((unsigned)(B * H), (unsigned)(chunks > counting ? chunks : counting));
   row_stats_kernel<<<pg, 256, 0, stream>>>(
       static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
       do_strides[0], do_strides[1], do_strides[2], o_strides[0], o_strides[1], o_strides[2], lse,
-      dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_item,
-      reinterpret_cast<int*>(ws + 256), (int)l.n_joined, counts[0], counts[1], p.mask, B, nk, status);
+      dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_item, p.joined[0], l.n_joined,
+      counts[0], counts[1], eights, p.mask, B, nk, status);
   SA_CUDA_TRY(cudaGetLastError());
-  SA_CUDA_TRY(sa::launch_after(kernel, dim3(items < sms ? items : sms), dim3(kThreads),
-                               kSmemBytes, stream, tq, tk, tv, td, p));
+  // one CTA per SM; fewer only where there are fewer tiles and none may be cut
+  const int64_t tiles = (int64_t)p.tiles[0] + p.tiles[1];
+  SA_CUDA_TRY(sa::launch_after(kernel, dim3((unsigned)(cut || tiles > sms ? sms : tiles)),
+                               dim3(kThreads), kSmemBytes, stream, tq, tk, tv, td, p));
   return SA_OK;
 }

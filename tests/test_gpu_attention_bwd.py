@@ -120,6 +120,33 @@ def test_shapes(B, H, Sq, Sk, p):
     both(*make(B, H, Sq, Sk, p, Sq * 7 + Sk))
 
 
+@pytest.mark.parametrize("B,H,Sq,Sk", [
+    (1, 1, 16384, 100),   # one key tile in sixteen pieces, short query tiles
+    (1, 1, 77, 12800),    # the same for one query tile
+    (1, 2, 4225, 2049),   # both kinds, tiles of different lengths
+    (2, 4, 5120, 5000),   # many tiles: one long column each head
+])
+def test_tiles_longer_than_a_share_of_the_gpu(B, H, Sq, Sk):
+    q, k, v, dout, mask = make(B, H, Sq, Sk, 0.02, 7 + Sq)
+    mask[:, -1, 0] = True  # a long query tile too, and every column kept once
+    got = both(q, k, v, dout, mask)
+    again = run(q, k, v, dout, mask)
+    for x, y in zip(got, again):
+        assert torch.equal(x, y)
+
+
+def test_long_tiles_of_one_kind_among_many_of_the_other():
+    """140 heads of 17 x 16 blocks; all but the first keep nothing: its key tiles may be cut,
+    its query tiles are too many to."""
+    q, k, v, dout, mask = make(1, 140, 2176, 2048, 0.0, 3, empty=0.5)
+    mask[:, 0] = True
+    got = run(q, k, v, dout, mask)
+    keep = token_mask(mask[:, :1], 1, 1, 2176, 2048)
+    ref, bound = reference(q[:, :1], k[:, :1], v[:, :1], dout[:, :1], keep, 1 / math.sqrt(128))
+    check([x[:, :1] for x in got], ref, bound)
+    assert not any(x[:, 1:].any() for x in got)
+
+
 @pytest.mark.parametrize("layout", ["bshd", "bhsd"])
 @pytest.mark.parametrize("empty", [0.3, 1.0])
 def test_rows_and_columns_that_keep_nothing(layout, empty):

@@ -49,8 +49,9 @@ def test_attention_backward_workspace(lib):
     assert size(0, 1, 1, 1) == 0 and size(1, 1, 0, 1) == 0 and size(1, 1, 131073, 1) == 0
     # many tiles: the counter and two fp32 statistics of every padded query row
     assert size(2, 12, 32760, 32760) == 256 + 2 * 4 * 24 * 32768
-    # few long tiles may be cut: room for their pieces' sums
+    # few long tiles may be cut: room for their pieces' sums, 2 per SM at most
     assert size(1, 1, 4096, 4096) > 256 + 2 * 4 * 4096 + 32 * 2 * 3 * 128 * 128 * 4
+    assert size(1, 1, 131072, 131072) < 2 * 4 * 131072 + 256 * 2 * 3 * 128 * 128 * 4 + (1 << 20)
 
 
 def _head(lib, *, B=1, S=4, Hq=4, Hk=2, D=128, dtype=0, wq=None, wk=None, wd=0, cos=256, sin=256,
