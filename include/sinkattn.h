@@ -153,8 +153,8 @@ SA_API int sa_sink_dynamic_attn_fwd(
  *   and *status becomes SA_DEV_BAD_INDEX). Sq, Sk <= 131072. P and dS enter
  *   their products as bf16 (as two bf16 halves each where the call has no more
  *   blocks than the GPU has SMs); the sums, dP and the row statistics are fp32.
- * Every sum is formed by one CTA in block order (no atomics on data), so equal
- *   calls give equal bits.
+ * Sums are formed in block order, those of long mask lines in pieces that are
+ *   added in a fixed order (no atomics on data), so equal calls give equal bits.
  * workspace: sa_bsattn_bwd_workspace_size(B, H, Sq, Sk) bytes, 256-byte
  *   aligned, with any contents. Calls sharing one workspace must not overlap
  *   on the GPU.

@@ -62,6 +62,16 @@ bool vectors(const at::Tensor& t) {
   return true;
 }
 
+// An output may not be expanded, a workspace is one run of bytes.
+bool output(const Arg& a) {
+  if (!a) return true;
+  for (int64_t i = 0; i < a->dim(); ++i)
+    if (a->size(i) > 1 && a->stride(i) == 0) return false;
+  return true;
+}
+
+bool workspace(const Arg& a) { return !a || a->is_contiguous(); }
+
 struct Strides {
   int64_t s[4] = {8, 8, 8, 1};
   explicit Strides(const at::Tensor& t) {
@@ -143,6 +153,7 @@ PyObject* bsattn_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
   for (const Arg* t : {&dout, &q, &k, &v, &out, &dq, &dk, &dv})
     if (*t && !vectors(**t)) return none();
+  if (!output(dq) || !output(dk) || !output(dv) || !workspace(ws)) return none();
   for (const Arg* t : {&lse, &dlse})
     if (*t && ((*t)->scalar_type() != at::kFloat || (*t)->dim() != 3 || (*t)->size(0) != B ||
                (*t)->size(1) != H || (*t)->size(2) != Sq || !(*t)->is_contiguous()))
@@ -215,6 +226,7 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     st[i] = *rows[i] ? row_stride(**rows[i]) : hidden;
     if (st[i] < 0) return none();
   }
+  if (!output(dq) || !output(dk) || !workspace(ws)) return none();
   if (bool(wq) != bool(wk) || bool(cos) != bool(sin)) return none();
   if (wq && (wq->dim() != 1 || wq->size(0) != hidden || !same(*wk, *wq) || !flat(*wq) ||
              !flat(*wk) ||
@@ -283,7 +295,7 @@ struct Head {
     if (wq) wdtype = dtype_of(wq->scalar_type());
     if (wdtype < 0 || bool(cos) != bool(sin)) return;
     if (cos) {
-      if (cos->dim() != 2 || cos->scalar_type() != at::kFloat || !same(*sin, *cos) ||
+      if (cos->dim() != 2 || cos->size(0) < 1 || cos->scalar_type() != at::kFloat || !same(*sin, *cos) ||
           !vectors(*cos) || !vectors(*sin) || cos->size(0) > 0x7fffffff || cos->size(1) > 128)
         return;
       rows = (int)cos->size(0);
@@ -321,7 +333,7 @@ PyObject* qk_head_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 11 || lib.head == nullptr) return none();
   const Head h(a);
   const Arg oq(a[9]), ok(a[10]);
-  if (!h.ok || !fits(oq, h.q) || !fits(ok, h.k)) return none();
+  if (!h.ok || !fits(oq, h.q) || !fits(ok, h.k) || !output(oq) || !output(ok)) return none();
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)h.dev);
   const at::Tensor rq = result(oq, h.q), rk = result(ok, h.k);
   const Strides sq(*h.q), sk = h.k ? Strides(*h.k) : Strides(), tq(rq),
@@ -343,7 +355,8 @@ PyObject* qk_head_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Head h(a);
   const Arg uq(a[9]), uk(a[10]), dq(a[11]), dk(a[12]), ws(a[13]);
   if (!h.ok || !uq || bool(uk) != bool(h.k) || !fits(uq, h.q) || !fits(uk, h.k) ||
-      !fits(dq, h.q) || !fits(dk, h.k) || !on(ws, h.dev))
+      !fits(dq, h.q) || !fits(dk, h.k) || !output(dq) || !output(dk) || !on(ws, h.dev) ||
+      !workspace(ws))
     return none();
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)h.dev);
   const at::Tensor rq = result(dq, h.q), rk = result(dk, h.k);

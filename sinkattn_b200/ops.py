@@ -86,6 +86,16 @@ def _kernel_strides(t: torch.Tensor):
         *(s if size > 1 else 8 for s, size in zip(t.stride()[:-1], t.shape[:-1])), 1)
 
 
+def _check_output(fn: str, name: str, t: torch.Tensor) -> None:
+    if any(s == 0 and size > 1 for s, size in zip(t.stride(), t.shape)):
+        raise RuntimeError(f"{fn}: {name} is expanded: its elements share memory")
+
+
+def _check_workspace(fn: str, t: torch.Tensor, dev: torch.device) -> None:
+    if t.device != dev or not t.is_contiguous():
+        raise RuntimeError(f"{fn}: workspace must be contiguous on {dev}")
+
+
 def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
@@ -299,8 +309,8 @@ def bsattn_bwd(
     dv = v.new_empty_strided(*grads[1]) if dv is None else dv
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.get_device() != idx:
-        raise RuntimeError(f"bsattn_bwd: workspace must be on {dev}")
+    else:
+        _check_workspace("bsattn_bwd", workspace, dev)
     _launch(idx, "sa_bsattn_bwd", _lib.load().sa_bsattn_bwd, *ins, *in_strides, lse.data_ptr(),
             _ptr(dlse), *middle[0], block_mask.data_ptr(), *middle[1], _ptr(head_mask_type),
             middle[2], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *out_strides,
@@ -322,9 +332,11 @@ def _bsattn_bwd_plan(dout, q, k, v, out, lse, block_mask, softmax_scale, head_ma
         if t.dtype != torch.bfloat16 or t.shape != (B, H, S, D):
             raise RuntimeError(f"bsattn_bwd: {name} must be bf16 {(B, H, S, D)}, got {t.dtype} "
                                f"{tuple(t.shape)}")
-        if name in ("dq", "dk", "dv") and not _view16_ok(t):
-            raise RuntimeError(f"bsattn_bwd: {name} must have stride(-1)=1, 16-byte strides and "
-                               "alignment")
+        if name in ("dq", "dk", "dv"):
+            _check_output("bsattn_bwd", name, t)
+            if not _view16_ok(t):
+                raise RuntimeError(f"bsattn_bwd: {name} must have stride(-1)=1, 16-byte strides "
+                                   "and alignment")
     for name, t in (("lse", lse), ("dlse", dlse)):
         if t is not None and (t.dtype != torch.float32 or t.shape != (B, H, Sq)):
             raise RuntimeError(f"bsattn_bwd: {name} must be fp32 {(B, H, Sq)}, got {t.dtype} "
@@ -1037,8 +1049,8 @@ def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor
         dw_k = torch.empty(sizes[2], dtype=torch.float32, device=dev)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        elif workspace.get_device() != idx:
-            raise RuntimeError(f"qk_norm_rope_bwd: workspace must be on {dev}")
+        else:
+            _check_workspace("qk_norm_rope_bwd", workspace, dev)
     ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if need \
         else (None, 0)
     _launch(idx, "sa_qk_norm_rope_bwd", _lib.load().sa_qk_norm_rope_bwd, ptrs[0], ptrs[1],
@@ -1071,8 +1083,10 @@ def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, w_q, w_k, cos, sin, d
         if t is not None and (t.dtype != torch.bfloat16 or t.shape != (B, S, hidden)):
             raise RuntimeError(f"qk_norm_rope_bwd: {name} must be bf16 {(B, S, hidden)}, got "
                                f"{t.dtype} {tuple(t.shape)}")
-        if t is not None and name in ("dq", "dk") and _row_stride(t) is None:
-            raise RuntimeError("qk_norm_rope_bwd outputs need uniform rows, 16-byte aligned")
+        if t is not None and name in ("dq", "dk"):
+            _check_output("qk_norm_rope_bwd", name, t)
+            if _row_stride(t) is None:
+                raise RuntimeError("qk_norm_rope_bwd outputs need uniform rows, 16-byte aligned")
     if (w_q is None) != (w_k is None) or (cos is None) != (sin is None):
         raise RuntimeError("qk_norm_rope_bwd: w_q and w_k, cos and sin go together")
     fits = all(_row_stride(t) is not None for t in (dq_out, dk_out, q, k))
@@ -1126,7 +1140,10 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
         if like is not None and t is None:
             raise RuntimeError(f"{fn}: {name} is missing")
     for name, t, _ in outs:
-        if t is not None and not _strides16_ok(t):
+        if t is None:
+            continue
+        _check_output(fn, name, t)
+        if not _strides16_ok(t):
             raise RuntimeError(f"{fn}: {name} must have stride(-1)=1, 16-byte strides and "
                                "alignment")
     fits = all(t is None or _strides16_ok(t) for t in (q, k, *(t for _, t, _ in more)))
@@ -1151,6 +1168,8 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
                                f", got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} "
                                f"{tuple(sin.shape)}")
         rows, rot = cos.shape[0], 2 * cos.shape[1]
+        if rows == 0 and q.numel():
+            raise RuntimeError(f"{fn}: cos and sin have no rows")
         fs = cos.stride(0) if rows > 1 else (rot // 2 + 3) // 4 * 4
         fits = fits and _strides16_ok(cos) and _strides16_ok(sin) and (
             rows == 1 or fs == sin.stride(0) >= rot // 2)
@@ -1277,8 +1296,8 @@ def qk_head_norm_rope_bwd(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], 
         dw_k = None if k is None else torch.empty(sizes[4], dtype=torch.float32, device=dev)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        elif workspace.get_device() != idx:
-            raise RuntimeError(f"{fn}: workspace must be on {dev}")
+        else:
+            _check_workspace(fn, workspace, dev)
     ws = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if need \
         else (None, 0)
     _launch(idx, "sa_qk_head_norm_rope_bwd", _lib.load().sa_qk_head_norm_rope_bwd, ptrs[0],

@@ -339,6 +339,26 @@ def test_refusals():
     refuse("mask has 1 heads", block_mask=mask[:, :1])
 
 
+def test_expanded_outputs_and_workspaces_are_refused():
+    from sinkattn_b200 import ops
+
+    q, k, v, dout, mask = make(2, 2, 200, 300, 1.0, 20)
+    out, lse = ops.bsattn_fwd(q, k, v, mask)
+    need = 1 << 22
+    for name, t in (("dq", q[:, :1].contiguous().expand(-1, 2, -1, -1)),
+                    ("dk", k[:1].contiguous().expand(2, -1, -1, -1)),
+                    ("dv", v[:, :, :1].contiguous().expand(-1, -1, 300, -1))):
+        with pytest.raises(RuntimeError, match=name + " is expanded"):
+            ops.bsattn_bwd(dout, q, k, v, out, lse, mask, **{name: t})
+    for ws in (torch.empty(1, dtype=torch.uint8, device="cuda").expand(need),
+               torch.empty(2 * need, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(RuntimeError, match="workspace must be contiguous"):
+            ops.bsattn_bwd(dout, q, k, v, out, lse, mask, workspace=ws)
+    # inputs may be: keys shared by the heads
+    k1 = k[:, :1].expand(-1, 2, -1, -1)
+    ops.bsattn_bwd(dout, q, k1, v, out, lse, mask)
+
+
 def test_from_a_thread_without_a_context():
     """A thread whose first CUDA call is ours (an autograd worker may be one):
     through the C entry point, as torch's own calls would bind the context."""

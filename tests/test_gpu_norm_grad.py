@@ -439,6 +439,33 @@ def test_refusals():
             ops.qk_norm_rope_bwd(**{**h, **kw})
 
 
+def test_expanded_outputs_workspaces_and_empty_tables_are_refused():
+    from sinkattn_b200 import ops
+
+    q = torch.randn(2, 3, 4, 64, device="cuda").bfloat16()
+    w = torch.ones(64, device="cuda").bfloat16()
+    none = torch.empty(0, 32, device="cuda")
+    wide = q[:, :, :1].contiguous().expand(-1, -1, 4, -1)
+    small = torch.empty(1, dtype=torch.uint8, device="cuda").expand(1 << 22)
+    with pytest.raises(RuntimeError, match="out_k is expanded"):
+        ops.qk_head_norm_rope(q, q, 1e-6, out_k=wide)
+    with pytest.raises(RuntimeError, match="dq is expanded"):
+        ops.qk_head_norm_rope_bwd(q, q, q, q, 1e-6, dq=wide)
+    with pytest.raises(RuntimeError, match="workspace must be contiguous"):
+        ops.qk_head_norm_rope_bwd(q, q, q, q, 1e-6, w, w, workspace=small)
+    with pytest.raises(RuntimeError, match="have no rows"):
+        ops.qk_head_norm_rope(q, q, 1e-6, w, w, none, none)
+    with pytest.raises(RuntimeError, match="have no rows"):
+        ops.qk_head_norm_rope(q, q, 1e-6, w, w, none, none,
+                              positions=torch.zeros(3, dtype=torch.int32, device="cuda"))
+    x = torch.randn(2, 3, 256, device="cuda").bfloat16()
+    w = torch.ones(256, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError, match="dk is expanded"):
+        ops.qk_norm_rope_bwd(x, x, x, x, 64, 1e-6, dk=x[:, :1].contiguous().expand(-1, 3, -1))
+    with pytest.raises(RuntimeError, match="workspace must be contiguous"):
+        ops.qk_norm_rope_bwd(x, x, x, x, 64, 1e-6, w, w, workspace=small)
+
+
 def test_the_short_way_is_taken_and_agrees_with_the_long_one(monkeypatch):
     from sinkattn_b200 import ops
 
