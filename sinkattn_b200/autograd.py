@@ -19,9 +19,6 @@ from torch.autograd.function import once_differentiable
 
 from . import ops
 
-MAX_TOKENS = 131072  # queries or keys of a call whose gradient is wanted
-
-
 def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a call on these tensors has to be recorded."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
@@ -58,10 +55,8 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     Arguments as for ops.bsattn_fwd. Returns (out [B,H,Sq,D] bf16, lse fp32
     [B,H,Sq]). Keys and values broadcast over heads (expanded views) get their
-    gradients summed over them by autograd."""
-    if needs_grad(q, k, v) and max(q.shape[-2], k.shape[-2]) > MAX_TOKENS:
-        raise RuntimeError(f"the attention's gradient takes at most {MAX_TOKENS} tokens, got "
-                           f"{q.shape[-2]} queries and {k.shape[-2]} keys")
+    gradients summed over them by autograd. The backward pass takes at most
+    131072 queries and keys and refuses more."""
     return _BlockSparseAttention.apply(q, k, v, block_mask, softmax_scale, head_mask_type)
 
 

@@ -113,6 +113,17 @@ PyObject* wrap(const at::Tensor& t) {
   return THPVariable_Wrap(t);
 }
 
+// The library's calls wait where the launch queue is full, so they run without
+// the interpreter lock.
+template <typename F>
+int without_gil(F&& f) {
+  struct Released {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Released() { PyEval_RestoreThread(state); }
+  } released;
+  return f();
+}
+
 // A tuple of results, or the library's return code for ops.py to raise.
 PyObject* finish(int rc, const std::initializer_list<at::Tensor>& out) {
   if (rc != SA_OK) return PyLong_FromLong(rc);
@@ -179,12 +190,14 @@ PyObject* bsattn_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t ms[4] = {mask->size(0) == 1 ? 0 : mask->stride(0), mask->stride(1),
                          mask->stride(2), mask->stride(3)};
   const Strides sd(*dout), sq(*q), sk(*k), sv(*v), so(*out), tq(gq), tk(gk), tv(gv);
-  const int rc = lib.bsattn_bwd(
-      dout.ptr(), q.ptr(), k.ptr(), v.ptr(), out.ptr(), sd.s, sq.s, sk.s, sv.s, so.s,
-      (const float*)lse.ptr(), (const float*)dlse.ptr(), (int)B, (int)H, (int)Sq, (int)Sk, 128,
-      (const uint8_t*)mask.ptr(), ms, (int)mask->size(1), (const int32_t*)hmt.ptr(), (float)scale,
-      gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), tq.s, tk.s, tv.s, w.data_ptr(),
-      (size_t)w.nbytes(), g_status[dev], c10::cuda::getCurrentCUDAStream(dev).stream());
+  const int rc = without_gil([&] {
+    return lib.bsattn_bwd(
+        dout.ptr(), q.ptr(), k.ptr(), v.ptr(), out.ptr(), sd.s, sq.s, sk.s, sv.s, so.s,
+        (const float*)lse.ptr(), (const float*)dlse.ptr(), (int)B, (int)H, (int)Sq, (int)Sk, 128,
+        (const uint8_t*)mask.ptr(), ms, (int)mask->size(1), (const int32_t*)hmt.ptr(), (float)scale,
+        gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), tq.s, tk.s, tv.s, w.data_ptr(),
+        (size_t)w.nbytes(), g_status[dev], c10::cuda::getCurrentCUDAStream(dev).stream());
+  });
   return finish(rc, {gq, gk, gv});
   END_HANDLE_TH_ERRORS
 }
@@ -246,13 +259,15 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     gwk = at::empty({hidden}, q->options().dtype(at::kFloat));
     w = ws ? *ws : bytes(lib.norm_bwd_ws((int)hidden), *q);
   }
-  const int rc = lib.norm_bwd(
-      dqo.ptr(), dko.ptr(), st[0], st[1], q.ptr(), k.ptr(), st[2], st[3], (int)(B * S), (int)S,
-      (int)hidden, D, wq.ptr(), wk.ptr(), wq && wq->scalar_type() == at::kBFloat16, (float)eps,
-      (const float*)cos.ptr(), (const float*)sin.ptr(), cos ? D / 2 : 0, gq.data_ptr(),
-      gk.data_ptr(), st[4], st[5], wq ? gwq.data_ptr<float>() : nullptr,
-      wq ? gwk.data_ptr<float>() : nullptr, wq ? w.data_ptr() : nullptr,
-      wq ? (size_t)w.nbytes() : 0, g_status[dev], c10::cuda::getCurrentCUDAStream(dev).stream());
+  const int rc = without_gil([&] {
+    return lib.norm_bwd(
+        dqo.ptr(), dko.ptr(), st[0], st[1], q.ptr(), k.ptr(), st[2], st[3], (int)(B * S), (int)S,
+        (int)hidden, D, wq.ptr(), wk.ptr(), wq && wq->scalar_type() == at::kBFloat16, (float)eps,
+        (const float*)cos.ptr(), (const float*)sin.ptr(), cos ? D / 2 : 0, gq.data_ptr(),
+        gk.data_ptr(), st[4], st[5], wq ? gwq.data_ptr<float>() : nullptr,
+        wq ? gwk.data_ptr<float>() : nullptr, wq ? w.data_ptr() : nullptr,
+        wq ? (size_t)w.nbytes() : 0, g_status[dev], c10::cuda::getCurrentCUDAStream(dev).stream());
+  });
   return finish(rc, {gq, gk, gwq, gwk});
   END_HANDLE_TH_ERRORS
 }
@@ -338,11 +353,13 @@ PyObject* qk_head_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor rq = result(oq, h.q), rk = result(ok, h.k);
   const Strides sq(*h.q), sk = h.k ? Strides(*h.k) : Strides(), tq(rq),
                 tk = h.k ? Strides(rk) : Strides();
-  const int rc = lib.head(
-      h.q.ptr(), h.k.ptr(), sq.s, sk.s, h.B, h.S, h.Hq, h.Hk, h.D, h.dtype, h.wq.ptr(), h.wk.ptr(),
-      h.wdtype, (float)h.eps, (const float*)h.cos.ptr(), (const float*)h.sin.ptr(), h.fs, h.rows,
-      h.rot, h.inter, h.pos.ptr(), h.pos64, h.pst, ptr(rq), ptr(rk), tq.s, tk.s, g_status[h.dev],
-      c10::cuda::getCurrentCUDAStream(h.dev).stream());
+  const int rc = without_gil([&] {
+    return lib.head(
+        h.q.ptr(), h.k.ptr(), sq.s, sk.s, h.B, h.S, h.Hq, h.Hk, h.D, h.dtype, h.wq.ptr(), h.wk.ptr(),
+        h.wdtype, (float)h.eps, (const float*)h.cos.ptr(), (const float*)h.sin.ptr(), h.fs, h.rows,
+        h.rot, h.inter, h.pos.ptr(), h.pos64, h.pst, ptr(rq), ptr(rk), tq.s, tk.s, g_status[h.dev],
+        c10::cuda::getCurrentCUDAStream(h.dev).stream());
+  });
   return finish(rc, {rq, rk});
   END_HANDLE_TH_ERRORS
 }
@@ -369,13 +386,15 @@ PyObject* qk_head_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const Strides sq(*h.q), sk = h.k ? Strides(*h.k) : Strides(), tq(rq),
                 tk = h.k ? Strides(rk) : Strides(), vq(*uq), vk = h.k ? Strides(*uk) : Strides();
-  const int rc = lib.head_bwd(
-      uq.ptr(), uk.ptr(), vq.s, vk.s, h.q.ptr(), h.k.ptr(), sq.s, sk.s, h.B, h.S, h.Hq, h.Hk, h.D,
-      h.dtype, h.wq.ptr(), h.wk.ptr(), h.wdtype, (float)h.eps, (const float*)h.cos.ptr(),
-      (const float*)h.sin.ptr(), h.fs, h.rows, h.rot, h.inter, h.pos.ptr(), h.pos64, h.pst,
-      ptr(rq), ptr(rk), tq.s, tk.s, (float*)ptr(gwq), (float*)ptr(gwk), ptr(w),
-      w.defined() ? (size_t)w.nbytes() : 0, g_status[h.dev],
-      c10::cuda::getCurrentCUDAStream(h.dev).stream());
+  const int rc = without_gil([&] {
+    return lib.head_bwd(
+        uq.ptr(), uk.ptr(), vq.s, vk.s, h.q.ptr(), h.k.ptr(), sq.s, sk.s, h.B, h.S, h.Hq, h.Hk, h.D,
+        h.dtype, h.wq.ptr(), h.wk.ptr(), h.wdtype, (float)h.eps, (const float*)h.cos.ptr(),
+        (const float*)h.sin.ptr(), h.fs, h.rows, h.rot, h.inter, h.pos.ptr(), h.pos64, h.pst,
+        ptr(rq), ptr(rk), tq.s, tk.s, (float*)ptr(gwq), (float*)ptr(gwk), ptr(w),
+        w.defined() ? (size_t)w.nbytes() : 0, g_status[h.dev],
+        c10::cuda::getCurrentCUDAStream(h.dev).stream());
+  });
   return finish(rc, {rq, rk, gwq, gwk});
   END_HANDLE_TH_ERRORS
 }

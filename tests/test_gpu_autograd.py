@@ -42,6 +42,21 @@ def test_attention_function_both_results():
         torch.autograd.grad(first.float().sum(), leaves[1])
 
 
+def test_more_queries_than_the_gradient_takes():
+    """The forward pass of a call that records runs as it does unrecorded; the backward refuses."""
+    from sinkattn_b200 import ops
+    from sinkattn_b200.autograd import block_sparse_attention
+
+    q = torch.randn(1, 1, 131073, 128, device="cuda").bfloat16().requires_grad_()
+    k, v = (torch.randn(1, 1, 100, 128, device="cuda").bfloat16() for _ in range(2))
+    mask = torch.ones(1, 1, 1025, 1, dtype=torch.bool, device="cuda")
+    out, lse = block_sparse_attention(q, k, v, mask)
+    want, want_lse = ops.bsattn_fwd(q.detach(), k, v, mask)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    with pytest.raises(RuntimeError, match="at most 131072"):
+        out.sum().backward()
+
+
 def test_broadcast_keys_and_a_broadcast_gradient():
     from sinkattn_b200.autograd import block_sparse_attention
 
