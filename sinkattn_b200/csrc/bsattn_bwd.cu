@@ -540,7 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         w.pitch[0] = p.dvs2;
         w.pitch[1] = kind ? p.dqs2 : p.dks2;
         w.out[0] = p.dv + w.b * p.dvs0 + w.h * p.dvs1 + row * p.dvs2;
-        w.out[1] = (kind ? p.dq + w.b * p.dqs0 + w.h * p.dqs1 : p.dk + w.b * p.dks0 + w.h * p.dks1) +
+        w.out[1] = (kind ? p.dq + w.b * p.dqs0 + w.h * p.dqs1
+                         : p.dk + w.b * p.dks0 + w.h * p.dks1) +
                    row * w.pitch[1];
       }
       ctl->kept[slot][lane] = word;
@@ -942,7 +943,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // one warp per part, took 200 us).
         const int64_t size = (kind ? 1 : 2) * kT * kT;
         float* parts = p.part[kind] + (warp - 4) * 32 * kCols;
-        const auto slot_of = [&](int i) { return i > 0 ? tl.first + i - 1 : p.max_extra + tl.first; };
+        const auto slot_of = [&](int i) {
+          return i > 0 ? tl.first + i - 1 : p.max_extra + tl.first;
+        };
 #pragma unroll 1
         for (int acc = kind; acc < 2; ++acc) {
           load_acc(t_self + (acc ? kColAcc2 : kColAcc1), o);

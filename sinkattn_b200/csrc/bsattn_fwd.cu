@@ -731,8 +731,9 @@ int launch_attention(const char* fn, const void* q, const void* k, const void* v
   SA_CHECK_ARG(nk + nk2 <= kMaxBlocks && nk2 < 0x8000,
                "%s: %d + %d key blocks exceed %d", fn, nk, nk2, kMaxBlocks);
   SA_CHECK_ARG((int64_t)nq * H * B <= 0x7fffffff, "%s: too many query tiles", fn);
-  SA_CHECK_ARG(sa::strides16_ok(q_strides) && sa::strides16_ok(k_strides) && sa::strides16_ok(v_strides) &&
-                   sa::strides16_ok(o_strides) && (!dual || (sa::strides16_ok(k2_strides) && sa::strides16_ok(v2_strides))),
+  SA_CHECK_ARG(sa::strides16_ok(q_strides) && sa::strides16_ok(k_strides) &&
+                   sa::strides16_ok(v_strides) && sa::strides16_ok(o_strides) &&
+                   (!dual || (sa::strides16_ok(k2_strides) && sa::strides16_ok(v2_strides))),
                "%s: q/k/v/out need stride(dim)=1 and other strides multiple of 8 "
                "elements (16 bytes)", fn);
   SA_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out |

@@ -416,7 +416,8 @@ bool aligned_ok(const void* base, const int64_t st[4], int dtype) {
   if (base == nullptr) return true;
   const int64_t mult = dtype == SA_DTYPE_FP32 ? 4 : 8;
   return (uintptr_t)base % 16 == 0 && st != nullptr && st[3] == 1 && st[0] >= 0 && st[1] >= 0 &&
-         st[2] >= 0 && st[0] % mult == 0 && st[1] % mult == 0 && st[2] % mult == 0 && st[2] <= 0x7fffffff;
+         st[2] >= 0 && st[0] % mult == 0 && st[1] % mult == 0 && st[2] % mult == 0 &&
+         st[2] <= 0x7fffffff;
 }
 
 // Arguments that the forward and the gradient share.
@@ -501,7 +502,8 @@ extern "C" int sa_qk_head_norm_rope(
   common(p, q, k, q_strides, k_strides, B, S, Hq, Hk, D, w_q, w_k, w_dtype, eps, cos_table,
          sin_table, freq_row_stride, table_rows, rot_dim, positions, positions_i64, pos_strides,
          q_out, k_out, qo_strides, ko_strides, status);
-  shape(p, dtype == SA_DTYPE_FP32 ? ahead<float>() : ahead<__half>(), (int64_t)sa::sm_count_current_device() * 64);
+  shape(p, dtype == SA_DTYPE_FP32 ? ahead<float>() : ahead<__half>(),
+        (int64_t)sa::sm_count_current_device() * 64);
   const int64_t blocks = ((int64_t)p.tokens * p.chunks + kWarps - 1) / kWarps;
   SA_CHECK_ARG(blocks <= 0x7fffffff / kWarps, "%s: too many tokens", fn);
   return dispatch(p, dtype, interleaved != 0, false, (int)blocks, stream);
@@ -510,7 +512,8 @@ extern "C" int sa_qk_head_norm_rope(
 extern "C" size_t sa_qk_head_norm_rope_bwd_workspace_size(int D) {
   if (D < 8) return 0;
   const int64_t most = (int64_t)sa::sm_count_current_device() * sa::headnorm::kBwdBlocksPerSm;
-  const int64_t least = sa::headnorm::kMaxHeads / (sa::headnorm::kAheadBwd * sa::headnorm::kWarps) + 1;
+  const int64_t least =
+      sa::headnorm::kMaxHeads / (sa::headnorm::kAheadBwd * sa::headnorm::kWarps) + 1;
   return (size_t)(most > least ? most : least) * 2 * D * sizeof(float);
 }
 

@@ -8,9 +8,9 @@
 // (6 bf16 values per hidden channel of Q and K together). A block takes whole
 // rows, one 8-channel vector of Q and one of K per thread, so that the angles
 // are read once for both and dw needs 16 registers. The rows and their angles
-// come through a ring of bulk copies, three rows ahead. (A warp per row with 48 channels a
-// lane needed 158 registers and reached 28% of the copy rate; rows loaded one
-// ahead into registers spilled and reached 55%.)
+// come through a ring of bulk copies, three rows ahead. (A warp per row with 48
+// channels a lane needed 158 registers and reached 28% of the copy rate; rows
+// loaded one ahead into registers spilled and reached 55%.)
 
 #include <math.h>
 

@@ -147,10 +147,10 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar_addr, uint32_t parity
   return ok != 0;
 }
 
-// Records a failure (a bounded wait that gave up, a bad index). The status word may live in device
-// memory or in mapped page-locked host memory (the host then reads it
-// without synchronising), so it is written with a plain store made visible
-// system-wide; the last writer's code stands.
+// Records a failure (a bounded wait that gave up, a bad index). The status
+// word may live in device memory or in mapped page-locked host memory (the
+// host then reads it without synchronising), so it is written with a plain
+// store made visible system-wide; the last writer's code stands.
 __device__ __forceinline__ void report_status(int32_t* status, int32_t code) {
   if (status == nullptr) return;
   *reinterpret_cast<volatile int32_t*>(status) = code;

@@ -1118,8 +1118,9 @@ _DTYPES = {torch.bfloat16: _lib.SA_DTYPE_BF16, torch.float16: _lib.SA_DTYPE_FP16
 
 
 def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, outs):
-    """What qk_head_norm_rope and its gradient derive from their tensors. more: further (name, tensor, like) inputs; outs: the same of
-    outputs, None for one to be allocated."""
+    """What qk_head_norm_rope and its gradient derive from their tensors. more:
+    further (name, tensor, like) inputs; outs: the same of outputs, None for
+    one to be allocated."""
     dev = _require_cuda(q, k, w_q, w_k, cos, sin, positions, *(t for _, t, _ in more + outs))
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise RuntimeError(f"{fn} expects q, k of [B, S, heads, D]")
