@@ -157,3 +157,19 @@ def test_bad_index_status_is_told_from_a_timeout(lib):
     word.value = _lib.SA_DEV_WAIT_TIMEOUT
     assert lib.sa_check_status(ctypes.addressof(word)) == _lib.SA_ETIMEOUT and word.value == 0
     assert lib.sa_check_status(ctypes.addressof(word)) == _lib.SA_OK
+
+
+def test_build_without_the_extension_warns_and_leaves_no_stale_one(monkeypatch, tmp_path):
+    from sinkattn_b200 import build
+
+    stale = tmp_path / "_fast.so"
+    stale.write_bytes(b"")
+
+    def fail(*args):
+        raise RuntimeError("no headers")
+
+    monkeypatch.setattr(build, "FAST", stale)
+    monkeypatch.setattr(build, "build_fast", fail)
+    with pytest.warns(UserWarning, match="no headers"):
+        assert build.build() == build.LIB
+    assert not stale.exists()
