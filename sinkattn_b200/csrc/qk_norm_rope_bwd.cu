@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
   }
   release_next_kernel();
   __syncthreads();
+  wait_prior_kernel();
   auto fetch = [&](int slot, int row) {
     uint8_t* dst = ring + slot * slot_bytes;
     mbar_arrive_expect_tx(&full[slot], slot_bytes);
@@ -295,9 +296,8 @@ extern "C" int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_ro
                                       // rows and angles of the widest head, D = hidden
                                       kRing * (4 * 2 + 4) * 8 * (threads <= 256 ? 256 : kMaxThreads));
     if (rc != SA_OK) return rc;
-    if (threads <= 256) kernel<256><<<part_rows, threads, smem, stream>>>(p);
-    else kernel<kMaxThreads><<<part_rows, threads, smem, stream>>>(p);
-    SA_CUDA_TRY(cudaGetLastError());
+    SA_CUDA_TRY(sa::launch_after(threads <= 256 ? kernel<256> : kernel<kMaxThreads>,
+                                 dim3(part_rows), dim3(threads), smem, stream, p));
   }
   if (dw_q == nullptr) return SA_OK;
   return sa::nr::sum_partial_rows(part, part_rows, 2 * hidden, 2 * hidden, dw_q, dw_k, hidden,

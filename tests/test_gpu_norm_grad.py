@@ -506,3 +506,58 @@ def test_the_short_way_is_taken_and_agrees_with_the_long_one(monkeypatch):
         assert len(got) == len(want)
         for p, q in zip(got, want):
             assert (p is None and q is None) or (torch.equal(p, q) and p.stride() == q.stride())
+
+
+def test_captured_after_a_copy_a_fill_and_another_stream():
+    """The launches may start while the one before them ends: whatever that one is, a replay gives
+    what an eager run gives."""
+    from sinkattn_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    src = torch.randn(2, 300, 6, 128, generator=g, device="cuda").bfloat16()
+    mask = torch.ones(2, 6, 3, 3, dtype=torch.bool, device="cuda")
+    w = torch.ones(128, device="cuda")
+    x, y, z = (torch.empty_like(src) for _ in range(3))
+    side = torch.cuda.Stream()
+
+    def step():
+        x.copy_(src)                                       # a copy
+        q, _ = ops.qk_head_norm_rope(x, None, 1e-6, w)
+        y.zero_()                                          # a fill
+        a = ops.qk_head_norm_rope_bwd(q, y, x, y, 1e-6, w, w)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):                      # another stream's kernel
+            z.copy_(a[0])
+            z.mul_(2)
+        torch.cuda.current_stream().wait_stream(side)
+        t = [s.transpose(1, 2) for s in (x, z, q)]
+        out, lse = ops.bsattn_fwd(*t, mask)
+        y.zero_()
+        b = ops.bsattn_bwd(out, *t, out, lse, mask)
+        y.copy_(b[0].transpose(1, 2))
+        return (q,) + a[:1] + a[2:] + b + ops.qk_norm_rope_bwd(
+            y.view(2, 300, 768), x.view(2, 300, 768), z.view(2, 300, 768), y.view(2, 300, 768),
+            128, 1e-6)[:2]
+
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    warm = torch.cuda.Stream()
+    with torch.cuda.stream(warm):
+        step()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        for t in got:
+            t.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+    for _ in range(20):  # many calls in a row, each reading what the one before wrote
+        eager = step()
+    torch.cuda.synchronize()
+    for a, b in zip(want, eager):
+        assert torch.equal(a, b)
+    ops.DeviceStatus.check()
