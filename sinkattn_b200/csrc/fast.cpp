@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -92,8 +93,13 @@ bool same(const at::Tensor& a, const at::Tensor& b) {
 
 bool flat(const at::Tensor& t) { return t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0; }
 
+// Fresh contiguous memory, past the dispatcher (0.25 us less than at::empty).
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(size, type, like.device(), std::nullopt));
+}
+
 at::Tensor bytes(size_t n, const at::Tensor& like) {
-  return at::empty({(int64_t)n}, like.options().dtype(at::kByte));
+  return fresh({(int64_t)n}, at::kByte, like);
 }
 
 bool number(PyObject* o, double& x) {
@@ -183,7 +189,8 @@ PyObject* bsattn_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // each gradient by default [B,S,H,D]-contiguous, viewed [B,H,S,D]
   const auto grad = [&](const Arg& given, int64_t S) {
     return given ? *given
-                 : at::empty_strided({B, H, S, 128}, {S * H * 128, 128, H * 128, 1}, q->options());
+                 : at::Tensor(at::detail::empty_strided_cuda(
+                       {B, H, S, 128}, {S * H * 128, 128, H * 128, 1}, at::kBFloat16, q->device()));
   };
   const at::Tensor gq = grad(dq, Sq), gk = grad(dk, Sk), gv = grad(dv, Sk);
   const at::Tensor w = ws ? *ws : bytes(lib.bsattn_bwd_ws((int)B, (int)H, (int)Sq, (int)Sk), *q);
@@ -251,12 +258,12 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
 
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-  const at::Tensor gq = dq ? *dq : at::empty(q->sizes(), q->options());
-  const at::Tensor gk = dk ? *dk : at::empty(q->sizes(), q->options());
+  const at::Tensor gq = dq ? *dq : fresh(q->sizes(), at::kBFloat16, *q);
+  const at::Tensor gk = dk ? *dk : fresh(q->sizes(), at::kBFloat16, *q);
   at::Tensor w, gwq, gwk;
   if (wq) {
-    gwq = at::empty({hidden}, q->options().dtype(at::kFloat));
-    gwk = at::empty({hidden}, q->options().dtype(at::kFloat));
+    gwq = fresh({hidden}, at::kFloat, *q);
+    gwk = fresh({hidden}, at::kFloat, *q);
     w = ws ? *ws : bytes(lib.norm_bwd_ws((int)hidden), *q);
   }
   const int rc = without_gil([&] {
@@ -337,7 +344,7 @@ bool fits(const Arg& t, const Arg& like) {
 
 at::Tensor result(const Arg& given, const Arg& like) {
   if (given) return *given;
-  return like ? at::empty(like->sizes(), like->options()) : at::Tensor();
+  return like ? fresh(like->sizes(), like->scalar_type(), *like) : at::Tensor();
 }
 
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -379,9 +386,8 @@ PyObject* qk_head_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor rq = result(dq, h.q), rk = result(dk, h.k);
   at::Tensor w, gwq, gwk;
   if (h.wq) {
-    const auto options = h.q->options().dtype(at::kFloat);
-    gwq = at::empty({h.D}, options);
-    if (h.k) gwk = at::empty({h.D}, options);
+    gwq = fresh({h.D}, at::kFloat, *h.q);
+    if (h.k) gwk = fresh({h.D}, at::kFloat, *h.q);
     w = ws ? *ws : bytes(lib.head_bwd_ws(h.D), *h.q);
   }
   const Strides sq(*h.q), sk = h.k ? Strides(*h.k) : Strides(), tq(rq),
