@@ -1,13 +1,13 @@
 // fast.cpp — a short way from Python to the C ABI for the training operators.
 //
 // ops.py checks and lays out its arguments in Python and converts them with
-// ctypes: 17 us a call with one launch, 25-28 us with two (with its checks kept
-// from call to call). The functions here do the same for calls that need
-// nothing done: every tensor on one GPU, of the right shape and type, laid out
-// as the kernels read it. They allocate the outputs and call the library's
-// entry point: 7 and 12 us. Anything else (a tensor to copy, an argument to
-// refuse, a device without its status word) gives None, and ops.py goes the
-// long way, which copies, refuses with a message, or launches.
+// ctypes: 37 us a call with one launch, 41 to 60 us with two. The functions here
+// do the same for calls that need nothing done: every tensor on one GPU, of the
+// right shape and type, laid out as the kernels read it. They allocate the
+// outputs and call the library's entry point: 5 and 10 us. Anything else (a
+// tensor to copy, an argument to refuse, a device without its status word) gives
+// None, and ops.py goes the long way, which copies, refuses with a message, or
+// launches.
 //
 // The entry points' addresses come from ops.py (bind), so that there is one
 // loaded library, whichever was loaded.
