@@ -42,6 +42,7 @@ constexpr int kStatBytes = 2 * kT * 4;         // -lse (log2 units) and -delta o
 constexpr int kMaxBlocks = 1024;               // per mask row or column (S <= 131072)
 constexpr int kLeastPiece = 8;                 // blocks
 constexpr int kJoin = 8;                       // pieces added up at a time
+constexpr int kFewTiles = 4;                   // per SM
 constexpr int kListReaders = 2 + kWorkers;
 constexpr uint32_t kColX = 0, kColY = 128, kColAcc1 = 256, kColAcc2 = 384;
 
@@ -123,6 +124,7 @@ struct __align__(16) SmemCtl {
   uint64_t ds_full[2];   // [block parity] dS written over Y, kWorkers arrivals
   uint64_t acc_full;     // a tile's sums are complete (commit)
   uint64_t acc_free;     // a tile's sums have been read, kWorkers arrivals
+  uint64_t claim;        // the producer has issued an item's last loads
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
@@ -331,14 +333,21 @@ __device__ __forceinline__ void split_bf16x2(float x0, float x1, uint32_t& hi, u
 // halves, each a product of its own in the columns that X and Y leave free.
 // The launch takes it where the blocks do not fill the GPU once and the extra
 // products hide behind latencies (300 tokens, 2 heads: 12.1 us become 13.0).
-// CUT: tiles may be cut into pieces. Without that code a launch of a few tiles is
-// 2 us shorter (300 tokens, 2 heads, cold caches: 19.3 and 17.4 us).
-template <bool FINE, bool CUT>
+// MODE: what may happen to the tiles. Compiled apart, as code that a launch does
+// not need costs it time: 2 us of 300 tokens, 2 heads (cold caches: 19.3 and 17.4
+// us), 0.6% of long ones.
+enum Mode {
+  kPlain,  // nothing
+  kFew,    // few tiles, none cut
+  kCut     // tiles may be cut into pieces, and may be few
+};
+template <bool FINE, Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     bsattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                       const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ CUtensorMap tm_do, const Params p) {
+  constexpr bool CUT = MODE == kCut;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* a_tile = smem;                       // A1, A2
   uint8_t* b1_ring = smem + 2 * kTileBytes;
@@ -369,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&ctl->x_done[1], kWorkers);
     mbar_init(&ctl->acc_full, 1);
     mbar_init(&ctl->acc_free, kWorkers);
+    mbar_init(&ctl->claim, 1);
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     fence_barrier_init();
@@ -434,11 +444,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         before_lane[q] = sum - own;
       }
     }
+    // With many tiles the next item is claimed as soon as a slot is free, which
+    // hides the way from the counter to its first tiles best. With few, that
+    // gives every CTA its second tile at the start; so it is claimed once the
+    // loads of the one before are issued, and where tiles are counted the long
+    // ones are taken first. Up to four per SM: 2 heads of 8192 tokens 65.4 -> 59.8
+    // us, 24 heads of 1024 47.1 -> 44.6; beyond: 4680 x 500 tokens 95.9 -> 99.9,
+    // 30 heads of 4096 242 -> 254.
+    const int all = p.tiles[0] + p.tiles[1];
+    const bool few = MODE == kFew || (CUT && all <= kFewTiles * (int)gridDim.x);
+    const bool by_length = CUT && few && p.counts[0] != nullptr && p.counts[1] != nullptr;
     int dealt = blockIdx.x;  // this CTA's next extra piece
     for (int k = 0;; ++k) {
       const int slot = k & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(&ctl->list_empty[slot], ((uint32_t)(k >> 1) & 1u) ^ 1u,
                                              p.status, abort_flag)))
+        break;
+      if (few && k > 0 &&
+          !__all_sync(0xffffffffu, mbar_wait(&ctl->claim, (uint32_t)(k - 1) & 1u, p.status,
+                                             abort_flag)))
         break;
       Item w;
       w.n = -1;
@@ -476,20 +500,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         w.first = first;
         dealt += gridDim.x;
       } else {
-        int it = 0;
-        if (lane == 0) it = atomicAdd(p.next_item, 1);
-        it = __shfl_sync(0xffffffffu, it, 0);
-        if (it < p.tiles[0] + p.tiles[1]) {
-          w.kind = it >= p.tiles[0] ? 1 : 0;
-          tile = it - (w.kind ? p.tiles[0] : 0);
-          const int* counts = w.kind ? p.counts[1] : p.counts[0];
-          if (CUT && (w.kind ? extra[1] : extra[0]) > 0 && counts[tile] >= 2 * least) {
-            const int width = w.kind ? span[1] : span[0], owner = tile / width;
-            int sum = 0;
-            for (int i = owner * width + lane; i < tile; i += 32) sum += extras_of(counts[i]);
-            w.first = __shfl_sync(0xffffffffu, w.kind ? before_lane[1] : before_lane[0], owner) +
-                      __reduce_add_sync(0xffffffffu, sum);
+        for (;;) {
+          int it = 0;
+          if (lane == 0) it = atomicAdd(p.next_item, 1);
+          it = __shfl_sync(0xffffffffu, it, 0);
+          if (it >= (by_length ? 2 * all : all)) break;
+          const bool second = by_length && it >= all;
+          if (second) it -= all;
+          const int kind = it >= p.tiles[0] ? 1 : 0;
+          tile = it - (kind ? p.tiles[0] : 0);
+          const bool maybe_cut = (kind ? extra[1] : extra[0]) > 0;
+          if (CUT && (by_length || maybe_cut)) {
+            const int* counts = kind ? p.counts[1] : p.counts[0];
+            const int count = counts[tile];
+            if (by_length && (count >= least) == second) continue;
+            if (maybe_cut && count >= 2 * least) {
+              const int width = kind ? span[1] : span[0], owner = tile / width;
+              int sum = 0;
+              for (int i = owner * width + lane; i < tile; i += 32) sum += extras_of(counts[i]);
+              w.first = __shfl_sync(0xffffffffu, kind ? before_lane[1] : before_lane[0], owner) +
+                        __reduce_add_sync(0xffffffffu, sum);
+            }
           }
+          w.kind = kind;
+          break;
         }
       }
       if (w.kind >= 0) {
@@ -626,6 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
         if (n > 0) ++e;
+        if (MODE != kPlain) mbar_arrive(&ctl->claim);
         mbar_arrive(&ctl->list_empty[slot]);
       }
       // no copy of this CTA may be in flight when it exits
@@ -1139,8 +1174,11 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
   p.max_extra = l.max_extra;
 
   const bool fine = (int64_t)nq * nk * B * H <= sms;
-  const auto kernel = fine ? cut ? bsattn_bwd_kernel<true, true> : bsattn_bwd_kernel<true, false>
-                           : cut ? bsattn_bwd_kernel<false, true> : bsattn_bwd_kernel<false, false>;
+  const int64_t tiles = (int64_t)p.tiles[0] + p.tiles[1];
+  const bool few = tiles > sms && tiles <= kFewTiles * sms;
+  const auto kernel = fine ? cut ? bsattn_bwd_kernel<true, kCut> : bsattn_bwd_kernel<true, kPlain>
+                      : cut ? bsattn_bwd_kernel<false, kCut>
+                      : few ? bsattn_bwd_kernel<false, kFew> : bsattn_bwd_kernel<false, kPlain>;
   if ((rc = sa::func_attr_once((const void*)kernel,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes)) !=
       SA_OK)
@@ -1157,7 +1195,6 @@ extern "C" int sa_bsattn_bwd(const void* dout, const void* q, const void* k, con
       dlse, H, Sq, nq * kT, nstat, p.stat_plane, p.next_item, p.joined[0], l.n_joined,
       counts[0], counts[1], eights, p.mask, B, nk, status));
   // one CTA per SM; fewer only where there are fewer tiles and none may be cut
-  const int64_t tiles = (int64_t)p.tiles[0] + p.tiles[1];
   SA_CUDA_TRY(sa::launch_after(kernel, dim3((unsigned)(cut || tiles > sms ? sms : tiles)),
                                dim3(kThreads), kSmemBytes, stream, tq, tk, tv, td, p));
   return SA_OK;

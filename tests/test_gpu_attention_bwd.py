@@ -135,6 +135,15 @@ def test_tiles_longer_than_a_share_of_the_gpu(B, H, Sq, Sk):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("B,H,Sq,Sk", [(1, 24, 700, 900), (3, 9, 1024, 513), (1, 4, 2500, 2300)])
+@pytest.mark.parametrize("empty", [0.0, 0.4])
+def test_a_few_tiles_for_each_processor(B, H, Sq, Sk, empty):
+    q, k, v, dout, mask = make(B, H, Sq, Sk, 0.4, Sq, empty=empty)
+    got = both(q, k, v, dout, mask)
+    for x, y in zip(got, run(q, k, v, dout, mask)):
+        assert torch.equal(x, y)
+
+
 def test_long_tiles_of_one_kind_among_many_of_the_other():
     """140 heads of 17 x 16 blocks; all but the first keep nothing: its key tiles may be cut,
     its query tiles are too many to."""
