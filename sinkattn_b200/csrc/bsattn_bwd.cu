@@ -454,6 +454,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int all = p.tiles[0] + p.tiles[1];
     const bool few = MODE == kFew || (CUT && all <= kFewTiles * (int)gridDim.x);
     const bool by_length = CUT && few && p.counts[0] != nullptr && p.counts[1] != nullptr;
+    // With two tiles per SM and few pieces, the SMs that add a tile's pieces up are
+    // the last to finish their first item, so they claim the next one, if any is
+    // left, only then: 4 heads of 4096 44.0 -> 37.9 us, one of 16384 66.6 -> 58.6.
+    // Where most items are pieces all would wait (+3%).
+    const bool piece_alone = CUT && all <= 2 * (int)gridDim.x &&
+                             2 * (extra[0] + extra[1]) <= (int)gridDim.x;
+    bool was_piece = false;
     int dealt = blockIdx.x;  // this CTA's next extra piece
     for (int k = 0;; ++k) {
       const int slot = k & 1;
@@ -463,6 +470,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (few && k > 0 &&
           !__all_sync(0xffffffffu, mbar_wait(&ctl->claim, (uint32_t)(k - 1) & 1u, p.status,
                                              abort_flag)))
+        break;
+      if (piece_alone && was_piece &&
+          *reinterpret_cast<volatile int*>(p.next_item) < (by_length ? 2 * all : all) &&
+          !__all_sync(0xffffffffu, mbar_wait(&ctl->list_empty[slot ^ 1],
+                                             (uint32_t)((k - 1) >> 1) & 1u, p.status, abort_flag)))
         break;
       Item w;
       w.n = -1;
@@ -572,6 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           count = hi - lo;
         }
+        was_piece = w.pieces > 1;
         w.n = count;
         const int64_t row = (int64_t)w.blk * kT;
         w.rows = (kind ? p.Sq : p.Sk) - (int)row;
