@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) bwd_kernel(const Params p) {
           const float ss = group_sum<G>(sum2(s2)), dot = group_sum<G>(sum2(t2));
           float r = inv_sqrt<T>(fmaf(ss, inv_d, p.eps));
           if (tk.bad) r = __int_as_float(0x7fc00000);
-          const float m = -r * r * r * dot * inv_d;
+          // the dot product first: r^3 alone leaves fp32 where x is about 1e14 or 1e-13
+          const float m = -(r * dot * inv_d) * r * r;
           const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
           if (on && h < hd.end) {
             V8 o;
