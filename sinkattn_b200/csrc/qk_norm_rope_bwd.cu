@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(MAXT, 768 / MAXT) kernel(const Params p) {
       const float dt = __shfl_sync(0xffffffffu, t, 2 * i + 1);
       float r = inv_sqrt<__nv_bfloat16>(fmaf(sq, inv_n, p.eps));
       if (!there) r = __int_as_float(0x7fc00000);
-      const float m = -r * r * r * dt * inv_n;
+      // the dot product first: r^3 alone leaves fp32 where x is about 1e14 or 1e-13
+      const float m = -(r * dt * inv_n) * r * r;
       const uint64_t r2 = f2_pack(r, r), m2 = f2_pack(m, m);
       V8 o;
 #pragma unroll

@@ -7,7 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_norm_grad import both, make
+from tests.test_gpu_norm_grad import backward_ref, both, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,27 @@ def test_head_norm_gradient_of_zero_rows_beside_a_small_eps():
     a["q"][0, 2] = 0
     a["k"][0, 4, 1] = 0
     both(a, w, cos, sin, pos, True, 1e-28)
+
+
+@pytest.mark.parametrize("size,eps", [(1e14, 1e-6), (1e15, 1e-6), (1e17, 1e-6), (1e-13, 0.0),
+                                      (1e-17, 0.0)])
+def test_hidden_norm_gradient_of_very_large_and_very_small_rows(size, eps):
+    from sinkattn_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(33)
+    B, S, hidden, D = 2, 21, 512, 128
+
+    def t(scale):
+        return (torch.randn(B, S, hidden, generator=g, device="cuda") * scale).bfloat16()
+
+    q, k, dq, dk = t(size), t(size), t(1.0), t(1.0)
+    w = [(1 + 0.3 * torch.randn(hidden, generator=g, device="cuda")) for _ in range(2)]
+    ang = torch.rand(S, D // 2, generator=g, device="cuda", dtype=torch.float64) * 6.3
+    cos, sin = torch.cos(ang).float(), torch.sin(ang).float()
+    got = ops.qk_norm_rope_bwd(dq, dk, q, k, D, eps, w[0], w[1], cos, sin)
+    split = (B, S, hidden // D, D)
+    for i, (d, x) in enumerate(((dq, q), (dk, k))):
+        dx, bx, dw, bw = backward_ref(d.view(split), x.view(split), w[i].view(hidden // D, D), eps,
+                                      cos, sin, None, True, over=2)
+        check("dx", got[i].view(split), dx, bx)
+        check("dw", got[2 + i].view(hidden // D, D), dw, bw)
