@@ -325,6 +325,8 @@ def _bsattn_bwd_plan(dout, q, k, v, out, lse, block_mask, softmax_scale, head_ma
         raise RuntimeError("bsattn_bwd expects 4-D [B,H,S,D] tensors")
     B, H, Sq, D = q.shape
     Sk = k.shape[2]
+    if D != BLOCK:  # before the layouts: no copy mends a size
+        raise RuntimeError(f"bsattn_bwd: head dim must be 128, got {D}")
     for name, t, S in (("dout", dout, Sq), ("q", q, Sq), ("k", k, Sk), ("v", v, Sk),
                        ("out", out, Sq), ("dq", dq, Sq), ("dk", dk, Sk), ("dv", dv, Sk)):
         if t is None:
@@ -1078,6 +1080,10 @@ def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, w_q, w_k, cos, sin, d
     if q.dim() != 3:
         raise RuntimeError("qk_norm_rope_bwd expects [B, S, hidden] tensors")
     B, S, hidden = q.shape
+    # before the layouts: no copy mends a size
+    if head_dim < 8 or head_dim % 8 or hidden < 8 or hidden % head_dim:
+        raise RuntimeError(f"qk_norm_rope_bwd: hidden ({hidden}) must be a multiple of head_dim "
+                           f"({head_dim}), and that of 8")
     for name, t in (("dq_out", dq_out), ("dk_out", dk_out), ("q", q), ("k", k), ("dq", dq),
                     ("dk", dk)):
         if t is not None and (t.dtype != torch.bfloat16 or t.shape != (B, S, hidden)):
@@ -1128,6 +1134,8 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
     Hk = 0 if k is None else k.shape[2]
     if q.dtype not in _DTYPES:
         raise RuntimeError(f"{fn} expects bf16, fp16 or fp32, got {q.dtype}")
+    if D < 8 or D > 256 or D % 8:  # before the layouts: no copy mends a size
+        raise RuntimeError(f"{fn}: head dim must be a multiple of 8 up to 256, got {D}")
     if k is not None and (k.dtype != q.dtype or k.shape != (B, S, Hk, D) or Hk == 0):
         raise RuntimeError(f"{fn}: k must be {q.dtype} [{B}, {S}, heads, {D}], got {k.dtype} "
                            f"{tuple(k.shape)}")
@@ -1169,6 +1177,10 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
                                f", got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} "
                                f"{tuple(sin.shape)}")
         rows, rot = cos.shape[0], 2 * cos.shape[1]
+        of = 8 if interleaved else 16
+        if rot < 8 or rot > D or rot % of:
+            raise RuntimeError(f"{fn}: the rotated channels must be a multiple of {of} up to D, got "
+                               f"{rot}")
         if rows == 0 and q.numel():
             raise RuntimeError(f"{fn}: cos and sin have no rows")
         fs = cos.stride(0) if rows > 1 else (rot // 2 + 3) // 4 * 4

@@ -54,3 +54,36 @@ def test_hidden_norm_gradient_of_very_large_and_very_small_rows(size, eps):
                                       cos, sin, None, True, over=2)
         check("dx", got[i].view(split), dx, bx)
         check("dw", got[2 + i].view(hidden // D, D), dw, bw)
+
+
+def test_sizes_that_no_copy_can_fit_are_refused():
+    """Contiguous tensors: the layout is not what is wrong with them."""
+    from sinkattn_b200 import ops
+
+    def t(*s, dtype=torch.bfloat16):
+        return torch.ones(*s, dtype=dtype, device="cuda")
+
+    for D, dtype in ((100, torch.bfloat16), (12, torch.float16), (12, torch.float32),
+                     (6, torch.float32), (264, torch.bfloat16)):
+        x = t(2, 5, 3, D, dtype=dtype)
+        with pytest.raises(RuntimeError, match="multiple of 8 up to 256"):
+            ops.qk_head_norm_rope(x, x, 1e-6)
+        with pytest.raises(RuntimeError, match="multiple of 8 up to 256"):
+            ops.qk_head_norm_rope_bwd(x, x, x, x, 1e-6)
+    x, f = t(2, 5, 3, 128), torch.float32
+    for half, inter, match in ((6, True, "multiple of 8 up to"), (0, True, "multiple of 8 up to"),
+                               (4, False, "multiple of 16 up to"), (68, True, "multiple of 8 up to")):
+        c = t(5, half, dtype=f)
+        with pytest.raises(RuntimeError, match=match):
+            ops.qk_head_norm_rope(x, x, 1e-6, cos=c, sin=c, interleaved=inter)
+        with pytest.raises(RuntimeError, match=match):
+            ops.qk_head_norm_rope_bwd(x, x, x, x, 1e-6, cos=c, sin=c, interleaved=inter)
+    for hidden, D in ((100, 100), (12, 12), (4104, 8), (256, 96)):
+        x = t(2, 5, hidden)
+        with pytest.raises(RuntimeError, match="hidden"):
+            ops.qk_norm_rope_bwd(x, x, x, x, D, 1e-6)
+    lse, mask = torch.zeros(1, 2, 130, device="cuda"), t(1, 2, 2, 2, dtype=torch.bool)
+    for D in (100, 64, 136):
+        x = t(1, 2, 130, D)
+        with pytest.raises(RuntimeError, match="head dim must be 128"):
+            ops.bsattn_bwd(x, x, x, x, x, lse, mask)

@@ -1,0 +1,50 @@
+"""Host-side refusals of the training operators that need no GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def on_device(monkeypatch):
+    """ops as it is on a GPU, up to the first look at the device."""
+    from sinkattn_b200 import ops
+
+    monkeypatch.setattr(ops, "_require_cuda", lambda *ts: torch.device("cuda", 0))
+    monkeypatch.setattr(ops, "_short", lambda *a: None)
+    return ops
+
+
+@pytest.mark.parametrize("D,dtype", [(100, torch.bfloat16), (12, torch.float32), (4, torch.float32),
+                                     (264, torch.float16)])
+def test_head_sizes_are_refused_whatever_the_layout(on_device, D, dtype):
+    x = torch.zeros(2, 5, 3, D, dtype=dtype)
+    for call in (lambda: on_device.qk_head_norm_rope(x, x, 1e-6),
+                 lambda: on_device.qk_head_norm_rope_bwd(x, x, x, x, 1e-6)):
+        with pytest.raises(RuntimeError, match="multiple of 8 up to 256"):
+            call()
+
+
+@pytest.mark.parametrize("half,inter,of", [(6, True, 8), (0, True, 8), (4, False, 16), (36, True, 8)])
+def test_rotated_sizes_are_refused_whatever_the_layout(on_device, half, inter, of):
+    x, c = torch.zeros(2, 5, 3, 64), torch.zeros(5, half)
+    for call in (lambda: on_device.qk_head_norm_rope(x, x, 1e-6, cos=c, sin=c, interleaved=inter),
+                 lambda: on_device.qk_head_norm_rope_bwd(x, x, x, x, 1e-6, cos=c, sin=c,
+                                                         interleaved=inter)):
+        with pytest.raises(RuntimeError, match=f"multiple of {of} up to D"):
+            call()
+
+
+@pytest.mark.parametrize("hidden,D", [(100, 100), (12, 12), (256, 96), (4, 4), (256, 0)])
+def test_hidden_sizes_are_refused_whatever_the_layout(on_device, hidden, D):
+    x = torch.zeros(2, 5, hidden, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="hidden"):
+        on_device.qk_norm_rope_bwd(x, x, x, x, D, 1e-6)
+
+
+@pytest.mark.parametrize("D", [64, 100, 136])
+def test_attention_head_sizes_are_refused_whatever_the_layout(on_device, D):
+    x = torch.zeros(1, 2, 130, D, dtype=torch.bfloat16)
+    mask = torch.ones(1, 2, 2, 2, dtype=torch.bool)
+    with pytest.raises(RuntimeError, match="head dim must be 128"):
+        on_device.bsattn_bwd(x, x, x, x, x, torch.zeros(1, 2, 130), mask)
