@@ -63,9 +63,10 @@ def _as_kernel_layout(t: torch.Tensor) -> torch.Tensor:
 
 def _strides16_ok(t: torch.Tensor) -> bool:
     """Whole 16-byte vectors along the last dimension, and from element to
-    element of the others (a dimension of size 1 is never stepped along)."""
+    element of the others (a dimension of size 1 is never stepped along, and
+    nothing of an empty tensor is)."""
     n = 16 // t.element_size()
-    return t.stride(-1) == 1 and not any(
+    return t.numel() == 0 or t.stride(-1) == 1 and not any(
         s % n for s, size in zip(t.stride()[:-1], t.shape[:-1]) if size > 1)
 
 
@@ -1066,7 +1067,9 @@ def _row_stride(t: torch.Tensor) -> Optional[int]:
     """The one stride at which the B * S rows of [B, S, hidden] lie, in whole
     16-byte vectors; None if there is none."""
     B, S, hidden = t.shape
-    if t.numel() == 0 or B * S == 1:
+    if t.numel() == 0:
+        return hidden
+    if B * S == 1:
         st = hidden
     elif S == 1:
         st = t.stride(0)
@@ -1185,7 +1188,7 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
             raise RuntimeError(f"{fn}: cos and sin have no rows")
         fs = cos.stride(0) if rows > 1 else (rot // 2 + 3) // 4 * 4
         fits = fits and _strides16_ok(cos) and _strides16_ok(sin) and (
-            rows == 1 or fs == sin.stride(0) >= rot // 2)
+            rows <= 1 or fs == sin.stride(0) >= rot // 2)
     pst = None
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \

@@ -87,3 +87,22 @@ def test_sizes_that_no_copy_can_fit_are_refused():
         x = t(1, 2, 130, D)
         with pytest.raises(RuntimeError, match="head dim must be 128"):
             ops.bsattn_bwd(x, x, x, x, x, lse, mask)
+
+
+def test_views_of_nothing():
+    from sinkattn_b200 import ops
+
+    bf = torch.bfloat16
+    odd = torch.zeros(2, 4, 3, 131, dtype=bf, device="cuda")[:, :0, :, 1:129]
+    wide, w = torch.zeros(5, 70, device="cuda")[:0, 2:66], torch.ones(128, device="cuda")
+    q, k = ops.qk_head_norm_rope(odd, odd, 1e-6, w, w, wide, wide)
+    assert q.shape == k.shape == (2, 0, 3, 128)
+    dq, dk, dwq, dwk = ops.qk_head_norm_rope_bwd(odd, odd, odd, odd, 1e-6, w, w, wide, wide)
+    assert dq.shape == dk.shape == (2, 0, 3, 128) and not dwq.any() and not dwk.any()
+    turned, w = torch.zeros(0, 256, 2, dtype=bf, device="cuda").permute(0, 2, 1), w.repeat(2)
+    dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(turned, turned, turned, turned, 128, 1e-6, w, w)
+    assert dq.shape == dk.shape == (0, 2, 256) and not dwq.any() and not dwk.any()
+    none = torch.zeros(1, 2, 4, 133, dtype=bf, device="cuda")[:, :, :0, 3:131]
+    with pytest.raises(RuntimeError, match="SA_EINVAL"):
+        ops.bsattn_bwd(none, none, none, none, none, torch.zeros(1, 2, 0, device="cuda"),
+                       torch.zeros(1, 2, 0, 0, dtype=torch.bool, device="cuda"))

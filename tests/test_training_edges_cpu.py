@@ -48,3 +48,27 @@ def test_attention_head_sizes_are_refused_whatever_the_layout(on_device, D):
     mask = torch.ones(1, 2, 2, 2, dtype=torch.bool)
     with pytest.raises(RuntimeError, match="head dim must be 128"):
         on_device.bsattn_bwd(x, x, x, x, x, torch.zeros(1, 2, 130), mask)
+
+
+def test_views_of_nothing_need_no_copy(on_device, monkeypatch):
+    """An empty tensor's strides may be anything, and contiguous() leaves them."""
+    from contextlib import nullcontext
+
+    ops = on_device
+    launched = []
+    monkeypatch.setattr(ops, "_launch", lambda idx, name, fn, *a: launched.append(name))
+    monkeypatch.setattr(ops.DeviceStatus, "pointer", classmethod(lambda cls, dev: 0))
+    monkeypatch.setattr(ops, "_check_workspace", lambda *a: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: nullcontext())
+    bf = torch.bfloat16
+    odd = torch.zeros(2, 4, 3, 131, dtype=bf)[:, :0, :, 1:129]
+    turned = torch.zeros(0, 256, 2, dtype=bf).permute(0, 2, 1)
+    wide = torch.zeros(5, 70)[:0, 2:66]
+    ops.qk_head_norm_rope(odd, odd, 1e-6, cos=wide, sin=wide)
+    ops.qk_head_norm_rope_bwd(odd, odd, odd, odd, 1e-6, cos=wide, sin=wide)
+    ops.qk_norm_rope_bwd(turned, turned, turned, turned, 128, 1e-6)
+    none = torch.zeros(1, 2, 4, 133, dtype=bf)[:, :, :0, 3:131]
+    ops.bsattn_bwd(none, none, none, none, none, torch.zeros(1, 2, 0),
+                   torch.zeros(1, 2, 0, 0, dtype=torch.bool), workspace=torch.zeros(0))
+    assert launched == ["sa_qk_head_norm_rope", "sa_qk_head_norm_rope_bwd", "sa_qk_norm_rope_bwd",
+                        "sa_bsattn_bwd"]
