@@ -91,7 +91,8 @@ SA_API int sa_device_sm_count(void);
  *   and value 0 => head h is dense (all blocks). Negative values (streaming
  *   heads upstream) are not supported; the library never reads device
  *   memory on the host, so the Python layer rejects them before the call and
- *   the kernel treats them as dense.
+ *   the kernel treats them as dense. A value t > Hm is not followed either: the
+ *   head is computed dense and *status becomes SA_DEV_BAD_INDEX.
  * softmax_scale: <= 0 selects 1/sqrt(D).
  * lse: nullable fp32 [B,H,Sq] contiguous, natural-log logsumexp per row. Rows
  *   whose mask row keeps no block produce out = 0 and lse = -inf.
@@ -149,10 +150,9 @@ SA_API int sa_sink_dynamic_attn_fwd(
  *   to lse. dq, dk and dv are written whole: rows whose mask row (key blocks
  *   whose mask column) keeps nothing get 0, whatever their lse and dout hold.
  * block_mask, m_strides, Hm, head_mask_type, softmax_scale, status: as for
- *   sa_bsattn_fwd (an entry t > Hm is not followed: the head is computed dense
- *   and *status becomes SA_DEV_BAD_INDEX). Sq, Sk <= 131072. P and dS enter
- *   their products as bf16 (as two bf16 halves each where the call has no more
- *   blocks than the GPU has SMs); the sums, dP and the row statistics are fp32.
+ *   sa_bsattn_fwd. Sq, Sk <= 131072. P and dS enter their products as bf16 (as
+ *   two bf16 halves each where the call has no more blocks than the GPU has
+ *   SMs); the sums, dP and the row statistics are fp32.
  * Sums are formed in block order, those of long mask lines in pieces that are
  *   added in a fixed order (no atomics on data), so equal calls give equal bits.
  * workspace: sa_bsattn_bwd_workspace_size(B, H, Sq, Sk) bytes, 256-byte

@@ -77,6 +77,7 @@ struct Params {
   const uint8_t* mask;
   int64_t ms0, ms1, ms2, ms3;
   const int32_t* head_mask_type;
+  int mask_heads;
   float scale_log2;  // softmax_scale * log2(e)
   const __nv_bfloat16* q;
   int64_t qs0, qs1, qs2;
@@ -237,7 +238,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool dense = false;
       if (p.head_mask_type != nullptr) {
         const int ty = p.head_mask_type[h];
-        if (ty > 0) mh = ty - 1; else dense = true;
+        // an entry past the mask's heads has no slice to read: dense, and reported
+        dense = ty <= 0 || ty > p.mask_heads;
+        if (!dense) mh = ty - 1;
+        else if (ty > 0 && lane == 0) report_status(p.status, SA_DEV_BAD_INDEX);
       }
       const uint8_t* row =
           p.mask + (int64_t)b * p.ms0 + (int64_t)mh * p.ms1 + (int64_t)qt * p.ms2;
@@ -763,6 +767,7 @@ int launch_attention(const char* fn, const void* q, const void* k, const void* v
   p.mask = block_mask;
   p.ms0 = m_strides[0]; p.ms1 = m_strides[1]; p.ms2 = m_strides[2]; p.ms3 = m_strides[3];
   p.head_mask_type = head_mask_type;
+  p.mask_heads = Hm;
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf((float)D);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);

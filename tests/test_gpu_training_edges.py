@@ -7,6 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from tests.test_gpu_attention_bwd import make as make_attn
 from tests.test_gpu_norm_grad import backward_ref, both, check, make
 
 pytestmark = pytest.mark.gpu
@@ -106,3 +107,34 @@ def test_views_of_nothing():
     with pytest.raises(RuntimeError, match="SA_EINVAL"):
         ops.bsattn_bwd(none, none, none, none, none, torch.zeros(1, 2, 0, device="cuda"),
                        torch.zeros(1, 2, 0, 0, dtype=torch.bool, device="cuda"))
+
+
+def test_the_forward_pass_reports_head_mask_type_past_the_mask():
+    """Such a head is dense in both directions; nothing past the mask is read."""
+    from sinkattn_b200 import ops
+    from sinkattn_b200.autograd import block_sparse_attention
+
+    q, k, v, dout, mask = make_attn(2, 3, 300, 400, 0.5, 41)
+    mask = mask[:, :2]
+    good = torch.tensor([1, 2, 0], dtype=torch.int32, device="cuda")
+    for past in (3, 4, 2 ** 31 - 1):
+        bad = torch.tensor([1, 2, past], dtype=torch.int32, device="cuda")
+        calls = (lambda t: ops.bsattn_fwd(q, k, v, mask, head_mask_type=t),
+                 lambda t: ops.sink_dynamic_attn(q, k, v, mask, k[:, :, :90], v[:, :, :90], 4,
+                                                 head_mask_type=t, return_lse=True))
+        for call in calls:
+            want, got = call(good), call(bad)
+            with pytest.raises(RuntimeError, match="head_mask_type entry"):
+                ops.DeviceStatus.check()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+        grads = []
+        for t in (good, bad):
+            leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+            out, _ = block_sparse_attention(*leaves, mask, head_mask_type=t)
+            grads.append(torch.autograd.grad(out, leaves, dout))
+        with pytest.raises(RuntimeError, match="head_mask_type entry"):
+            ops.DeviceStatus.check()
+        for a, b in zip(*grads):
+            assert torch.equal(a, b)
+    ops.DeviceStatus.check()
