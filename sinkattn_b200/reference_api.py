@@ -28,6 +28,7 @@ import sys
 from typing import Optional
 
 import torch
+from torch.utils.weak import WeakIdKeyDictionary
 
 from . import autograd, ops
 
@@ -65,16 +66,17 @@ def _reports_device_failures(fn):
 
 
 def _hmt_host(head_mask_type: torch.Tensor) -> list[int]:
-    # small int32 [H]; cached on the tensor's identity and version counter
+    # small int32 [H]; kept with the tensor object, as an address may come to hold another's
+    # entries, until its version counter or its memory changes
     key = (head_mask_type.data_ptr(), head_mask_type._version, head_mask_type.numel())
-    cached = _HMT_CACHE.get(key)
-    if cached is None:
-        cached = [int(x) for x in head_mask_type.detach().cpu().tolist()]
-        _HMT_CACHE[key] = cached
-    return cached
+    kept = _HMT_CACHE.get(head_mask_type)
+    if kept is None or kept[0] != key:
+        kept = (key, [int(x) for x in head_mask_type.detach().cpu().tolist()])
+        _HMT_CACHE[head_mask_type] = kept
+    return kept[1]
 
 
-_HMT_CACHE: dict = {}
+_HMT_CACHE = WeakIdKeyDictionary()
 
 
 @_reports_device_failures

@@ -72,3 +72,22 @@ def test_views_of_nothing_need_no_copy(on_device, monkeypatch):
                    torch.zeros(1, 2, 0, 0, dtype=torch.bool), workspace=torch.zeros(0))
     assert launched == ["sa_qk_head_norm_rope", "sa_qk_head_norm_rope_bwd", "sa_qk_norm_rope_bwd",
                         "sa_bsattn_bwd"]
+
+
+def test_head_mask_type_of_another_tensor_is_read_anew():
+    """Two tensors at one address, as a freed one and the next of its size: the second's entries
+    count."""
+    import numpy as np
+
+    from sinkattn_b200.reference_api import _hmt_host
+
+    memory = np.array([1, 0, 2], dtype=np.int32)
+    t = torch.from_numpy(memory)
+    assert _hmt_host(t) == [1, 0, 2]
+    memory[:] = [0, -1, 1]
+    u = torch.from_numpy(memory)
+    assert u.data_ptr() == t.data_ptr() and u._version == t._version
+    assert _hmt_host(u) == [0, -1, 1]
+    u[0] = 3
+    assert _hmt_host(u) == [3, -1, 1]
+    assert _hmt_host(u) is _hmt_host(u)  # the same tensor, unchanged, is not copied again
