@@ -118,16 +118,14 @@ def block_sparse_attn_func(
     B = int(cu_seqlens_q.numel()) - 1
     Sq, Sk = int(max_seqlen_q_), int(max_seqlen_k_)
     hmt = None
-    if HEAD_MASK_TYPE_MODE == "upstream":
+    # fewer mask slices than heads only makes sense with the mapping
+    if HEAD_MASK_TYPE_MODE == "upstream" or base_blockmask.shape[1] != H:
         hv = _hmt_host(head_mask_type)
         if any(t < 0 for t in hv):
             raise NotImplementedError("sinkattn_b200: streaming heads (head_mask_type < 0)")
-        hmt = head_mask_type.to(torch.int32)
-    elif base_blockmask.shape[1] != H:
-        # fewer mask slices than heads only makes sense with the mapping
-        hv = _hmt_host(head_mask_type)
-        if any(t < 0 for t in hv):
-            raise NotImplementedError("sinkattn_b200: streaming heads (head_mask_type < 0)")
+        if max(hv, default=0) > base_blockmask.shape[1]:
+            raise ValueError(f"head_mask_type names mask slice {max(hv)} of "
+                             f"{base_blockmask.shape[1]}")
         hmt = head_mask_type.to(torch.int32)
     record = autograd.needs_grad(q_unpad, k_unpad, v_unpad)
     if total_q == B * Sq and total_k == B * Sk and record:

@@ -91,3 +91,18 @@ def test_head_mask_type_of_another_tensor_is_read_anew():
     u[0] = 3
     assert _hmt_host(u) == [3, -1, 1]
     assert _hmt_host(u) is _hmt_host(u)  # the same tensor, unchanged, is not copied again
+
+
+@pytest.mark.parametrize("mode,heads", [("per_head", 2), ("upstream", 2), ("upstream", 3)])
+def test_head_mask_type_past_the_mask_is_refused(monkeypatch, mode, heads):
+    from sinkattn_b200 import reference_api
+
+    monkeypatch.setattr(reference_api, "HEAD_MASK_TYPE_MODE", mode)
+    q = torch.zeros(200, 3, 128, dtype=torch.bfloat16)
+    cu = torch.tensor([0, 200], dtype=torch.int32)
+    mask = torch.ones(1, heads, 2, 2, dtype=torch.bool)
+    hmt = torch.tensor([1, 0, heads + 1], dtype=torch.int32)
+    for grad in (False, True):
+        with pytest.raises(ValueError, match=f"head_mask_type names mask slice {heads + 1} of {heads}"):
+            reference_api.block_sparse_attn_func(q.requires_grad_(grad), q, q, cu, cu, hmt, None,
+                                                 mask, 200, 200)
