@@ -401,13 +401,13 @@ def sink_dynamic_attn(
             raise RuntimeError("sink_dynamic_attn expects 4-D bf16 tensors")
     B, H, Sq, D = q.shape
     Sk, Skp = k.shape[2], k_pool.shape[2]
+    if k.shape != (B, H, Sk, D) or v.shape != (B, H, Sk, D):
+        raise RuntimeError("sink_dynamic_attn: k and v must be [B,H,Sk,D] of q's B, H and D")
     if k_pool.shape != (B, H, Skp, D) or v_pool.shape != (B, H, Skp, D):
         raise RuntimeError("k_pool / v_pool must be [B,H,Sk_pool,D]")
-    nq, nk = math.ceil(Sq / BLOCK), math.ceil(Sk / BLOCK)
-    if block_mask.dim() != 4 or block_mask.shape[-2:] != (nq, nk) or block_mask.shape[0] not in (1, B):
-        raise RuntimeError(f"block_mask must be [B|1, Hm, {nq}, {nk}], got {tuple(block_mask.shape)}")
     if head_mask_type is not None:
-        head_mask_type = head_mask_type.to(torch.int32).contiguous()
+        head_mask_type = head_mask_type.to(torch.int32)
+    head_mask_type = _check_block_mask("sink_dynamic_attn", block_mask, head_mask_type, B, H, Sq, Sk)
     q, k, v = _as_kernel_layout(q), _as_kernel_layout(k), _as_kernel_layout(v)
     k_pool, v_pool = _as_kernel_layout(k_pool), _as_kernel_layout(v_pool)
     if out is None:

@@ -106,3 +106,19 @@ def test_head_mask_type_past_the_mask_is_refused(monkeypatch, mode, heads):
         with pytest.raises(ValueError, match=f"head_mask_type names mask slice {heads + 1} of {heads}"):
             reference_api.block_sparse_attn_func(q.requires_grad_(grad), q, q, cu, cu, hmt, None,
                                                  mask, 200, 200)
+
+
+def test_sink_dynamic_attention_refuses_what_the_kernel_would_read_past(on_device):
+    def t(H=3, S=200, dtype=torch.bfloat16):
+        return torch.zeros(2, H, S, 128, dtype=dtype)
+
+    mask, hmt = torch.ones(1, 3, 2, 2, dtype=torch.bool), torch.ones(3, dtype=torch.int64)
+    ok = dict(q=t(), k=t(), v=t(), block_mask=mask, k_pool=t(S=20), v_pool=t(S=20), sample_gap=4,
+              head_mask_type=hmt)
+    for match, kw in (("head_mask_type must be", dict(head_mask_type=hmt[:2])),
+                      ("block_mask must be", dict(block_mask=mask.float())),
+                      ("block_mask must be", dict(block_mask=mask[..., :1])),
+                      ("k and v must be", dict(k=t(H=2))), ("k and v must be", dict(v=t(S=199))),
+                      ("k_pool / v_pool must be", dict(k_pool=t(H=2, S=20)))):
+        with pytest.raises(RuntimeError, match=match):
+            on_device.sink_dynamic_attn(**{**ok, **kw})
