@@ -29,6 +29,7 @@ class _BlockSparseAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, block_mask, softmax_scale, head_mask_type):
         out, lse = ops.bsattn_fwd(q, k, v, block_mask, softmax_scale=softmax_scale,
                                   head_mask_type=head_mask_type)
+        out = out.detach()  # torch refuses to write over one of several results that is a view
         ctx.save_for_backward(q, k, v, out, lse, block_mask, head_mask_type)
         ctx.softmax_scale = softmax_scale
         ctx.set_materialize_grads(False)

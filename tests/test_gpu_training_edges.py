@@ -138,3 +138,23 @@ def test_the_forward_pass_reports_head_mask_type_past_the_mask():
         for a, b in zip(*grads):
             assert torch.equal(a, b)
     ops.DeviceStatus.check()
+
+
+def test_results_may_be_written_over():
+    """As without a gradient: what was recorded needs the output, so only its backward refuses."""
+    from sinkattn_b200.autograd import block_sparse_attention
+    from sinkattn_b200.reference_api import _block_sparse_attn
+
+    q, k, v, dout, mask = make_attn(1, 2, 260, 260, 0.6, 5)
+    want, want_lse = _block_sparse_attn(q, k, v, mask)
+    q.requires_grad_()
+    for call in (lambda: block_sparse_attention(q, k, v, mask),
+                 lambda: _block_sparse_attn(q, k, v, mask)):
+        out, lse = call()
+        assert out.requires_grad and out.stride() == want.stride()
+        out.mul_(2)
+        out[:, :, 3] = 0
+        lse.add_(1)
+        assert torch.equal(out[:, :, 4:], 2 * want[:, :, 4:]) and not out[:, :, 3].any()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
