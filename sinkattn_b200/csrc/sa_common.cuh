@@ -152,10 +152,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar_addr, uint32_t parity
 // Records a failure (a bounded wait that gave up, a bad index). The status
 // word may live in device memory or in mapped page-locked host memory (the
 // host then reads it without synchronising), so it is written with a plain
-// store made visible system-wide; the last writer's code stands.
+// store made visible system-wide. A wait that gave up says that outputs are not
+// valid, a bad index only where they are NaN or dense, so the one does not
+// replace the other (a read over PCIe, on failure only). Should both be written
+// within that read's time, either may stand.
 __device__ __forceinline__ void report_status(int32_t* status, int32_t code) {
   if (status == nullptr) return;
-  *reinterpret_cast<volatile int32_t*>(status) = code;
+  volatile int32_t* word = status;
+  if (code != SA_DEV_WAIT_TIMEOUT && *word == SA_DEV_WAIT_TIMEOUT) return;
+  *word = code;
   __threadfence_system();
 }
 

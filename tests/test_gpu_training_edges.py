@@ -158,3 +158,25 @@ def test_results_may_be_written_over():
         assert torch.equal(out[:, :, 4:], 2 * want[:, :, 4:]) and not out[:, :, 3].any()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             out.sum().backward()
+
+
+def test_a_bad_index_does_not_hide_a_wait_that_gave_up():
+    """The word says that outputs are not valid until the host has read it."""
+    import ctypes
+
+    from sinkattn_b200 import _lib, ops
+
+    x = torch.ones(1, 3, 2, 64, device="cuda")
+    table = torch.ones(4, 32, device="cuda")
+    bad = torch.tensor([0, 1, 4], device="cuda")
+    ops.DeviceStatus.check()
+    word = ctypes.c_int32.from_address(ops.DeviceStatus._word(x.device.index)[0])
+    word.value = _lib.SA_DEV_WAIT_TIMEOUT
+    ops.qk_head_norm_rope(x, x, 1e-6, cos=table, sin=table, positions=bad)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        ops.DeviceStatus.check()
+    ops.qk_head_norm_rope(x, x, 1e-6, cos=table, sin=table, positions=bad)
+    with pytest.raises(RuntimeError, match="position outside"):
+        ops.DeviceStatus.check()
+    ops.DeviceStatus.check()
