@@ -471,11 +471,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           !__all_sync(0xffffffffu, mbar_wait(&ctl->claim, (uint32_t)(k - 1) & 1u, p.status,
                                              abort_flag)))
         break;
-      if (piece_alone && was_piece &&
-          *reinterpret_cast<volatile int*>(p.next_item) < (by_length ? 2 * all : all) &&
-          !__all_sync(0xffffffffu, mbar_wait(&ctl->list_empty[slot ^ 1],
-                                             (uint32_t)((k - 1) >> 1) & 1u, p.status, abort_flag)))
-        break;
+      if (piece_alone && was_piece) {
+        // one lane's reading for all: other CTAs count on meanwhile
+        int claimed = 0;
+        if (lane == 0) claimed = *reinterpret_cast<volatile int*>(p.next_item);
+        claimed = __shfl_sync(0xffffffffu, claimed, 0);
+        if (claimed < (by_length ? 2 * all : all) &&
+            !__all_sync(0xffffffffu,
+                        mbar_wait(&ctl->list_empty[slot ^ 1], (uint32_t)((k - 1) >> 1) & 1u,
+                                  p.status, abort_flag)))
+          break;
+      }
       Item w;
       w.n = -1;
       uint32_t word = 0;  // lane i: blocks 32 i .. 32 i + 31

@@ -7,6 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from tests.test_gpu_attention_bwd import both as both_attn
 from tests.test_gpu_attention_bwd import make as make_attn
 from tests.test_gpu_norm_grad import backward_ref, both, check, make
 
@@ -179,4 +180,23 @@ def test_a_bad_index_does_not_hide_a_wait_that_gave_up():
     ops.qk_head_norm_rope(x, x, 1e-6, cos=table, sin=table, positions=bad)
     with pytest.raises(RuntimeError, match="position outside"):
         ops.DeviceStatus.check()
+    ops.DeviceStatus.check()
+
+
+def test_pieces_at_two_tiles_for_each_processor_beside_another_stream():
+    """256 tiles, the first of every head cut: each block of threads claims by the shared counter."""
+    from sinkattn_b200 import ops
+
+    q, k, v, dout, mask = make_attn(1, 4, 4096, 4096, 0.2, 26, layout="bhsd")
+    want = both_attn(q, k, v, dout, mask)
+    out, lse = ops.bsattn_fwd(q, k, v, mask)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        got = ops.bsattn_bwd(dout, q, k, v, out, lse, mask)
+        with torch.cuda.stream(side):
+            beside = ops.bsattn_bwd(dout, q, k, v, out, lse, mask)
+        torch.cuda.synchronize()
+        for a, b, c in zip(want, got, beside):
+            assert torch.equal(a, b) and torch.equal(a, c)
     ops.DeviceStatus.check()
