@@ -142,12 +142,11 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 // makes every P of theirs 0. Bound by reading dO and O once.
 constexpr int kPrepRows = 4;  // rows of a 16-lane group, loaded together
 __global__ void __launch_bounds__(256)
-    row_stats_kernel(const __nv_bfloat16* __restrict__ dout, const __nv_bfloat16* __restrict__ out,
-                     int64_t ds0, int64_t ds1, int64_t ds2, int64_t os0, int64_t os1, int64_t os2,
-                     const float* __restrict__ lse, const float* __restrict__ dlse, int H, int Sq,
-                     int rows_pad, float* __restrict__ nstat, int64_t plane, int* next_item,
-                     int* joined, int n_joined, int* counts0, int* counts1, int* eights,
-                     const Mask mask, int B, int nk, int32_t* status) {
+    row_stats_kernel(const __nv_bfloat16* dout, const __nv_bfloat16* out, int64_t ds0, int64_t ds1,
+                     int64_t ds2, int64_t os0, int64_t os1, int64_t os2, const float* lse,
+                     const float* dlse, int H, int Sq, int rows_pad, float* nstat, int64_t plane,
+                     int* next_item, int* joined, int n_joined, int* counts0, int* counts1,
+                     int* eights, const Mask mask, int B, int nk, int32_t* status) {
   release_next_kernel();  // it waits for this one's completion all the same
   // The call before may still be ending: calls in a row then take 48.0 -> 45.6 us
   // (4 heads of 4096) and 14.3 -> 12.4 us (2 heads of 300). The main kernel lets
@@ -214,7 +213,7 @@ __global__ void __launch_bounds__(256)
         row_lse[i] = lse[(int64_t)bh * Sq + r];
         if (dlse != nullptr) row_dlse[i] = dlse[(int64_t)bh * Sq + r];
       }
-      x[i] = __ldg(reinterpret_cast<const uint4*>(dout + b * ds0 + h * ds1 + (int64_t)r * ds2) + l);
+      x[i] = reinterpret_cast<const uint4*>(dout + b * ds0 + h * ds1 + (int64_t)r * ds2)[l];
       y[i] = __ldcs(reinterpret_cast<const uint4*>(out + b * os0 + h * os1 + (int64_t)r * os2) + l);
     }
   }

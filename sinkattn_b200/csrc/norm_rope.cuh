@@ -120,9 +120,9 @@ __device__ __forceinline__ float sum2(uint64_t v) {
 __device__ __forceinline__ V8 load_weight8(const void* w, int dtype, int c0) {
   if (w == nullptr) return fill8(1.f);
   const uint4* p = reinterpret_cast<const uint4*>(w);
-  if (dtype == SA_DTYPE_BF16) return unpack8(Raw8<__nv_bfloat16>{{__ldg(p + (c0 >> 3))}});
-  if (dtype == SA_DTYPE_FP16) return unpack8(Raw8<__half>{{__ldg(p + (c0 >> 3))}});
-  return unpack8(Raw8<float>{{__ldg(p + (c0 >> 2)), __ldg(p + (c0 >> 2) + 1)}});
+  if (dtype == SA_DTYPE_BF16) return unpack8(Raw8<__nv_bfloat16>{{p[c0 >> 3]}});
+  if (dtype == SA_DTYPE_FP16) return unpack8(Raw8<__half>{{p[c0 >> 3]}});
+  return unpack8(Raw8<float>{{p[c0 >> 2], p[(c0 >> 2) + 1]}});
 }
 
 // 1 / sqrt(v): the hardware's approximation (within 2^-22), with one Newton

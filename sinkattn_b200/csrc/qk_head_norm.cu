@@ -107,8 +107,8 @@ __device__ __forceinline__ Angles<INTER> load_angles(const Params& p, int64_t ro
   if (INTER) {
     float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c0 < p.rot) {
-      c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t + row * p.fs + (c0 >> 1)));
-      s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t + row * p.fs + (c0 >> 1)));
+      c4 = *reinterpret_cast<const float4*>(p.cos_t + row * p.fs + (c0 >> 1));
+      s4 = *reinterpret_cast<const float4*>(p.sin_t + row * p.fs + (c0 >> 1));
     }
     a.c[0] = f2_pack(c4.x, c4.y); a.c[1] = f2_pack(c4.z, c4.w);
     a.s[0] = f2_pack(sign * s4.x, sign * s4.y); a.s[1] = f2_pack(sign * s4.z, sign * s4.w);
@@ -122,8 +122,8 @@ __device__ __forceinline__ Angles<INTER> load_angles(const Params& p, int64_t ro
       const float m = c0 < half ? -sign : sign;
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
-        const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t + row * p.fs + i0 + i));
-        const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.sin_t + row * p.fs + i0 + i));
+        const float4 c4 = *reinterpret_cast<const float4*>(p.cos_t + row * p.fs + i0 + i);
+        const float4 s4 = *reinterpret_cast<const float4*>(p.sin_t + row * p.fs + i0 + i);
         c[i] = c4.x; c[i + 1] = c4.y; c[i + 2] = c4.z; c[i + 3] = c4.w;
         s[i] = m * s4.x; s[i + 1] = m * s4.y; s[i + 2] = m * s4.z; s[i + 3] = m * s4.w;
       }

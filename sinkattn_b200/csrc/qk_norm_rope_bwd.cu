@@ -23,8 +23,8 @@ namespace nr {
 // loads of a chain are all in flight (8 chains took 10 us for 600 rows).
 constexpr int kChains = 32;
 __global__ void __launch_bounds__(32 * kChains)
-    partial_rows_kernel(const float* __restrict__ part, int rows, int cols, int pitch,
-                        float* __restrict__ out0, float* __restrict__ out1, int cols0) {
+    partial_rows_kernel(const float* part, int rows, int cols, int pitch, float* out0, float* out1,
+                        int cols0) {
   __shared__ float red[kChains][33];
   wait_prior_kernel();
   const int l = threadIdx.x & 31, chain = threadIdx.x >> 5;

@@ -52,6 +52,7 @@ bool strides16_ok(const int64_t st[4]);
 // before it touches what that kernel writes, in every thread, so that it does
 // not complete before that kernel either. That kernel may be anything: one that
 // does not call release_next_kernel() is waited for as in an ordinary launch.
+// Its inputs may be written while it already runs: no read-only loads of them.
 template <typename... Params, typename... Args>
 cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
                          cudaStream_t stream, Args... args) {

@@ -122,3 +122,19 @@ def test_sink_dynamic_attention_refuses_what_the_kernel_would_read_past(on_devic
                       ("k_pool / v_pool must be", dict(k_pool=t(H=2, S=20)))):
         with pytest.raises(RuntimeError, match=match):
             on_device.sink_dynamic_attn(**{**ok, **kw})
+
+
+def test_kernels_that_start_early_promise_nothing_read_only():
+    """A kernel of a dependent launch runs while the one before it still writes, so its inputs are
+    not read-only for as long as it runs: no read-only loads, and no __restrict__ that allows them
+    (a compiler may move either above the wait)."""
+    from pathlib import Path
+
+    import sinkattn_b200
+
+    csrc = Path(sinkattn_b200.__file__).parent / "csrc"
+    early = [f for f in csrc.glob("*.cu") if "launch_after(" in f.read_text()]
+    assert len(early) == 3
+    for f in early + [csrc / "norm_rope.cuh"]:
+        text = f.read_text()
+        assert "__ldg(" not in text and "__restrict__" not in text, f.name
