@@ -19,6 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from . import ops
 
+
 def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a call on these tensors has to be recorded."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
@@ -118,3 +119,31 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, head_dim: int, eps: float,
     (the tables get none); the bf16 rounding between the norm and the rotation
     counts as the identity."""
     return _QKNormRope.apply(q, k, head_dim, eps, w_q, w_k, cos, sin)
+
+
+class _MeanPool(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, pool, prefix):
+        ctx.size, ctx.pool, ctx.prefix = x.shape[2], pool, prefix
+        return ops.mean_pool_seq(x, pool, prefix).detach()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        pooled = dout[:, :, ctx.prefix:]
+        tokens = ctx.size - ctx.prefix
+        # the last pool counts the final token once more for each token it lacks
+        last = 1 + pooled.shape[2] * ctx.pool - tokens
+        spread = (pooled.float() / ctx.pool).to(dout.dtype)
+        dx = spread.repeat_interleave(ctx.pool, dim=2)[:, :, :tokens]
+        if last > 1:
+            dx[:, :, -1] = (pooled[:, :, -1].float() * (last / ctx.pool)).to(dout.dtype)
+        return torch.cat([dout[:, :, :ctx.prefix], dx], dim=2), None, None
+
+
+def mean_pool_seq(x: torch.Tensor, pool: int, prefix: int = 0) -> torch.Tensor:
+    """ops.mean_pool_seq with a gradient for x (torch operations, one rounding)."""
+    prefix = min(max(int(prefix), 0), x.shape[2])
+    if pool <= 1 or prefix == x.shape[2]:
+        return x
+    return _MeanPool.apply(x, int(pool), prefix)

@@ -328,18 +328,19 @@ def _build_direct_mean_coverage_mask(mean_scores: torch.Tensor, config) -> torch
 
 @_reports_device_failures
 def _mean_pool_sequence_preserve_prefix(x: torch.Tensor, pool_size: int, *, prefix_tokens: int = 0):
-    """sparse_attention.py:97-115 (bf16 in/out, fp32 accumulation)."""
+    """sparse_attention.py:97-115 (bf16 in/out, fp32 accumulation). Differentiable
+    where x requires a gradient."""
     if pool_size <= 1:
         return x
-    return ops.mean_pool_seq(x, int(pool_size), int(prefix_tokens))
+    pool = autograd.mean_pool_seq if autograd.needs_grad(x) else ops.mean_pool_seq
+    return pool(x, int(pool_size), int(prefix_tokens))
 
 
 @_reports_device_failures
 def _mean_pool_sequence(x: torch.Tensor, pool_size: int):
-    """sparse_attention.py:88-94 for bf16 tensors (Z-Image pooled branch)."""
-    if pool_size <= 1:
-        return x
-    return ops.mean_pool_seq(x, int(pool_size), 0)
+    """sparse_attention.py:88-94 for bf16 tensors (Z-Image pooled branch).
+    Differentiable where x requires a gradient."""
+    return _mean_pool_sequence_preserve_prefix(x, pool_size)
 
 
 @_reports_device_failures
