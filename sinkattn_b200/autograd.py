@@ -12,6 +12,7 @@ stream it was first recorded on).
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -147,3 +148,30 @@ def mean_pool_seq(x: torch.Tensor, pool: int, prefix: int = 0) -> torch.Tensor:
     if pool <= 1 or prefix == x.shape[2]:
         return x
     return _MeanPool.apply(x, int(pool), prefix)
+
+
+class _MixOutputs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, sink_out, sink_lse, dyn_out, dyn_lse, sample_gap):
+        ctx.save_for_backward(sink_out, sink_lse, dyn_out, dyn_lse)
+        ctx.log_gap = math.log(float(max(1, int(sample_gap))))
+        return ops.mix_outputs(sink_out, sink_lse, dyn_out, dyn_lse, sample_gap).detach()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        sink_out, sink_lse, dyn_out, dyn_lse = ctx.saved_tensors
+        rows = (*sink_out.shape[:3], 1)
+        lead = sink_lse.reshape(rows).float() - (dyn_lse.reshape(rows).float() + ctx.log_gap)
+        w_sink, w_dyn = torch.sigmoid(lead), torch.sigmoid(-lead)
+        d = dout.float()
+        dlead = w_sink * w_dyn * (d * (sink_out.float() - dyn_out.float())).sum(-1, keepdim=True)
+        return ((d * w_sink).to(sink_out.dtype), dlead.reshape(sink_lse.shape).to(sink_lse.dtype),
+                (d * w_dyn).to(dyn_out.dtype), -dlead.reshape(dyn_lse.shape).to(dyn_lse.dtype), None)
+
+
+def mix_outputs(sink_out: torch.Tensor, sink_lse: torch.Tensor, dyn_out: torch.Tensor,
+                dyn_lse: torch.Tensor, sample_gap: int) -> torch.Tensor:
+    """ops.mix_outputs with gradients for both outputs and both log-sum-exps
+    (torch operations in fp32, one rounding)."""
+    return _MixOutputs.apply(sink_out, sink_lse, dyn_out, dyn_lse, sample_gap)

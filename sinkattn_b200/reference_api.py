@@ -345,13 +345,16 @@ def _mean_pool_sequence(x: torch.Tensor, pool_size: int):
 
 @_reports_device_failures
 def _mix_attention_outputs(sink_out, sink_lse, dynamic_out, dynamic_lse, config, dynamic_sample_gap=None):
-    """sparse_attention.py:898-919 (adaptive mode) as one fused kernel."""
+    """sparse_attention.py:898-919 (adaptive mode) as one fused kernel.
+    Differentiable where an output or a log-sum-exp requires a gradient."""
     if config.mixing_mode != "adaptive":
         raise ValueError(f"Unsupported mixing_mode: {config.mixing_mode}")
     if sink_lse is None or dynamic_lse is None:
         raise ValueError("Adaptive Sink-Sparse mixing requires both sink_lse and dynamic_lse.")
     gap = config.sample_gap if dynamic_sample_gap is None else int(dynamic_sample_gap)
-    return ops.mix_outputs(sink_out, sink_lse, dynamic_out, dynamic_lse, gap)
+    record = autograd.needs_grad(sink_out, sink_lse, dynamic_out, dynamic_lse)
+    mix = autograd.mix_outputs if record else ops.mix_outputs
+    return mix(sink_out, sink_lse, dynamic_out, dynamic_lse, gap)
 
 
 @_reports_device_failures

@@ -8,6 +8,9 @@ terms), as in the modules of the other gradients.
 """
 from __future__ import annotations
 
+import math
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -88,3 +91,47 @@ def test_sequence_pooling(B, H, S, pool, prefix, layout):
         (dx,) = torch.autograd.grad(out, leaf, d)
         d[:, :, 0] = 0
         close("dx", dx, *pool_grad(d, S, pool, prefix))
+
+
+def mix_grads(os, ls, od, ld, gap, d):
+    """Gradients and bounds of the adaptive mix, in 64 bits."""
+    os, ls, od, ld, d = (t.double() for t in (os, ls, od, ld, d))
+    lead = ls - (ld + math.log(gap))
+    ws, wd = torch.sigmoid(lead), torch.sigmoid(-lead)
+    dl = ws * wd * (d * (os - od)).sum(-1, keepdim=True)
+    bl = E * ws * wd * (d.abs() * (os.abs() + od.abs())).sum(-1, keepdim=True)
+    out = (d * ws, dl, d * wd, -dl)
+    return out, [(E + U) * out[0].abs(), bl, (E + U) * out[2].abs(), bl]
+
+
+@pytest.mark.parametrize("lse_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,S,gap", [(1, 1, 1, 30), (2, 3, 77, 4), (1, 2, 300, 1)])
+def test_adaptive_mix(B, H, S, gap, lse_dtype):
+    from sinkattn_b200 import autograd, ops
+    from sinkattn_b200.reference_api import _mix_attention_outputs
+
+    os, od, d = (randn(B, H, S, 128, seed=s) for s in (2, 3, 4))
+    ls, ld = ((3 * randn(B, H, S, 1, seed=s)).to(lse_dtype) for s in (5, 6))
+    ls[:, :, S // 2] = float("-inf")  # a row that keeps no sink block
+    os[:, :, S // 2] = 0
+    want = ops.mix_outputs(os, ls, od, ld, gap)
+    cfg = SimpleNamespace(mixing_mode="adaptive", sample_gap=gap)
+    ref, bound = mix_grads(os, ls, od, ld, gap, d)
+    for call in (lambda a, b, c, e: autograd.mix_outputs(a, b, c, e, gap),
+                 lambda a, b, c, e: _mix_attention_outputs(a, b, c, e, cfg)):
+        leaves = [t.detach().clone().requires_grad_() for t in (os, ls, od, ld)]
+        out = call(*leaves)
+        assert torch.equal(out, want) and out.stride() == want.stride()
+        got = torch.autograd.grad(out, leaves, d, retain_graph=True)
+        for n, t, g, r, b in zip(("sink", "sink lse", "dynamic", "dynamic lse"), leaves, got, ref,
+                                 bound):
+            assert g.dtype == t.dtype
+            close(n, g, r, b + (U * r.abs() if "lse" in n and lse_dtype != torch.float32 else 0))
+        with torch.no_grad():
+            assert not call(*leaves).requires_grad
+        out.mul_(2)  # may be written over, as unrecorded, and keeps its gradient
+        got = torch.autograd.grad(out, leaves[0], d)[0]
+        close("sink", got, 2 * ref[0], 2 * bound[0])
+        # one of them alone
+        out = call(os, leaves[1], od, ld)
+        assert torch.equal(out, want) and torch.autograd.grad(out, leaves[1], d)[0].shape == ls.shape
