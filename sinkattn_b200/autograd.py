@@ -175,3 +175,53 @@ def mix_outputs(sink_out: torch.Tensor, sink_lse: torch.Tensor, dyn_out: torch.T
     """ops.mix_outputs with gradients for both outputs and both log-sum-exps
     (torch operations in fp32, one rounding)."""
     return _MixOutputs.apply(sink_out, sink_lse, dyn_out, dyn_lse, sample_gap)
+
+
+class _SinkDynamicAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, block_mask, k_pool, v_pool, sample_gap, softmax_scale,
+                head_mask_type):
+        out, lse = ops.sink_dynamic_attn(q, k, v, block_mask, k_pool, v_pool, sample_gap,
+                                         softmax_scale=softmax_scale,
+                                         head_mask_type=head_mask_type, return_lse=True)
+        out = out.detach()  # as above
+        if head_mask_type is not None:
+            head_mask_type = head_mask_type.to(torch.int32)
+        ctx.save_for_backward(q, k, v, k_pool, v_pool, out, lse, block_mask, head_mask_type)
+        ctx.softmax_scale = softmax_scale
+        ctx.log_gap = math.log(float(max(1, int(sample_gap))))
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlse):
+        if dout is None and dlse is None:
+            return (None,) * 9
+        q, k, v, k_pool, v_pool, out, lse, block_mask, head_mask_type = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros_like(out)
+        # One softmax over both kinds of keys: with the joint output and log-sum-exp the
+        # backward pass of either kind is that of the attention alone. The pooled keys' logits
+        # are raised by ln(gap), which taken from the log-sum-exp is the same probability.
+        dq, dk, dv = ops.bsattn_bwd(dout, q, k, v, out, lse, block_mask,
+                                    softmax_scale=ctx.softmax_scale,
+                                    head_mask_type=head_mask_type, dlse=dlse)
+        dense = torch.zeros(q.shape[1], dtype=torch.int32, device=q.device)
+        blocks = [-(-t.shape[2] // ops.BLOCK) for t in (q, k_pool)]
+        unread = torch.ones(1, 1, *blocks, dtype=torch.bool, device=q.device)
+        dq2, dk_pool, dv_pool = ops.bsattn_bwd(dout, q, k_pool, v_pool, out, lse - ctx.log_gap,
+                                               unread, softmax_scale=ctx.softmax_scale,
+                                               head_mask_type=dense, dlse=dlse)
+        return dq.add_(dq2), dk, dv, None, dk_pool, dv_pool, None, None, None
+
+
+def sink_dynamic_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           block_mask: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                           sample_gap: int, softmax_scale: Optional[float] = None,
+                           head_mask_type: Optional[torch.Tensor] = None):
+    """ops.sink_dynamic_attn with gradients for q, k, v, k_pool and v_pool, through
+    both results. Returns (out, lse); the backward pass takes at most 131072
+    queries and keys and refuses more."""
+    return _SinkDynamicAttention.apply(q, k, v, block_mask, k_pool, v_pool, sample_gap,
+                                       softmax_scale, head_mask_type)

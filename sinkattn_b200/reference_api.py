@@ -364,9 +364,10 @@ def fused_wan_inner_forward(self, q, k, v):
     into one kernel (sa_sink_dynamic_attn_fwd).
 
     The runtime mask, timing sections and mask statistics are the reference
-    method's own. Configurations other than the Wan default (dynamic_mode
-    pooled_kv, adaptive mixing, block-sparse dynamic kernel) run the
-    reference's unfused method, which uses the other drop-in functions.
+    method's own. Differentiable where q, k or v requires a gradient.
+    Configurations other than the Wan default (dynamic_mode pooled_kv, adaptive
+    mixing, block-sparse dynamic kernel) run the reference's unfused method,
+    which uses the other drop-in functions.
     """
     from contextlib import nullcontext
 
@@ -389,7 +390,9 @@ def fused_wan_inner_forward(self, q, k, v):
             v_dyn = _mean_pool_sequence_preserve_prefix(v, gap, prefix_tokens=prefix_tokens)
             dynamic_seq_len_k = int(k_dyn.size(2))
         with (time_section("sparse_main") if time_section is not None else nullcontext()):
-            mixed_out, _ = ops.sink_dynamic_attn(q, k, v, base_runtime_mask, k_dyn, v_dyn, gap)
+            record = autograd.needs_grad(q, k, v)
+            attention = autograd.sink_dynamic_attention if record else ops.sink_dynamic_attn
+            mixed_out, _ = attention(q, k, v, base_runtime_mask, k_dyn, v_dyn, gap)
         if self.runtime_state is not None:
             with self.runtime_state.time_section("stats"):
                 self.runtime_state.record_mask_stats(
