@@ -596,7 +596,8 @@ SA_API int sa_ulysses_combine_units(const void* out_units, const float* lse_unit
  *   sa_status_destroy frees it.
  * sa_check_status: reads a host-readable status word without synchronising:
  *   SA_OK if no kernel reported a failure, else SA_ETIMEOUT (SA_EINVAL for
- *   SA_DEV_BAD_INDEX) with a message, and the word is reset to SA_DEV_OK. A
+ *   SA_DEV_BAD_INDEX, which does not replace a SA_DEV_WAIT_TIMEOUT that stands)
+ *   with a message, and the word is reset to SA_DEV_OK. A
  *   launch's report becomes visible once the launch has run, so a caller that
  *   needs a verdict on a given launch synchronises its stream first.
  */

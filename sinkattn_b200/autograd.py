@@ -1,9 +1,11 @@
 """Differentiable forms of the tensor-level operators.
 
 Each function runs the same kernel as its namesake in :mod:`sinkattn_b200.ops`
-and records what its gradient kernel needs; without a differentiable input
-(or under torch.no_grad()) nothing is recorded. The gradients are first-order
-only. reference_api's drop-ins call these where an input requires a gradient.
+(sink_dynamic_attention: sink_dynamic_attn) and records what its gradient needs;
+without a differentiable input (or under torch.no_grad()) nothing is recorded.
+The gradients are first-order only. reference_api's drop-ins call these where
+an input requires a gradient. Results may be written over; where the gradient
+needs the output (both attentions) the backward pass then refuses.
 
 A backward pass may be captured into a CUDA graph like any other torch one:
 warm it up on a side stream and let no graph of the same leaves that was

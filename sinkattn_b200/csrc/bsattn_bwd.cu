@@ -331,7 +331,8 @@ __device__ __forceinline__ void split_bf16x2(float x0, float x1, uint32_t& hi, u
 // single roundings show, up to twice that, so FINE keeps P and dS as two bf16
 // halves, each a product of its own in the columns that X and Y leave free.
 // The launch takes it where the blocks do not fill the GPU once and the extra
-// products hide behind latencies (300 tokens, 2 heads: 12.1 us become 13.0).
+// products hide behind latencies (300 tokens, 2 heads, in a captured graph: 11.9
+// us become 13.4).
 // MODE: what may happen to the tiles. Compiled apart, as code that a launch does
 // not need costs it time: 2 us of 300 tokens, 2 heads (cold caches: 19.3 and 17.4
 // us), 0.6% of long ones.
@@ -447,16 +448,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // hides the way from the counter to its first tiles best. With few, that
     // gives every CTA its second tile at the start; so it is claimed once the
     // loads of the one before are issued, and where tiles are counted the long
-    // ones are taken first. Up to four per SM: 2 heads of 8192 tokens 65.4 -> 59.8
-    // us, 24 heads of 1024 47.1 -> 44.6; beyond: 4680 x 500 tokens 95.9 -> 99.9,
-    // 30 heads of 4096 242 -> 254.
+    // ones are taken first. Up to four per SM: 2 heads of 8192 tokens 60.6 -> 53.4
+    // us, 24 of 1024 33.9 -> 29.2, 6 of 5000 80.0 -> 71.0, 4 of 9000 116 -> 111.5;
+    // beyond: 4680 x 500 tokens 94 -> 97, 30 heads of 4096 206.7 -> 213.8.
     const int all = p.tiles[0] + p.tiles[1];
     const bool few = MODE == kFew || (CUT && all <= kFewTiles * (int)gridDim.x);
     const bool by_length = CUT && few && p.counts[0] != nullptr && p.counts[1] != nullptr;
     // With two tiles per SM and few pieces, the SMs that add a tile's pieces up are
     // the last to finish their first item, so they claim the next one, if any is
-    // left, only then: 4 heads of 4096 44.0 -> 37.9 us, one of 16384 66.6 -> 58.6.
-    // Where most items are pieces all would wait (+3%).
+    // left, only then: 4 heads of 4096 44.0 -> 38.2 us, 3 of 4096 39.1 -> 33.7, 5 of
+    // 3700 52.2 -> 48.0, one of 18000 67.2 -> 62.5; one of 8192 42.1 -> 42.9. Where
+    // most items are pieces all would wait (+3%).
     const bool piece_alone = CUT && all <= 2 * (int)gridDim.x &&
                              2 * (extra[0] + extra[1]) <= (int)gridDim.x;
     bool was_piece = false;
@@ -1062,8 +1064,8 @@ namespace {
 // Which kinds of tiles may be cut, and where everything lies in the workspace.
 // Few tiles do not fill the GPU, and among more of them a long one (a key block
 // that every query keeps) holds one SM after the others are done: one head of
-// 65536 tokens, a twentieth of its blocks kept, took 976 us without cutting
-// and takes 360. With 16 tiles per SM and a sixteenth of the blocks kept a full
+// 65536 tokens, a twentieth of its blocks kept, takes 800 us without cutting
+// and 304 with it. With 16 tiles per SM and a sixteenth of the blocks kept a full
 // line is within an SM's share, and the counting is saved.
 struct Layout {
   int tiles[2], max_extra, n_joined, n_eights;
