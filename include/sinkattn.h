@@ -149,6 +149,7 @@ SA_API int sa_sink_dynamic_attn_fwd(
  *   scale. dlse: nullable fp32 [B,H,Sq] contiguous, the gradient with respect
  *   to lse. dq, dk and dv are written whole: rows whose mask row (key blocks
  *   whose mask column) keeps nothing get 0, whatever their lse and dout hold.
+ *   They may share no element with an input or with one another.
  * block_mask, m_strides, Hm, head_mask_type, softmax_scale, status: as for
  *   sa_bsattn_fwd. Sq, Sk <= 131072. P and dS enter their products as bf16 (as
  *   two bf16 halves each where the call has no more blocks than the GPU has
@@ -441,8 +442,8 @@ SA_API int sa_qk_norm_rope_bwd(const void* dq, const void* dk, int64_t dq_row_st
  *   channels from rot_dim on are y. fp32 throughout, rounded once.
  * q, q_out [B,S,Hq,D], k, k_out [B,S,Hk,D] of `dtype` (SA_DTYPE_*), strides in
  *   the order (batch, seq, head, dim) with stride(dim) = 1, 16-byte aligned
- *   bases and strides; an output may be its input. Hk may be 0 (no k). D a
- *   multiple of 8 up to 256.
+ *   bases and strides; an output may be its input (q_out q, k_out k, nothing
+ *   else). Hk may be 0 (no k). D a multiple of 8 up to 256.
  * w_q, w_k: [D] of w_dtype, both NULL for none. cos/sin: fp32 [table_rows,
  *   >= rot_dim/2] with the given row stride, both NULL for no rotation; rot_dim
  *   a multiple of 8 (16 without interleaving) up to D.

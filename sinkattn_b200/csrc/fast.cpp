@@ -71,6 +71,13 @@ bool output(const Arg& a) {
   return true;
 }
 
+// ops.py refuses an output that begins where a tensor does that is still read.
+bool apart(const Arg& out, std::initializer_list<const Arg*> others) {
+  for (const Arg* o : others)
+    if (out && *o && out.ptr() == o->ptr()) return false;
+  return true;
+}
+
 bool workspace(const Arg& a) { return !a || a->is_contiguous(); }
 
 struct Strides {
@@ -171,6 +178,9 @@ PyObject* bsattn_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   for (const Arg* t : {&dout, &q, &k, &v, &out, &dq, &dk, &dv})
     if (*t && !vectors(**t)) return none();
   if (!output(dq) || !output(dk) || !output(dv) || !workspace(ws)) return none();
+  if (!apart(dq, {&dout, &q, &k, &v, &out, &dk, &dv}) ||
+      !apart(dk, {&dout, &q, &k, &v, &out, &dv}) || !apart(dv, {&dout, &q, &k, &v, &out}))
+    return none();
   for (const Arg* t : {&lse, &dlse})
     if (*t && ((*t)->scalar_type() != at::kFloat || (*t)->dim() != 3 || (*t)->size(0) != B ||
                (*t)->size(1) != H || (*t)->size(2) != Sq || !(*t)->is_contiguous()))
@@ -247,6 +257,7 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (st[i] < 0) return none();
   }
   if (!output(dq) || !output(dk) || !workspace(ws)) return none();
+  if (!apart(dq, {&k, &dko, &dk}) || !apart(dk, {&q, &dqo})) return none();
   if (bool(wq) != bool(wk) || bool(cos) != bool(sin)) return none();
   if (wq && (wq->dim() != 1 || wq->size(0) != hidden || !same(*wk, *wq) || !flat(*wq) ||
              !flat(*wk) ||
@@ -355,7 +366,9 @@ PyObject* qk_head_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 11 || lib.head == nullptr) return none();
   const Head h(a);
   const Arg oq(a[9]), ok(a[10]);
-  if (!h.ok || !fits(oq, h.q) || !fits(ok, h.k) || !output(oq) || !output(ok)) return none();
+  if (!h.ok || !fits(oq, h.q) || !fits(ok, h.k) || !output(oq) || !output(ok) ||
+      !apart(oq, {&h.k, &ok}) || !apart(ok, {&h.q}))
+    return none();
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)h.dev);
   const at::Tensor rq = result(oq, h.q), rk = result(ok, h.k);
   const Strides sq(*h.q), sk = h.k ? Strides(*h.k) : Strides(), tq(rq),
@@ -380,7 +393,7 @@ PyObject* qk_head_norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Arg uq(a[9]), uk(a[10]), dq(a[11]), dk(a[12]), ws(a[13]);
   if (!h.ok || !uq || bool(uk) != bool(h.k) || !fits(uq, h.q) || !fits(uk, h.k) ||
       !fits(dq, h.q) || !fits(dk, h.k) || !output(dq) || !output(dk) || !on(ws, h.dev) ||
-      !workspace(ws))
+      !workspace(ws) || !apart(dq, {&h.k, &uk, &dk}) || !apart(dk, {&h.q, &uq}))
     return none();
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)h.dev);
   const at::Tensor rq = result(dq, h.q), rk = result(dk, h.k);

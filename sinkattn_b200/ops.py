@@ -92,6 +92,18 @@ def _check_output(fn: str, name: str, t: torch.Tensor) -> None:
         raise RuntimeError(f"{fn}: {name} is expanded: its elements share memory")
 
 
+def _check_apart(fn: str, outs: dict, others: dict) -> None:
+    """Refuses outputs that begin where another tensor of the call does, one that other blocks of
+    threads may still read or write (views that interleave in one buffer begin apart)."""
+    seen = {t.data_ptr(): name for name, t in others.items() if t is not None and t.numel()}
+    for name, t in outs.items():
+        if t is None or not t.numel():
+            continue
+        if t.data_ptr() in seen:
+            raise RuntimeError(f"{fn}: {name} has the address of {seen[t.data_ptr()]}")
+        seen[t.data_ptr()] = name
+
+
 def _check_workspace(fn: str, t: torch.Tensor, dev: torch.device) -> None:
     if t.device != dev or not t.is_contiguous():
         raise RuntimeError(f"{fn}: workspace must be contiguous on {dev}")
@@ -285,8 +297,8 @@ def bsattn_bwd(
     dout [B,H,Sq,D] bf16; q, k, v, block_mask, softmax_scale, head_mask_type
     as given to bsattn_fwd, out and lse as it returned them; dlse: optional
     fp32 [B,H,Sq] gradient with respect to lse. Returns (dq, dk, dv) bf16;
-    each defaults to a [B,S,H,D]-contiguous buffer viewed as [B,H,S,D]. Equal
-    calls give equal bits. A given `workspace` (uint8,
+    each defaults to a [B,S,H,D]-contiguous buffer viewed as [B,H,S,D], and
+    may share no element with an input. Equal calls give equal bits. A given `workspace` (uint8,
     sa_bsattn_bwd_workspace_size bytes) may hold anything; calls sharing one
     must not overlap on the GPU.
     """
@@ -345,6 +357,8 @@ def _bsattn_bwd_plan(dout, q, k, v, out, lse, block_mask, softmax_scale, head_ma
             raise RuntimeError(f"bsattn_bwd: {name} must be fp32 {(B, H, Sq)}, got {t.dtype} "
                                f"{tuple(t.shape)}")
     _check_block_mask("bsattn_bwd", block_mask, head_mask_type, B, H, Sq, Sk)
+    _check_apart("bsattn_bwd", {"dq": dq, "dk": dk, "dv": dv},
+                 {"dout": dout, "q": q, "k": k, "v": v, "out": out})
     fits = (all(_strides16_ok(t) for t in (dout, q, k, v, out))
             and all(t is None or t.is_contiguous() for t in (lse, dlse, head_mask_type)))
     with torch.cuda.device(dev):
@@ -1096,6 +1110,8 @@ def _qk_norm_rope_bwd_plan(dq_out, dk_out, q, k, head_dim, w_q, w_k, cos, sin, d
             _check_output("qk_norm_rope_bwd", name, t)
             if _row_stride(t) is None:
                 raise RuntimeError("qk_norm_rope_bwd outputs need uniform rows, 16-byte aligned")
+    _check_apart("qk_norm_rope_bwd", {"dq": dq}, {"dk_out": dk_out, "k": k, "dk": dk})
+    _check_apart("qk_norm_rope_bwd", {"dk": dk}, {"dq_out": dq_out, "q": q})
     if (w_q is None) != (w_k is None) or (cos is None) != (sin is None):
         raise RuntimeError("qk_norm_rope_bwd: w_q and w_k, cos and sin go together")
     fits = all(_row_stride(t) is not None for t in (dq_out, dk_out, q, k))
@@ -1158,6 +1174,11 @@ def _head_norm_plan(fn, q, k, w_q, w_k, cos, sin, positions, interleaved, more, 
         if not _strides16_ok(t):
             raise RuntimeError(f"{fn}: {name} must have stride(-1)=1, 16-byte strides and "
                                "alignment")
+    # an output may lie over its own tensor's inputs
+    (out_of_q, o_q, _), (out_of_k, o_k, _) = outs
+    up = {name: t for name, t, _ in more}
+    _check_apart(fn, {out_of_q: o_q}, {"k": k, "dk_out": up.get("dk_out"), out_of_k: o_k})
+    _check_apart(fn, {out_of_k: o_k}, {"q": q, "dq_out": up.get("dq_out")})
     fits = all(t is None or _strides16_ok(t) for t in (q, k, *(t for _, t, _ in more)))
     w_dtype = _lib.SA_DTYPE_FP32
     if w_q is None and w_k is not None or k is not None and (w_q is None) != (w_k is None):
@@ -1248,7 +1269,8 @@ def qk_head_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], eps: float,
     uses table row s, or row positions[b, s] (int32 / int64 [B,S] or [S]) where
     given; a position outside the table makes the token's rows NaN and is
     reported by DeviceStatus. fp32 throughout, rounded once. Returns (q, k) of
-    the input type; out_q/out_k may alias q/k or be views of a larger buffer.
+    the input type; out_q may alias q and out_k k, or be views of a larger
+    buffer.
     """
     fn = "qk_head_norm_rope"
     got = _short(fn, q, k, eps, w_q, w_k, cos, sin, positions, interleaved, out_q, out_k)

@@ -200,3 +200,31 @@ def test_pieces_at_two_tiles_for_each_processor_beside_another_stream():
         for a, b, c in zip(want, got, beside):
             assert torch.equal(a, b) and torch.equal(a, c)
     ops.DeviceStatus.check()
+
+
+def test_outputs_in_the_place_of_inputs():
+    """By either way into the library: refused where other blocks still read them, else the same."""
+    from sinkattn_b200 import ops
+
+    q, k, v, dout, mask = make_attn(1, 2, 300, 300, 0.5, 42)
+    out, lse = ops.bsattn_fwd(q, k, v, mask)
+    ops.bsattn_bwd(dout, q, k, v, out, lse, mask)
+    for kw in (dict(dq=dout), dict(dk=k), dict(dv=out), dict(dq=v, dk=v)):
+        with pytest.raises(RuntimeError, match="has the address of"):
+            ops.bsattn_bwd(dout, q, k, v, out, lse, mask, **kw)
+    # views that interleave in one buffer are apart
+    want = ops.bsattn_bwd(dout, q, k, v, out, lse, mask)
+    packed = torch.zeros(1, 300, 3, 2, 128, dtype=torch.bfloat16, device="cuda")
+    dq, dk, dv = (packed[:, :, i].transpose(1, 2) for i in range(3))
+    for a, b in zip(ops.bsattn_bwd(dout, q, k, v, out, lse, mask, dq=dq, dk=dk, dv=dv), want):
+        assert torch.equal(a, b)
+    a, w, cos, sin, _ = make(2, 9, 3, 3, 128, 128, torch.bfloat16, seed=43)
+    args = (a["dq"], a["dk"], a["q"], a["k"], 1e-6, *w, cos, sin)
+    for kw in (dict(dq=a["dk"]), dict(dk=a["q"])):
+        with pytest.raises(RuntimeError, match="has the address of"):
+            ops.qk_head_norm_rope_bwd(*args, **kw)
+    with pytest.raises(RuntimeError, match="has the address of"):
+        ops.qk_head_norm_rope(a["q"], a["k"], 1e-6, *w, cos, sin, out_q=a["k"])
+    rows = [a[n].flatten(2) for n in ("dq", "dk", "q", "k")]
+    with pytest.raises(RuntimeError, match="has the address of"):
+        ops.qk_norm_rope_bwd(*rows, 128, 1e-6, dq=rows[1])

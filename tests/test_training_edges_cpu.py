@@ -138,3 +138,29 @@ def test_kernels_that_start_early_promise_nothing_read_only():
     for f in early + [csrc / "norm_rope.cuh"]:
         text = f.read_text()
         assert "__ldg(" not in text and "__restrict__" not in text, f.name
+
+
+def test_outputs_in_the_place_of_what_is_still_read_are_refused(on_device):
+    """Blocks of threads read one another's inputs, so those may not be written over."""
+    ops = on_device
+
+    def t(*s):
+        return torch.zeros(*s, dtype=torch.bfloat16)
+
+    dout, q, k, v, out = (t(1, 2, 130, 128) for _ in range(5))
+    lse, mask, new = torch.zeros(1, 2, 130), torch.ones(1, 2, 2, 2, dtype=torch.bool), t(1, 2, 130, 128)
+    for kw in (dict(dq=dout), dict(dq=q), dict(dk=k), dict(dv=v), dict(dk=out), dict(dv=q),
+               dict(dq=new, dk=new), dict(dk=new, dv=new)):
+        with pytest.raises(RuntimeError, match="bsattn_bwd: d. has the address of"):
+            ops.bsattn_bwd(dout, q, k, v, out, lse, mask, **kw)
+    q, k, dq, dk, new = (t(2, 5, 3, 128) for _ in range(5))
+    for kw in (dict(out_q=k), dict(out_k=q), dict(out_q=new, out_k=new)):
+        with pytest.raises(RuntimeError, match="rope: out_. has the address of"):
+            ops.qk_head_norm_rope(q, k, 1e-6, **kw)
+    for kw in (dict(dq=k), dict(dq=dk), dict(dk=q), dict(dk=dq), dict(dq=new, dk=new)):
+        with pytest.raises(RuntimeError, match="rope_bwd: d. has the address of"):
+            ops.qk_head_norm_rope_bwd(dq, dk, q, k, 1e-6, **kw)
+    q, k, dq, dk, new = (t(2, 5, 384) for _ in range(5))
+    for kw in (dict(dq=k), dict(dq=dk), dict(dk=q), dict(dk=dq), dict(dq=new, dk=new)):
+        with pytest.raises(RuntimeError, match="rope_bwd: d. has the address of"):
+            ops.qk_norm_rope_bwd(dq, dk, q, k, 128, 1e-6, **kw)
